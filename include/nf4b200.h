@@ -460,6 +460,95 @@ int nf4b_qkv_attention_ex(const void* qkv, const void* q_norm_w, const void* k_n
                           int max_len, int window, void* workspace, size_t workspace_bytes, int dtype,
                           void* stream);
 
+/*
+ * Paged KV cache: the caches of n_seqs sequences in fixed-size pages of a pool,
+ * so that memory follows the sequences' real lengths, for a batch of streams
+ * that decode together. No counterpart in the reference, whose cache is one
+ * dense (1, n_kv, max_len, 128) buffer of one stream
+ * (app/engine/fusedlayer.py:212-269).
+ *   k, v         [n_pages, n_kv, page_size, 128], bf16 or fp16 (dtype), 16-byte aligned
+ *   block_table  int32 [n_seqs, max_pages]: row r of sequence s is row r % page_size
+ *                of page block_table[s, r / page_size]; an entry outside
+ *                [0, n_pages) is an unassigned page, whose rows take no part
+ *   weight       fp32 [n_pages, n_kv, page_size]: the attention weight each row
+ *                has received, summed over the query heads of its KV head and over
+ *                all tokens since the row was written; NULL where it is not kept
+ *   position     int32 [n_pages, n_kv, page_size]: each row's token position; or NULL
+ * page_size is a multiple of 16, n_seqs at most 4096, n_seqs * n_kv at most 65535
+ * and a sequence's capacity max_pages * page_size below 2^31 rows. int32 and
+ * fp32 arrays are 4-byte aligned. Lengths, rows and tables are read on the device, so a
+ * captured graph serves every state of the cache.
+ */
+typedef struct nf4b_paged_kv {
+  void* k;
+  void* v;
+  const int32_t* block_table;
+  float* weight;
+  int32_t* position;
+  int32_t n_seqs;
+  int32_t max_pages;
+  int32_t n_pages;
+  int32_t n_kv;
+  int32_t page_size;
+  int32_t dtype; /* NF4B_BF16 or NF4B_F16, of q, qkv, norm weights and out too */
+} nf4b_paged_kv;
+
+/*
+ * n_tokens tokens enter their pages: nf4b_qk_rope_kv (optional q/k norm, rotary,
+ * the same rounding points, so rows have the same bits as in a dense cache) for
+ * every token of qkv [n_tokens, n_head + 2 n_kv, 128], with the rotary row
+ * freqs[positions[t]] of a table of freqs_rows rows and the cache row rows[t] of
+ * sequence seqs[t] (seqs NULL: sequence t). Writes q_out [n_tokens, n_head, 128],
+ * the k and v rows, position = positions[t] and weight = 0. Rows and positions
+ * are apart because an eviction leaves a sequence fewer rows than tokens.
+ * A token whose row, sequence or page is out of range writes no cache row; one
+ * whose position is outside [0, freqs_rows) writes none and has q = 0 (padding).
+ * Two tokens of one call must not name the same row. qkv and q_out 16-byte aligned.
+ */
+int nf4b_paged_write(const nf4b_paged_kv* cache, const void* qkv, const int32_t* seqs, const int32_t* rows,
+                     const int32_t* positions, const void* freqs, int freqs_dtype, int freqs_rows,
+                     const void* q_norm_w, const void* k_norm_w, float eps, void* q_out, int n_tokens, int n_head,
+                     void* stream);
+
+/*
+ * Grouped-query attention of one new token of each sequence: q [n_seqs, n_head,
+ * 128] over rows [0, lens[s]) of sequence s (lens is brought into [0, capacity]),
+ * out [n_seqs, n_head, 128] = softmax(scale q k^T) v, one rounding at the end.
+ * Rows whose `mask` byte (uint8 [n_seqs, max_pages * page_size], NULL = all
+ * visible) is 0 take no part, whatever their pages hold. A sequence without a
+ * visible row, or whose scores are all -inf, gets zeros. Query head h reads KV head
+ * h / (n_head / n_kv); up to 16 query heads to a KV head.
+ * With cache->weight every visible row's weight (the sum over the query heads
+ * of its KV head) is added to it, in fp32; a page that several sequences share
+ * receives all of theirs, in no fixed order. Otherwise results do not depend on
+ * timing. `workspace` (nf4b_paged_attention_workspace_size, tracked = whether
+ * weight is given) is zeroed once before its first use and serves calls of any
+ * sizes that fit it; calls that overlap on the GPU must not share one.
+ */
+int nf4b_paged_attention(const nf4b_paged_kv* cache, const void* q, const int32_t* lens, const uint8_t* mask,
+                         float scale, void* out, int n_head, void* workspace, size_t workspace_bytes, void* stream);
+
+size_t nf4b_paged_attention_workspace_size(int n_seqs, int n_head, int n_kv, int max_pages, int page_size,
+                                           int tracked);
+
+/*
+ * Eviction by accumulated attention weight, in place: of each sequence and KV
+ * head min(lens[s], budget) rows stay. First the protected ones: token position
+ * below `sink`, or among the `recent` newest positions of that head's rows. Then those
+ * with the greatest weight (NaN counts as -inf), equal ones by rising row. Rows that stay and
+ * lie at or past the budget move, in order, into the rows below it that do not
+ * stay; nothing else moves (attention does not depend on the order of rows), so
+ * rows [0, lens_out[s]) hold the sequence and later pages are free. weight_out, position_out and
+ * lens_out receive those rows' weights and positions and the new lengths; each may be
+ * its input. Needs weight and position, budget >= 1, sink + recent <= budget,
+ * and pages that no other sequence shares. The workspace needs no initial value.
+ */
+int nf4b_paged_evict(const nf4b_paged_kv* cache, const int32_t* lens, int budget, int recent, int sink,
+                     float* weight_out, int32_t* position_out, int32_t* lens_out, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+size_t nf4b_paged_evict_workspace_size(int n_seqs, int n_kv, int max_pages, int page_size, int budget);
+
 #ifdef __cplusplus
 }
 #endif

@@ -65,6 +65,11 @@ EXPORTS = (
     "nf4b_qk_rope_kv_ex",
     "nf4b_decode_attention_ex",
     "nf4b_qkv_attention_ex",
+    "nf4b_paged_write",
+    "nf4b_paged_attention",
+    "nf4b_paged_attention_workspace_size",
+    "nf4b_paged_evict",
+    "nf4b_paged_evict_workspace_size",
 )
 
 
@@ -115,6 +120,15 @@ class RopeKv(ctypes.Structure):
                 ("n_head", ctypes.c_int), ("n_kv", ctypes.c_int), ("max_len", ctypes.c_int)]
 
 
+class PagedKv(ctypes.Structure):
+    """`nf4b_paged_kv`: a paged KV cache, by pointer."""
+
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("block_table", ctypes.c_void_p),
+                ("weight", ctypes.c_void_p), ("position", ctypes.c_void_p), ("n_seqs", ctypes.c_int32),
+                ("max_pages", ctypes.c_int32), ("n_pages", ctypes.c_int32), ("n_kv", ctypes.c_int32),
+                ("page_size", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
 class Nf4bError(RuntimeError):
     """A non-zero status from the library, with its message."""
 
@@ -129,7 +143,7 @@ _lib = None
 
 def _declare(lib) -> None:
     vp, i32, f32, sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
-    wp = ctypes.POINTER(Nf4Weight)
+    wp, pp = ctypes.POINTER(Nf4Weight), ctypes.POINTER(PagedKv)
     sig = {
         "nf4b_version": (i32, []),
         "nf4b_last_error": (ctypes.c_char_p, []),
@@ -167,6 +181,11 @@ def _declare(lib) -> None:
         "nf4b_decode_attention_ex": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp, sz, i32, vp]),
         "nf4b_qkv_attention_ex": (i32, [vp, vp, vp, f32, vp, i32, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, vp,
                                         sz, i32, vp]),
+        "nf4b_paged_write": (i32, [pp, vp, vp, vp, vp, vp, i32, i32, vp, vp, f32, vp, i32, i32, vp]),
+        "nf4b_paged_attention": (i32, [pp, vp, vp, vp, f32, vp, i32, vp, sz, vp]),
+        "nf4b_paged_attention_workspace_size": (sz, [i32, i32, i32, i32, i32, i32]),
+        "nf4b_paged_evict": (i32, [pp, vp, i32, i32, i32, vp, vp, vp, vp, sz, vp]),
+        "nf4b_paged_evict_workspace_size": (sz, [i32, i32, i32, i32, i32]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

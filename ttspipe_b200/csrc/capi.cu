@@ -982,3 +982,201 @@ int nf4b_qkv_attention_ex(const void* qkv, const void* q_norm_w, const void* k_n
 }
 
 }  // extern "C"
+
+namespace {
+
+// What every call on a paged cache checks of its description.
+int check_paged(const nf4b_paged_kv* c, bool* f16) {
+  if (c == nullptr || c->k == nullptr || c->v == nullptr || c->block_table == nullptr)
+    return fail(NF4B_ERR_ARG, "paged cache, its pools or its block table are null");
+  if (int e = elem_type(c->dtype, f16)) return e;
+  if (c->n_seqs <= 0 || c->n_seqs > PAGED_MAX_SEQS)
+    return fail(NF4B_ERR_SHAPE, "%d sequences outside [1, %d]", c->n_seqs, PAGED_MAX_SEQS);
+  if (c->n_kv <= 0 || (long long)c->n_seqs * c->n_kv > PAGED_MAX_LISTS)
+    return fail(NF4B_ERR_SHAPE, "%d KV heads of %d sequences (at most %d in all)", c->n_kv, c->n_seqs,
+                PAGED_MAX_LISTS);
+  if (c->page_size <= 0 || c->page_size % PAGED_TILE)
+    return fail(NF4B_ERR_SHAPE, "page size %d is not a multiple of %d", c->page_size, PAGED_TILE);
+  if (c->n_pages <= 0 || c->max_pages <= 0 || (long long)c->max_pages * c->page_size >= (1LL << 31) ||
+      (long long)c->n_seqs * c->n_kv * c->max_pages * (c->page_size / PAGED_TILE) >= (1LL << 31))
+    return fail(NF4B_ERR_SHAPE, "%d pages, %d of %d rows for each sequence", c->n_pages, c->max_pages, c->page_size);
+  if (!aligned(c->k, 16) || !aligned(c->v, 16)) return fail(NF4B_ERR_ALIGN, "pools not 16-byte aligned");
+  if (!aligned(c->block_table, 4) || !aligned(c->weight, 4) || !aligned(c->position, 4))
+    return fail(NF4B_ERR_ALIGN, "block table, weights or positions not 4-byte aligned");
+  return NF4B_OK;
+}
+
+int check_paged_heads(int n_head, int n_kv) {
+  if (n_head <= 0 || n_head % n_kv) return fail(NF4B_ERR_SHAPE, "n_head %d is not a multiple of n_kv %d", n_head, n_kv);
+  if (n_head / n_kv > PAGED_MAX_GROUPS)
+    return fail(NF4B_ERR_SHAPE, "%d query heads to a KV head (at most %d)", n_head / n_kv, PAGED_MAX_GROUPS);
+  return NF4B_OK;
+}
+
+int check_workspace(const void* workspace, size_t given, size_t need) {
+  if (workspace == nullptr || given < need)
+    return fail(NF4B_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace ? given : (size_t)0);
+  if (!aligned(workspace, 256)) return fail(NF4B_ERR_ALIGN, "workspace is not 256-byte aligned");
+  return NF4B_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int nf4b_paged_write(const nf4b_paged_kv* cache, const void* qkv, const int32_t* seqs, const int32_t* rows,
+                     const int32_t* positions, const void* freqs, int freqs_dtype, int freqs_rows,
+                     const void* q_norm_w, const void* k_norm_w, float eps, void* q_out, int n_tokens, int n_head,
+                     void* stream) {
+  bool f16 = false;
+  int st = check_paged(cache, &f16);
+  if (st) return st;
+  if (!qkv || !rows || !positions || !freqs || !q_out) return fail(NF4B_ERR_ARG, "null pointer");
+  if ((q_norm_w == nullptr) != (k_norm_w == nullptr))
+    return fail(NF4B_ERR_ARG, "q and k norm weights must both be given or both be null");
+  if (q_norm_w != nullptr && !(eps >= 0.f)) return fail(NF4B_ERR_ARG, "eps must be >= 0");
+  if (freqs_dtype < NF4B_F32 || freqs_dtype > NF4B_BF16)
+    return fail(NF4B_ERR_DTYPE, "unknown freqs dtype %d", freqs_dtype);
+  if (n_head <= 0 || n_head % cache->n_kv)
+    return fail(NF4B_ERR_SHAPE, "n_head %d is not a multiple of n_kv %d", n_head, cache->n_kv);
+  if (n_tokens <= 0 || freqs_rows <= 0)
+    return fail(NF4B_ERR_SHAPE, "%d tokens, rotary table of %d rows", n_tokens, freqs_rows);
+  if (seqs == nullptr && n_tokens > cache->n_seqs)
+    return fail(NF4B_ERR_SHAPE, "%d tokens of %d sequences need seqs", n_tokens, cache->n_seqs);
+  if (!aligned(qkv, 16) || !aligned(q_out, 16)) return fail(NF4B_ERR_ALIGN, "qkv / q_out not 16-byte aligned");
+  if (!aligned(q_norm_w, 2) || !aligned(k_norm_w, 2) || !aligned(seqs, 4) || !aligned(rows, 4) ||
+      !aligned(positions, 4) || !freqs_aligned(freqs, freqs_dtype))
+    return fail(NF4B_ERR_ALIGN, "norm weights, sequences, rows, positions or freqs misaligned");
+  if ((st = check_device())) return st;
+  PagedWriteParams p;
+  p.qkv = static_cast<const uint16_t*>(qkv);
+  p.seqs = seqs;
+  p.rows = rows;
+  p.positions = positions;
+  p.freqs = freqs;
+  p.ftype = freqs_dtype;
+  p.freqs_rows = freqs_rows;
+  p.qw = static_cast<const uint16_t*>(q_norm_w);
+  p.kw = static_cast<const uint16_t*>(k_norm_w);
+  p.eps = eps;
+  p.q_out = static_cast<uint16_t*>(q_out);
+  p.k = static_cast<uint16_t*>(cache->k);
+  p.v = static_cast<uint16_t*>(cache->v);
+  p.table = cache->block_table;
+  p.weight = cache->weight;
+  p.position = cache->position;
+  p.n_tokens = n_tokens;
+  p.n_head = n_head;
+  p.n_kv = cache->n_kv;
+  p.page_size = cache->page_size;
+  p.max_pages = cache->max_pages;
+  p.n_pages = cache->n_pages;
+  p.n_seqs = cache->n_seqs;
+  return launch_status(launch_paged_write(p, current_sm_count(), f16, reinterpret_cast<cudaStream_t>(stream)),
+                       "paged write launch");
+}
+
+size_t nf4b_paged_attention_workspace_size(int n_seqs, int n_head, int n_kv, int max_pages, int page_size,
+                                           int tracked) {
+  if (n_seqs <= 0 || n_kv <= 0 || n_head <= 0 || n_head % n_kv || max_pages <= 0 || page_size <= 0) return 0;
+  PagedAttnPlan plan;
+  paged_attention_plan(n_seqs, n_head, n_kv, (long long)max_pages * page_size, tracked != 0, current_sm_count(),
+                       &plan);
+  return plan.bytes;
+}
+
+int nf4b_paged_attention(const nf4b_paged_kv* cache, const void* q, const int32_t* lens, const uint8_t* mask,
+                         float scale, void* out, int n_head, void* workspace, size_t workspace_bytes, void* stream) {
+  bool f16 = false;
+  int st = check_paged(cache, &f16);
+  if (st) return st;
+  if (!q || !lens || !out) return fail(NF4B_ERR_ARG, "null pointer");
+  if (!(scale - scale == 0.f)) return fail(NF4B_ERR_ARG, "scale %g is not finite", scale);
+  if ((st = check_paged_heads(n_head, cache->n_kv))) return st;
+  if (!aligned(q, 16) || !aligned(out, 16)) return fail(NF4B_ERR_ALIGN, "q / out not 16-byte aligned");
+  if (!aligned(lens, 4)) return fail(NF4B_ERR_ALIGN, "lens not 4-byte aligned");
+  PagedAttnPlan plan;
+  const int sms = current_sm_count();
+  paged_attention_plan(cache->n_seqs, n_head, cache->n_kv, (long long)cache->max_pages * cache->page_size,
+                       cache->weight != nullptr, sms, &plan);
+  if ((st = check_workspace(workspace, workspace_bytes, plan.bytes))) return st;
+  if ((st = check_device())) return st;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  PagedAttnParams p;
+  p.q = static_cast<const uint16_t*>(q);
+  p.k = static_cast<const uint16_t*>(cache->k);
+  p.v = static_cast<const uint16_t*>(cache->v);
+  p.table = cache->block_table;
+  p.lens = lens;
+  p.mask = mask;
+  p.out = static_cast<uint16_t*>(out);
+  p.scale_log2 = (float)((double)scale * 1.4426950408889634);
+  p.n_seqs = cache->n_seqs;
+  p.n_head = n_head;
+  p.n_kv = cache->n_kv;
+  p.groups = n_head / cache->n_kv;
+  p.page_size = cache->page_size;
+  p.max_pages = cache->max_pages;
+  p.n_pages = cache->n_pages;
+  p.counters = reinterpret_cast<int*>(ws);
+  p.part_o = reinterpret_cast<float*>(ws + plan.part_o);
+  p.part_ml = reinterpret_cast<float2*>(ws + plan.part_ml);
+  p.lse = cache->weight ? reinterpret_cast<float*>(ws + plan.lse) : nullptr;
+  p.scores = cache->weight ? reinterpret_cast<float*>(ws + plan.scores) : nullptr;
+  p.weight = cache->weight;
+  return launch_status(launch_paged_attention(p, plan.grid, sms, f16, reinterpret_cast<cudaStream_t>(stream)),
+                       "paged attention launch");
+}
+
+size_t nf4b_paged_evict_workspace_size(int n_seqs, int n_kv, int max_pages, int page_size, int budget) {
+  if (n_seqs <= 0 || n_kv <= 0 || max_pages <= 0 || page_size <= 0 || budget <= 0) return 0;
+  PagedEvictPlan plan;
+  paged_evict_plan(n_seqs, n_kv, (long long)max_pages * page_size, budget, &plan);
+  return plan.bytes;
+}
+
+int nf4b_paged_evict(const nf4b_paged_kv* cache, const int32_t* lens, int budget, int recent, int sink,
+                     float* weight_out, int32_t* position_out, int32_t* lens_out, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  bool f16 = false;
+  int st = check_paged(cache, &f16);
+  if (st) return st;
+  if (!cache->weight || !cache->position) return fail(NF4B_ERR_ARG, "eviction needs the cache's weights and positions");
+  if (!lens || !weight_out || !position_out || !lens_out) return fail(NF4B_ERR_ARG, "null pointer");
+  if (budget < 1 || recent < 0 || sink < 0 || (long long)recent + sink > budget)
+    return fail(NF4B_ERR_ARG, "budget %d of which %d recent and %d first rows are protected", budget, recent, sink);
+  if (!aligned(lens, 4) || !aligned(weight_out, 4) || !aligned(position_out, 4) || !aligned(lens_out, 4))
+    return fail(NF4B_ERR_ALIGN, "lens, weight_out, position_out or lens_out not 4-byte aligned");
+  PagedEvictPlan plan;
+  paged_evict_plan(cache->n_seqs, cache->n_kv, (long long)cache->max_pages * cache->page_size, budget, &plan);
+  if ((st = check_workspace(workspace, workspace_bytes, plan.bytes))) return st;
+  if ((st = check_device())) return st;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  PagedEvictParams p;
+  p.k = static_cast<uint16_t*>(cache->k);
+  p.v = static_cast<uint16_t*>(cache->v);
+  p.table = cache->block_table;
+  p.lens = lens;
+  p.weight = cache->weight;
+  p.position = cache->position;
+  p.weight_out = weight_out;
+  p.position_out = position_out;
+  p.lens_out = lens_out;
+  p.budget = budget;
+  p.recent = recent;
+  p.sink = sink;
+  p.n_seqs = cache->n_seqs;
+  p.n_kv = cache->n_kv;
+  p.page_size = cache->page_size;
+  p.max_pages = cache->max_pages;
+  p.n_pages = cache->n_pages;
+  p.count = reinterpret_cast<int*>(ws);
+  p.left = reinterpret_cast<int*>(ws + plan.left);
+  p.to = reinterpret_cast<int32_t*>(ws + plan.to);
+  p.src = reinterpret_cast<int32_t*>(ws + plan.src);
+  p.max_moves = plan.max_moves;
+  return launch_status(launch_paged_evict(p, current_sm_count(), reinterpret_cast<cudaStream_t>(stream)),
+                       "paged evict launch");
+}
+
+}  // extern "C"

@@ -386,4 +386,84 @@ cudaError_t launch_qkv_attention(const QkvIn& in, const int64_t* pos, uint16_t* 
                                  uint16_t* vc, uint16_t* out, int nh, int nkv, int max_len, int window,
                                  float* partial, int* counters, cudaStream_t stream, bool f16 = false);
 
+// ---- paged KV cache (paged_attention.cu, paged_kv.cu) ------------------------
+
+constexpr int PAGED_TILE = 16;        // rows of one unit of attention work; page sizes are multiples of it
+constexpr int PAGED_MIN_TILES = 8;    // tiles of one CTA's part, where there are that many
+constexpr int PAGED_MAX_SEQS = 4096;  // sequences of one call (their tile counts lie in shared memory)
+constexpr int PAGED_MAX_GROUPS = 16;
+constexpr int PAGED_MAX_LISTS = 65535;  // (sequence, KV head) pairs of one call
+// The workspace's counters, at its start whatever the call's sizes: zero between calls of any sizes.
+constexpr size_t PAGED_COUNTER_BYTES = 65536 * sizeof(int);
+
+struct PagedAttnParams {
+  const uint16_t* q;     // [n_seqs, n_head, 128]
+  const uint16_t* k;     // [n_pages, n_kv, page_size, 128]
+  const uint16_t* v;
+  const int32_t* table;  // [n_seqs, max_pages]
+  const int32_t* lens;   // [n_seqs]
+  const uint8_t* mask;   // [n_seqs, max_pages * page_size] or null
+  uint16_t* out;         // [n_seqs, n_head, 128]
+  float scale_log2;      // scale * log2(e)
+  int n_seqs, n_head, n_kv, groups, page_size, max_pages, n_pages;
+  int* counters;    // [n_seqs, n_kv], zero between calls
+  float* part_o;    // [2 grid, groups, 128]
+  float2* part_ml;  // [2 grid, groups]
+  float* lse;       // [n_seqs, n_head], log2; null without weight
+  float* scores;    // [tiles, groups, 16], log2; null without weight
+  float* weight;    // [n_pages, n_kv, page_size] or null
+};
+struct PagedAttnPlan {
+  int grid;
+  size_t part_o, part_ml, lse, scores, bytes;  // offsets in the workspace and its size
+};
+void paged_attention_plan(int n_seqs, int n_head, int n_kv, long long max_rows, bool tracked, int sms,
+                          PagedAttnPlan* plan);
+cudaError_t launch_paged_attention(const PagedAttnParams& p, int grid, int sms, bool f16, cudaStream_t stream);
+
+struct PagedWriteParams {
+  const uint16_t* qkv;  // [n_tokens, n_head + 2 n_kv, 128]
+  const int32_t* seqs;  // [n_tokens] or null: token t is sequence t's
+  const int32_t* rows;
+  const int32_t* positions;
+  const void* freqs;  // [freqs_rows, 64, 2]
+  int ftype, freqs_rows;
+  const uint16_t* qw;  // [128] or null
+  const uint16_t* kw;
+  float eps;
+  uint16_t* q_out;  // [n_tokens, n_head, 128]
+  uint16_t* k;
+  uint16_t* v;
+  const int32_t* table;
+  float* weight;      // or null
+  int32_t* position;  // or null
+  int n_tokens, n_head, n_kv, page_size, max_pages, n_pages, n_seqs;
+};
+cudaError_t launch_paged_write(const PagedWriteParams& p, int sms, bool f16, cudaStream_t stream);
+
+struct PagedEvictParams {
+  uint16_t* k;
+  uint16_t* v;
+  const int32_t* table;
+  const int32_t* lens;
+  const float* weight;
+  const int32_t* position;
+  float* weight_out;
+  int32_t* position_out;
+  int32_t* lens_out;
+  int budget, recent, sink;
+  int n_seqs, n_kv, page_size, max_pages, n_pages;
+  int* count;    // [n_seqs, n_kv] moves
+  int* left;     // [n_seqs] rows left
+  int32_t* to;   // [n_seqs, n_kv, max_moves] rows that are overwritten
+  int32_t* src;  // [n_seqs, n_kv, max_moves] rows that move there
+  int max_moves;
+};
+struct PagedEvictPlan {
+  size_t left, to, src, bytes;
+  int max_moves;
+};
+void paged_evict_plan(int n_seqs, int n_kv, long long max_rows, int budget, PagedEvictPlan* plan);
+cudaError_t launch_paged_evict(const PagedEvictParams& p, int sms, cudaStream_t stream);
+
 }  // namespace nf4b

@@ -1,0 +1,478 @@
+// Decode attention over a paged KV cache: one new token of each of n_seqs
+// sequences against its own pages, with the rows' attention weights accumulated
+// for a later eviction.
+//
+// Mathematics. Query head g of sequence b reads KV head h = g / groups. Over the
+// rows j < lens[b] that take part (the mask's byte is not 0, the row's page is
+// assigned)
+//     s_j = scale * (q_g . k_j),  m = max s_j,  l = sum exp(s_j - m),
+//     out_g = sum exp(s_j - m) v_j / l,
+//     weight[h][j] += sum over the group's heads of exp(s_j - m) / l.
+// A sequence without such a row (or whose scores are all -inf) gets zeros and adds
+// nothing. Scores are kept in units of log2 (scale * log2 e folded in after the
+// product), products and sums in fp32.
+//
+// Work split. The unit of work is a tile of 16 rows of one (sequence, KV head):
+// page sizes are multiples of 16, so a tile lies in one page. All tiles of all
+// sequences and heads, in that order, are one line that is cut into equal parts,
+// one for each CTA, from the lengths on the device: ragged batches balance, and one
+// captured graph serves every length. A (sequence, head) that lies in one CTA's
+// part is finished there; one that several CTAs share is joined by the CTA that
+// finishes it last (a counter of each (sequence, head), back at 0 afterwards), in
+// the order of the parts, so results do not depend on timing.
+
+#include "common.cuh"
+#include "gemv_unit.cuh"
+#include "kernels.cuh"
+
+namespace nf4b {
+
+namespace {
+
+constexpr int kD = 128;
+constexpr int kTile = PAGED_TILE;
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Tiles of a sequence: its length is brought into [0, capacity].
+__device__ __forceinline__ int seq_rows(const PagedAttnParams& p, int b) {
+  const int n = p.lens[b];
+  const int cap = p.max_pages * p.page_size;
+  return n < 0 ? 0 : n > cap ? cap : n;
+}
+
+// pre[b] = tiles of all (sequence < b, head); pre[n_seqs] the total. Ends with a barrier.
+__device__ __forceinline__ void tile_prefix(const PagedAttnParams& p, int* pre) {
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    int base = 0;
+    for (int b0 = 0; b0 < p.n_seqs; b0 += 32) {
+      const int b = b0 + lane;
+      int t = b < p.n_seqs ? (seq_rows(p, b) + kTile - 1) / kTile * p.n_kv : 0;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, t, off);
+        if (lane >= off) t += o;
+      }
+      if (b < p.n_seqs) pre[b + 1] = base + t;
+      base += __shfl_sync(0xffffffffu, t, 31);
+    }
+    if (lane == 0) pre[0] = 0;
+  }
+  __syncthreads();
+}
+
+// The sequence of tile u: the last b with pre[b] <= u.
+__device__ __forceinline__ int seq_of(const int* pre, int n_seqs, int u) {
+  int lo = 0, hi = n_seqs - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (pre[mid] <= u)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+
+// One (sequence, head) part's running state in a warp. NT: tiles of eight query
+// heads (groups <= 8: one, else two). o is O^T from the MMA: o[nt][j][.] holds
+// dimensions d = (j / 4) * 64 + (lane / 4) * 8 + 2 (j % 4) + {0, 1} of heads
+// 8 nt + 2 (lane % 4) + {0, 1}: [0] (d, head), [1] (d, head + 1), [2] (d + 1, head),
+// [3] (d + 1, head + 1). m and l belong to head 8 nt + lane / 4; l is this lane's
+// share of the sum. o and l are both kept times 2^kLift.
+//
+// The weights exp(s - m) enter the second product in 16 bits. Rounded once, each
+// would be off by as much as the output's own rounding; so they enter twice, as the
+// rounded value and as what rounding left (the MMA units idle otherwise: memory bounds
+// this kernel), which leaves 2^-17. fp16 has no exponents for the small weights of
+// many rows next to one large one, so there they are lifted by 2^14 (exact).
+template <bool F16>
+constexpr float kLift = F16 ? 14.f : 0.f;
+
+template <int NT>
+struct WarpState {
+  float o[NT][8][4];
+  float m[NT], l[NT];
+};
+
+// kFloats of shared memory after the prefix: the warps' outputs, or the joining
+// CTA's factors of each part.
+template <int NT>
+struct AttnShared {
+  float o[kWarps][NT * 8][kD];
+  float m[kWarps][NT * 8], l[kWarps][NT * 8];
+  float M[NT * 8], L[NT * 8];
+  int last;
+};
+
+template <int NT, bool F16>
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
+    paged_attention_kernel(const __grid_constant__ PagedAttnParams p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  AttnShared<NT>& sm = *reinterpret_cast<AttnShared<NT>*>(smem);
+  int* pre = reinterpret_cast<int*>(smem + sizeof(AttnShared<NT>));
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int G = p.groups;
+
+  pdl_wait();  // q, the new rows and the lengths come from earlier kernels
+  tile_prefix(p, pre);
+  for (int b = blockIdx.x; b < p.n_seqs; b += gridDim.x)
+    if (pre[b + 1] == pre[b])
+      for (int i = tid; i < p.n_head * kD; i += kThreads) p.out[(size_t)b * p.n_head * kD + i] = 0;
+  const int U = pre[p.n_seqs];
+  const int N = min((int)gridDim.x, (U + PAGED_MIN_TILES - 1) / PAGED_MIN_TILES);
+  const int c = blockIdx.x;
+  if (c >= N) return;
+  int u = (int)((long long)c * U / N);
+  const int u1 = (int)((long long)(c + 1) * U / N);
+  const int tpp = p.page_size / kTile;
+  int b = seq_of(pre, p.n_seqs, u);
+
+  while (u < u1) {
+    while (pre[b + 1] <= u) ++b;
+    const int T = (pre[b + 1] - pre[b]) / p.n_kv;
+    const int h = (u - pre[b]) / T, t0 = (u - pre[b]) - h * T;
+    const int t1 = min(T, t0 + (u1 - u));
+    const int rows = seq_rows(p, b);
+    const int* table = p.table + (size_t)b * p.max_pages;
+    const uint8_t* mask = p.mask == nullptr ? nullptr : p.mask + (size_t)b * p.max_pages * p.page_size;
+    float* scores = p.scores == nullptr ? nullptr : p.scores + (size_t)(u - t0) * G * kTile;
+
+    // the group's queries as the A operand, dimensions in the order in which a
+    // lane reads a key row: 16-byte pieces c * 4 + t
+    uint4 qa[NT][2][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const int head = nt * 8 + g;
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc) qa[nt][hf][cc] = make_uint4(0, 0, 0, 0);
+        if (hf == 0 && head < G) {
+          const uint4* qr =
+              reinterpret_cast<const uint4*>(p.q + ((size_t)b * p.n_head + (size_t)h * G + head) * kD);
+#pragma unroll
+          for (int cc = 0; cc < 4; ++cc) qa[nt][0][cc] = qr[cc * 4 + t];
+        }
+      }
+
+    WarpState<NT> s;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      s.m[nt] = -INFINITY;
+      s.l[nt] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s.o[nt][j][i] = 0.f;
+    }
+
+    for (int tile = t0 + warp; tile < t1; tile += kWarps) {
+      const int pg = table[tile / tpp];
+      const bool assigned = pg >= 0 && pg < p.n_pages;
+      const size_t row0 = ((size_t)(assigned ? pg : 0) * p.n_kv + h) * p.page_size + (size_t)(tile % tpp) * kTile;
+      uint4 kr[2][4], vr[4][2];
+      const uint4* kp = reinterpret_cast<const uint4*>(p.k + row0 * kD);
+      const uint4* vp = reinterpret_cast<const uint4*>(p.v + row0 * kD);
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc) kr[n][cc] = ld_stream_u4(kp + (n * 8 + g) * 16 + cc * 4 + t);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh)
+          vr[r][hh] = ld_stream_u4(vp + (2 * t + (r & 1) + (r >> 1) * 8) * 16 + hh * 8 + g);
+      // the lane's four rows 2t, 2t + 1, 8 + 2t, 9 + 2t: which take part
+      bool see[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int j = tile * kTile + 2 * t + (r & 1) + (r >> 1) * 8;
+        see[r] = assigned && j < rows && (mask == nullptr || mask[j] != 0);
+        if (!see[r]) vr[r][0] = vr[r][1] = make_uint4(0, 0, 0, 0);  // 0 * NaN of an unwritten row is NaN
+      }
+      float sc[2][4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[n][i] = 0.f;
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc) {
+          if (NT == 1) {
+            mma_act<F16>(sc[n], qa[0][0][cc].x, 0u, qa[0][0][cc].y, 0u, kr[n][cc].x, kr[n][cc].y);
+            mma_act<F16>(sc[n], qa[0][0][cc].z, 0u, qa[0][0][cc].w, 0u, kr[n][cc].z, kr[n][cc].w);
+          } else {
+            mma_act<F16>(sc[n], qa[0][0][cc].x, qa[NT - 1][0][cc].x, qa[0][0][cc].y, qa[NT - 1][0][cc].y, kr[n][cc].x,
+                         kr[n][cc].y);
+            mma_act<F16>(sc[n], qa[0][0][cc].z, qa[NT - 1][0][cc].z, qa[0][0][cc].w, qa[NT - 1][0][cc].w, kr[n][cc].z,
+                         kr[n][cc].w);
+          }
+        }
+      }
+      uint32_t ph[NT][2], pl[NT][2];  // P^T as the B operand: the rounded weights and what rounding left
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float x[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = see[r] ? sc[r >> 1][nt * 2 + (r & 1)] * p.scale_log2 : -INFINITY;
+        if (scores != nullptr && nt * 8 + g < G) {
+          float* sp = scores + ((size_t)tile * G + nt * 8 + g) * kTile + 2 * t;
+          *reinterpret_cast<float2*>(sp) = make_float2(x[0], x[1]);
+          *reinterpret_cast<float2*>(sp + 8) = make_float2(x[2], x[3]);
+        }
+        float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float mnew = fmaxf(s.m[nt], mx);
+        const float mu = mnew == -INFINITY ? 0.f : mnew;
+        if (__any_sync(0xffffffffu, mnew > s.m[nt])) {
+          const float f = exp2_fast(s.m[nt] - mu);
+          const float f0 = __shfl_sync(0xffffffffu, f, 8 * t), f1 = __shfl_sync(0xffffffffu, f, 8 * t + 4);
+          s.l[nt] *= f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            s.o[nt][j][0] *= f0;
+            s.o[nt][j][1] *= f1;
+            s.o[nt][j][2] *= f0;
+            s.o[nt][j][3] *= f1;
+          }
+          s.m[nt] = mnew;
+        }
+        float e[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          e[r] = exp2_fast(x[r] - mu + kLift<F16>);
+          s.l[nt] += e[r];
+        }
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          ph[nt][n] = pack_act2<F16>(e[2 * n], e[2 * n + 1]);
+          pl[nt][n] = pack_act2<F16>(e[2 * n] - act_lo<F16>(ph[nt][n]), e[2 * n + 1] - act_hi<F16>(ph[nt][n]));
+        }
+      }
+#pragma unroll
+      for (int hh = 0; hh < 2; ++hh) {
+        const uint32_t* w0 = &vr[0][hh].x;
+        const uint32_t* w1 = &vr[1][hh].x;
+        const uint32_t* w2 = &vr[2][hh].x;
+        const uint32_t* w3 = &vr[3][hh].x;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t a0 = prmt(w0[w], w1[w], 0x5410u), a1 = prmt(w0[w], w1[w], 0x7632u);
+          const uint32_t a2 = prmt(w2[w], w3[w], 0x5410u), a3 = prmt(w2[w], w3[w], 0x7632u);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma_act<F16>(s.o[nt][hh * 4 + w], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
+            mma_act<F16>(s.o[nt][hh * 4 + w], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
+          }
+        }
+      }
+    }
+
+    // the warps' states into shared memory
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      s.l[nt] += __shfl_xor_sync(0xffffffffu, s.l[nt], 1);
+      s.l[nt] += __shfl_xor_sync(0xffffffffu, s.l[nt], 2);
+      if (t == 0) {
+        sm.m[warp][nt * 8 + g] = s.m[nt];
+        sm.l[warp][nt * 8 + g] = s.l[nt];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int d = (j >> 2) * 64 + g * 8 + (j & 3) * 2;
+        *reinterpret_cast<float2*>(&sm.o[warp][nt * 8 + 2 * t][d]) = make_float2(s.o[nt][j][0], s.o[nt][j][2]);
+        *reinterpret_cast<float2*>(&sm.o[warp][nt * 8 + 2 * t + 1][d]) = make_float2(s.o[nt][j][1], s.o[nt][j][3]);
+      }
+    }
+    __syncthreads();
+    const bool whole = t0 == 0 && t1 == T;
+    const int slot = 2 * c + (t0 == 0 ? 1 : 0);  // a CTA shares at most its first and its last (sequence, head)
+    for (int head = 0; head < G; ++head) {
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm.m[w][head]);
+      const float mu = M == -INFINITY ? 0.f : M;
+      float l = 0.f, o = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float f = exp2_fast(sm.m[w][head] - mu);
+        l = fmaf(f, sm.l[w][head], l);
+        o = fmaf(f, sm.o[w][head][tid], o);
+      }
+      const size_t oh = (size_t)b * p.n_head + (size_t)h * G + head;
+      if (whole) {
+        p.out[oh * kD + tid] = f2act<F16>(l == 0.f ? 0.f : o / l);
+        if (tid == 0 && p.lse != nullptr) p.lse[oh] = l == 0.f ? -INFINITY : mu + log2f(l) - kLift<F16>;
+      } else {
+        p.part_o[((size_t)slot * G + head) * kD + tid] = o;
+        if (tid == 0) p.part_ml[(size_t)slot * G + head] = make_float2(M, l);
+      }
+    }
+    if (!whole) {
+      // join: the CTAs whose parts hold this (sequence, head), first to last
+      const int s0 = u - t0;
+      const int c0 = (int)(((long long)(s0 + 1) * N - 1) / U), c1 = (int)(((long long)(s0 + T) * N - 1) / U);
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) sm.last = atomicAdd(&p.counters[b * p.n_kv + h], 1) == c1 - c0;
+      __syncthreads();
+      if (sm.last) {
+        __threadfence();
+        if (tid == 0) p.counters[b * p.n_kv + h] = 0;
+        for (int head = warp; head < G; head += kWarps) {
+          float M = -INFINITY;
+          for (int q = c0 + lane; q <= c1; q += 32) {
+            const float2 ml = __ldcg(&p.part_ml[(size_t)(2 * q + (q == c0 ? 1 : 0)) * G + head]);
+            M = fmaxf(M, ml.x);
+          }
+#pragma unroll
+          for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+          float l = 0.f;
+          for (int q = c0 + lane; q <= c1; q += 32) {
+            const float2 ml = __ldcg(&p.part_ml[(size_t)(2 * q + (q == c0 ? 1 : 0)) * G + head]);
+            l += exp2_fast(ml.x - (M == -INFINITY ? 0.f : M)) * ml.y;
+          }
+#pragma unroll
+          for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+          if (lane == 0) {
+            sm.M[head] = M == -INFINITY ? 0.f : M;
+            sm.L[head] = l;
+            if (p.lse != nullptr)
+              p.lse[(size_t)b * p.n_head + (size_t)h * G + head] = l == 0.f ? -INFINITY : sm.M[head] + log2f(l) - kLift<F16>;
+          }
+        }
+        __syncthreads();
+        for (int head = 0; head < G; ++head) {
+          float o = 0.f;
+          for (int q = c0; q <= c1; ++q) {
+            const size_t sl = (size_t)(2 * q + (q == c0 ? 1 : 0)) * G + head;
+            o = fmaf(exp2_fast(__ldcg(&p.part_ml[sl]).x - sm.M[head]), __ldcg(&p.part_o[sl * kD + tid]), o);
+          }
+          p.out[((size_t)b * p.n_head + (size_t)h * G + head) * kD + tid] =
+              f2act<F16>(sm.L[head] == 0.f ? 0.f : o / sm.L[head]);
+        }
+      }
+    }
+    __syncthreads();  // the shared state is free again
+    u += t1 - t0;
+  }
+  pdl_launch_dependents();
+}
+
+// weight[row] += sum over the group's heads of 2^(score - lse), from the scores the
+// attention kernel left. One thread a row; a reduction instruction instead of a read
+// and a write, so that sequences which share a page add up.
+constexpr int kWThreads = 256;
+
+__global__ void __launch_bounds__(kWThreads) paged_weight_kernel(const __grid_constant__ PagedAttnParams p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  int* pre = reinterpret_cast<int*>(smem);
+  pdl_wait();
+  tile_prefix(p, pre);
+  const int U = pre[p.n_seqs], tpp = p.page_size / kTile, G = p.groups;
+  const int i = threadIdx.x % kTile;
+  for (long long uu = (long long)blockIdx.x * (kWThreads / kTile) + threadIdx.x / kTile; uu < U;
+       uu += (long long)gridDim.x * (kWThreads / kTile)) {
+    const int u = (int)uu;
+    const int b = seq_of(pre, p.n_seqs, u);
+    const int T = (pre[b + 1] - pre[b]) / p.n_kv;
+    const int h = (u - pre[b]) / T, tile = (u - pre[b]) - h * T;
+    const int pg = p.table[(size_t)b * p.max_pages + tile / tpp];
+    if (pg < 0 || pg >= p.n_pages || tile * kTile + i >= seq_rows(p, b)) continue;
+    const float* lse = p.lse + (size_t)b * p.n_head + (size_t)h * G;
+    const float* sp = p.scores + (size_t)u * G * kTile + i;
+    float w = 0.f;
+    for (int head = 0; head < G; ++head) {
+      const float L = lse[head];
+      w += L == -INFINITY ? 0.f : exp2_fast(sp[head * kTile] - L);
+    }
+    atomicAdd(p.weight + ((size_t)pg * p.n_kv + h) * p.page_size + (size_t)(tile % tpp) * kTile + i, w);
+  }
+  pdl_launch_dependents();
+}
+
+template <typename K>
+cudaError_t launch(K kernel, int grid, int threads, size_t smem, const PagedAttnParams& p, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <int NT, bool F16>
+cudaError_t launch_attention(const PagedAttnParams& p, int grid, cudaStream_t stream) {
+  const size_t smem = sizeof(AttnShared<NT>) + (size_t)(p.n_seqs + 1) * sizeof(int);
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!configured[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(paged_attention_kernel<NT, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)(sizeof(AttnShared<NT>) + (PAGED_MAX_SEQS + 1) * sizeof(int)));
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
+  }
+  return launch(paged_attention_kernel<NT, F16>, grid, kThreads, smem, p, stream);
+}
+
+long long most_tiles(int n_seqs, int n_kv, long long max_rows) {
+  return (long long)n_seqs * n_kv * ((max_rows + kTile - 1) / kTile);
+}
+
+int grid_for(long long tiles, int groups, int sms) {
+  const long long n = (tiles + PAGED_MIN_TILES - 1) / PAGED_MIN_TILES, most = (long long)sms * (groups <= 8 ? 3 : 2);
+  return (int)(n < most ? n : most);
+}
+
+size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+}  // namespace
+
+void paged_attention_plan(int n_seqs, int n_head, int n_kv, long long max_rows, bool tracked, int sms,
+                          PagedAttnPlan* plan) {
+  const long long tiles = most_tiles(n_seqs, n_kv, max_rows);
+  const int groups = n_head / n_kv;
+  plan->grid = grid_for(tiles, groups, sms);
+  size_t at = PAGED_COUNTER_BYTES;
+  plan->part_o = at;
+  at += up256((size_t)2 * plan->grid * groups * kD * sizeof(float));
+  plan->part_ml = at;
+  at += up256((size_t)2 * plan->grid * groups * sizeof(float2));
+  plan->lse = plan->scores = at;
+  if (tracked) {
+    at += up256((size_t)n_seqs * n_head * sizeof(float));
+    plan->scores = at;
+    at += up256((size_t)tiles * kTile * groups * sizeof(float));
+  }
+  plan->bytes = at;
+}
+
+cudaError_t launch_paged_attention(const PagedAttnParams& p, int grid, int sms, bool f16, cudaStream_t stream) {
+  cudaError_t e;
+  if (p.groups <= 8)
+    e = f16 ? launch_attention<1, true>(p, grid, stream) : launch_attention<1, false>(p, grid, stream);
+  else
+    e = f16 ? launch_attention<2, true>(p, grid, stream) : launch_attention<2, false>(p, grid, stream);
+  if (e != cudaSuccess || p.weight == nullptr) return e;
+  const long long tiles = most_tiles(p.n_seqs, p.n_kv, (long long)p.max_pages * p.page_size);
+  const long long n = (tiles + kWThreads / kTile - 1) / (kWThreads / kTile);
+  return launch(paged_weight_kernel, (int)(n < 8LL * sms ? n : 8LL * sms), kWThreads,
+                (size_t)(p.n_seqs + 1) * sizeof(int), p, stream);
+}
+
+}  // namespace nf4b
