@@ -68,6 +68,13 @@ __device__ __forceinline__ void tile_prefix(const PagedAttnParams& p, int* pre) 
   __syncthreads();
 }
 
+// The number of parts: as many CTAs as there are, but PAGED_MIN_TILES tiles for each unless that puts
+// several (sequence, head)s into one part while CTAs are left.
+__device__ __forceinline__ int parts(const PagedAttnParams& p, int tiles, int ctas) {
+  const int by_tiles = (tiles + PAGED_MIN_TILES - 1) / PAGED_MIN_TILES;
+  return min(ctas, max(by_tiles, min(p.n_seqs * p.n_kv, tiles)));
+}
+
 // The sequence of tile u: the last b with pre[b] <= u.
 __device__ __forceinline__ int seq_of(const int* pre, int n_seqs, int u) {
   int lo = 0, hi = n_seqs - 1;
@@ -102,15 +109,23 @@ struct WarpState {
   float m[NT], l[NT];
 };
 
-// kFloats of shared memory after the prefix: the warps' outputs, or the joining
-// CTA's factors of each part.
+// The warps' states of one (sequence, head) part, for the join inside the CTA.
 template <int NT>
 struct AttnShared {
   float o[kWarps][NT * 8][kD];
   float m[kWarps][NT * 8], l[kWarps][NT * 8];
-  float M[NT * 8], L[NT * 8];
   int last;
 };
+
+// The finished row of one query head, four dimensions to a lane.
+template <bool F16>
+__device__ __forceinline__ void store_out(const PagedAttnParams& p, size_t head, int lane, float m, float l,
+                                          const float (&o)[4]) {
+  const float r = l == 0.f ? 0.f : 1.f / l;
+  const uint2 w = l == 0.f ? make_uint2(0, 0) : make_uint2(pack_act2<F16>(o[0] * r, o[1] * r), pack_act2<F16>(o[2] * r, o[3] * r));
+  *reinterpret_cast<uint2*>(p.out + head * kD + lane * 4) = w;
+  if (lane == 0 && p.lse != nullptr) p.lse[head] = l == 0.f ? -INFINITY : m + log2f(l) - kLift<F16>;
+}
 
 template <int NT, bool F16>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
@@ -127,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
     if (pre[b + 1] == pre[b])
       for (int i = tid; i < p.n_head * kD; i += kThreads) p.out[(size_t)b * p.n_head * kD + i] = 0;
   const int U = pre[p.n_seqs];
-  const int N = min((int)gridDim.x, (U + PAGED_MIN_TILES - 1) / PAGED_MIN_TILES);
+  const int N = parts(p, U, (int)gridDim.x);
   const int c = blockIdx.x;
   if (c >= N) return;
   int u = (int)((long long)c * U / N);
@@ -147,21 +162,14 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
 
     // the group's queries as the A operand, dimensions in the order in which a
     // lane reads a key row: 16-byte pieces c * 4 + t
-    uint4 qa[NT][2][4];
+    uint4 qa[NT][4];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt) {
+      const int head = nt * 8 + g;
+      const uint4* qr = reinterpret_cast<const uint4*>(p.q + ((size_t)b * p.n_head + (size_t)h * G + head) * kD);
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const int head = nt * 8 + g;
-#pragma unroll
-        for (int cc = 0; cc < 4; ++cc) qa[nt][hf][cc] = make_uint4(0, 0, 0, 0);
-        if (hf == 0 && head < G) {
-          const uint4* qr =
-              reinterpret_cast<const uint4*>(p.q + ((size_t)b * p.n_head + (size_t)h * G + head) * kD);
-#pragma unroll
-          for (int cc = 0; cc < 4; ++cc) qa[nt][0][cc] = qr[cc * 4 + t];
-        }
-      }
+      for (int cc = 0; cc < 4; ++cc) qa[nt][cc] = head < G ? qr[cc * 4 + t] : make_uint4(0, 0, 0, 0);
+    }
 
     WarpState<NT> s;
 #pragma unroll
@@ -174,29 +182,50 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
         for (int i = 0; i < 4; ++i) s.o[nt][j][i] = 0.f;
     }
 
-    for (int tile = t0 + warp; tile < t1; tile += kWarps) {
-      const int pg = table[tile / tpp];
-      const bool assigned = pg >= 0 && pg < p.n_pages;
-      const size_t row0 = ((size_t)(assigned ? pg : 0) * p.n_kv + h) * p.page_size + (size_t)(tile % tpp) * kTile;
-      uint4 kr[2][4], vr[4][2];
-      const uint4* kp = reinterpret_cast<const uint4*>(p.k + row0 * kD);
-      const uint4* vp = reinterpret_cast<const uint4*>(p.v + row0 * kD);
+    // Keys and values of the next tile are requested as soon as this tile's have been
+    // multiplied, its page is looked up one tile earlier still.
+    uint4 kr[2][4], vr[4][2];
+    int tile = t0 + warp;
+    auto page_of = [&](int at) -> int {
+      const int pg = at < t1 ? table[at / tpp] : 0;
+      return pg < p.n_pages ? pg : -1;
+    };
+    auto row_of = [&](int at, int pg) -> size_t {
+      return (((size_t)max(pg, 0) * p.n_kv + h) * p.page_size + (size_t)(at % tpp) * kTile) * (kD / 8);
+    };
+    auto load_k = [&](size_t row) {
+      const uint4* kp = reinterpret_cast<const uint4*>(p.k) + row;
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int cc = 0; cc < 4; ++cc) kr[n][cc] = ld_stream_u4(kp + (n * 8 + g) * 16 + cc * 4 + t);
+    };
+    auto load_v = [&](size_t row) {
+      const uint4* vp = reinterpret_cast<const uint4*>(p.v) + row;
 #pragma unroll
       for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh)
           vr[r][hh] = ld_stream_u4(vp + (2 * t + (r & 1) + (r >> 1) * 8) * 16 + hh * 8 + g);
+    };
+    int pg = page_of(tile), pg1 = page_of(tile + kWarps);
+    size_t row = row_of(tile, pg);
+    if (tile < t1) {
+      load_k(row);
+      load_v(row);
+    }
+    for (; tile < t1; tile += kWarps) {
+      const int next = tile + kWarps, pg2 = page_of(next + kWarps);
+      row = row_of(next, pg1);
       // the lane's four rows 2t, 2t + 1, 8 + 2t, 9 + 2t: which take part
-      bool see[4];
+      const bool full = pg >= 0 && (tile + 1) * kTile <= rows && mask == nullptr;
+      bool see[4] = {true, true, true, true};
+      if (!full) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int j = tile * kTile + 2 * t + (r & 1) + (r >> 1) * 8;
-        see[r] = assigned && j < rows && (mask == nullptr || mask[j] != 0);
-        if (!see[r]) vr[r][0] = vr[r][1] = make_uint4(0, 0, 0, 0);  // 0 * NaN of an unwritten row is NaN
+        for (int r = 0; r < 4; ++r) {
+          const int j = tile * kTile + 2 * t + (r & 1) + (r >> 1) * 8;
+          see[r] = pg >= 0 && j < rows && (mask == nullptr || mask[j] != 0);
+        }
       }
       float sc[2][4];
 #pragma unroll
@@ -205,17 +234,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
         for (int i = 0; i < 4; ++i) sc[n][i] = 0.f;
 #pragma unroll
         for (int cc = 0; cc < 4; ++cc) {
-          if (NT == 1) {
-            mma_act<F16>(sc[n], qa[0][0][cc].x, 0u, qa[0][0][cc].y, 0u, kr[n][cc].x, kr[n][cc].y);
-            mma_act<F16>(sc[n], qa[0][0][cc].z, 0u, qa[0][0][cc].w, 0u, kr[n][cc].z, kr[n][cc].w);
-          } else {
-            mma_act<F16>(sc[n], qa[0][0][cc].x, qa[NT - 1][0][cc].x, qa[0][0][cc].y, qa[NT - 1][0][cc].y, kr[n][cc].x,
-                         kr[n][cc].y);
-            mma_act<F16>(sc[n], qa[0][0][cc].z, qa[NT - 1][0][cc].z, qa[0][0][cc].w, qa[NT - 1][0][cc].w, kr[n][cc].z,
-                         kr[n][cc].w);
-          }
+          const uint4 q0 = qa[0][cc], q1 = NT == 1 ? make_uint4(0, 0, 0, 0) : qa[NT - 1][cc];
+          mma_act<F16>(sc[n], q0.x, q1.x, q0.y, q1.y, kr[n][cc].x, kr[n][cc].y);
+          mma_act<F16>(sc[n], q0.z, q1.z, q0.w, q1.w, kr[n][cc].z, kr[n][cc].w);
         }
       }
+      if (next < t1) load_k(row);
       uint32_t ph[NT][2], pl[NT][2];  // P^T as the B operand: the rounded weights and what rounding left
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -257,6 +281,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
           pl[nt][n] = pack_act2<F16>(e[2 * n] - act_lo<F16>(ph[nt][n]), e[2 * n + 1] - act_hi<F16>(ph[nt][n]));
         }
       }
+      if (!full) {  // 0 * NaN of an unwritten row is NaN
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (!see[r]) vr[r][0] = vr[r][1] = make_uint4(0, 0, 0, 0);
+      }
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
         const uint32_t* w0 = &vr[0][hh].x;
@@ -274,6 +303,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
           }
         }
       }
+      if (next < t1) load_v(row);
+      pg = pg1;
+      pg1 = pg2;
     }
 
     // the warps' states into shared memory
@@ -285,35 +317,42 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
         sm.m[warp][nt * 8 + g] = s.m[nt];
         sm.l[warp][nt * 8 + g] = s.l[nt];
       }
+      if (nt * 8 + 2 * t < G) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int d = (j >> 2) * 64 + g * 8 + (j & 3) * 2;
-        *reinterpret_cast<float2*>(&sm.o[warp][nt * 8 + 2 * t][d]) = make_float2(s.o[nt][j][0], s.o[nt][j][2]);
-        *reinterpret_cast<float2*>(&sm.o[warp][nt * 8 + 2 * t + 1][d]) = make_float2(s.o[nt][j][1], s.o[nt][j][3]);
+        for (int j = 0; j < 8; ++j) {
+          const int d = (j >> 2) * 64 + g * 8 + (j & 3) * 2;
+          *reinterpret_cast<float2*>(&sm.o[warp][nt * 8 + 2 * t][d]) = make_float2(s.o[nt][j][0], s.o[nt][j][2]);
+          *reinterpret_cast<float2*>(&sm.o[warp][nt * 8 + 2 * t + 1][d]) = make_float2(s.o[nt][j][1], s.o[nt][j][3]);
+        }
       }
     }
     __syncthreads();
+    // a warp joins the states of a query head, four dimensions to a lane
     const bool whole = t0 == 0 && t1 == T;
     const int slot = 2 * c + (t0 == 0 ? 1 : 0);  // a CTA shares at most its first and its last (sequence, head)
-    for (int head = 0; head < G; ++head) {
+    const size_t head0 = (size_t)b * p.n_head + (size_t)h * G;
+    for (int head = warp; head < G; head += kWarps) {
       float M = -INFINITY;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm.m[w][head]);
       const float mu = M == -INFINITY ? 0.f : M;
-      float l = 0.f, o = 0.f;
+      float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float f = exp2_fast(sm.m[w][head] - mu);
+        const float4 x = *reinterpret_cast<const float4*>(&sm.o[w][head][lane * 4]);
         l = fmaf(f, sm.l[w][head], l);
-        o = fmaf(f, sm.o[w][head][tid], o);
+        o[0] = fmaf(f, x.x, o[0]);
+        o[1] = fmaf(f, x.y, o[1]);
+        o[2] = fmaf(f, x.z, o[2]);
+        o[3] = fmaf(f, x.w, o[3]);
       }
-      const size_t oh = (size_t)b * p.n_head + (size_t)h * G + head;
       if (whole) {
-        p.out[oh * kD + tid] = f2act<F16>(l == 0.f ? 0.f : o / l);
-        if (tid == 0 && p.lse != nullptr) p.lse[oh] = l == 0.f ? -INFINITY : mu + log2f(l) - kLift<F16>;
+        store_out<F16>(p, head0 + head, lane, mu, l, o);
       } else {
-        p.part_o[((size_t)slot * G + head) * kD + tid] = o;
-        if (tid == 0) p.part_ml[(size_t)slot * G + head] = make_float2(M, l);
+        *reinterpret_cast<float4*>(&p.part_o[((size_t)slot * G + head) * kD + lane * 4]) =
+            make_float4(o[0], o[1], o[2], o[3]);
+        if (lane == 0) p.part_ml[(size_t)slot * G + head] = make_float2(M, l);
       }
     }
     if (!whole) {
@@ -328,36 +367,34 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
         __threadfence();
         if (tid == 0) p.counters[b * p.n_kv + h] = 0;
         for (int head = warp; head < G; head += kWarps) {
+          auto at = [&](int q) -> size_t { return (size_t)(2 * q + (q == c0 ? 1 : 0)) * G + head; };
           float M = -INFINITY;
-          for (int q = c0 + lane; q <= c1; q += 32) {
-            const float2 ml = __ldcg(&p.part_ml[(size_t)(2 * q + (q == c0 ? 1 : 0)) * G + head]);
-            M = fmaxf(M, ml.x);
-          }
+          for (int q = c0 + lane; q <= c1; q += 32) M = fmaxf(M, __ldcg(&p.part_ml[at(q)]).x);
 #pragma unroll
           for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-          float l = 0.f;
-          for (int q = c0 + lane; q <= c1; q += 32) {
-            const float2 ml = __ldcg(&p.part_ml[(size_t)(2 * q + (q == c0 ? 1 : 0)) * G + head]);
-            l += exp2_fast(ml.x - (M == -INFINITY ? 0.f : M)) * ml.y;
+          const float mu = M == -INFINITY ? 0.f : M;
+          float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+          for (int q0 = c0; q0 <= c1; q0 += 32) {
+            const int n = min(32, c1 - q0 + 1);
+            float f = 0.f;
+            if (lane < n) {
+              const float2 ml = __ldcg(&p.part_ml[at(q0 + lane)]);
+              f = exp2_fast(ml.x - mu);
+              l = fmaf(f, ml.y, l);
+            }
+#pragma unroll 8
+            for (int i = 0; i < n; ++i) {
+              const float4 x = __ldcg(reinterpret_cast<const float4*>(&p.part_o[at(q0 + i) * kD + lane * 4]));
+              const float fi = __shfl_sync(0xffffffffu, f, i);
+              o[0] = fmaf(fi, x.x, o[0]);
+              o[1] = fmaf(fi, x.y, o[1]);
+              o[2] = fmaf(fi, x.z, o[2]);
+              o[3] = fmaf(fi, x.w, o[3]);
+            }
           }
 #pragma unroll
           for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
-          if (lane == 0) {
-            sm.M[head] = M == -INFINITY ? 0.f : M;
-            sm.L[head] = l;
-            if (p.lse != nullptr)
-              p.lse[(size_t)b * p.n_head + (size_t)h * G + head] = l == 0.f ? -INFINITY : sm.M[head] + log2f(l) - kLift<F16>;
-          }
-        }
-        __syncthreads();
-        for (int head = 0; head < G; ++head) {
-          float o = 0.f;
-          for (int q = c0; q <= c1; ++q) {
-            const size_t sl = (size_t)(2 * q + (q == c0 ? 1 : 0)) * G + head;
-            o = fmaf(exp2_fast(__ldcg(&p.part_ml[sl]).x - sm.M[head]), __ldcg(&p.part_o[sl * kD + tid]), o);
-          }
-          p.out[((size_t)b * p.n_head + (size_t)h * G + head) * kD + tid] =
-              f2act<F16>(sm.L[head] == 0.f ? 0.f : o / sm.L[head]);
+          store_out<F16>(p, head0 + head, lane, mu, l, o);
         }
       }
     }
@@ -434,8 +471,9 @@ long long most_tiles(int n_seqs, int n_kv, long long max_rows) {
   return (long long)n_seqs * n_kv * ((max_rows + kTile - 1) / kTile);
 }
 
-int grid_for(long long tiles, int groups, int sms) {
-  const long long n = (tiles + PAGED_MIN_TILES - 1) / PAGED_MIN_TILES, most = (long long)sms * (groups <= 8 ? 3 : 2);
+int grid_for(long long tiles, long long lists, int groups, int sms) {
+  const long long by_tiles = (tiles + PAGED_MIN_TILES - 1) / PAGED_MIN_TILES, n = by_tiles > lists ? by_tiles : lists;
+  const long long most = (long long)sms * (groups <= 8 ? 3 : 2);
   return (int)(n < most ? n : most);
 }
 
@@ -447,7 +485,7 @@ void paged_attention_plan(int n_seqs, int n_head, int n_kv, long long max_rows, 
                           PagedAttnPlan* plan) {
   const long long tiles = most_tiles(n_seqs, n_kv, max_rows);
   const int groups = n_head / n_kv;
-  plan->grid = grid_for(tiles, groups, sms);
+  plan->grid = grid_for(tiles, (long long)n_seqs * n_kv, groups, sms);
   size_t at = PAGED_COUNTER_BYTES;
   plan->part_o = at;
   at += up256((size_t)2 * plan->grid * groups * kD * sizeof(float));
