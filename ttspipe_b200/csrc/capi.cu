@@ -1001,8 +1001,8 @@ int check_paged(const nf4b_paged_kv* c, bool* f16) {
       (long long)c->n_seqs * c->n_kv * c->max_pages * (c->page_size / PAGED_TILE) >= (1LL << 31))
     return fail(NF4B_ERR_SHAPE, "%d pages, %d of %d rows for each sequence", c->n_pages, c->max_pages, c->page_size);
   if (!aligned(c->k, 16) || !aligned(c->v, 16)) return fail(NF4B_ERR_ALIGN, "pools not 16-byte aligned");
-  if (!aligned(c->block_table, 4) || !aligned(c->weight, 4) || !aligned(c->position, 4))
-    return fail(NF4B_ERR_ALIGN, "block table, weights or positions not 4-byte aligned");
+  if (!aligned(c->block_table, 4) || !aligned(c->weight, 16) || !aligned(c->position, 4))
+    return fail(NF4B_ERR_ALIGN, "weights not 16-byte or block table or positions not 4-byte aligned");
   return NF4B_OK;
 }
 

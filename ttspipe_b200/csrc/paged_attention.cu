@@ -405,9 +405,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
 }
 
 // weight[row] += sum over the group's heads of 2^(score - lse), from the scores the
-// attention kernel left. One thread a row; a reduction instruction instead of a read
-// and a write, so that sequences which share a page add up.
+// attention kernel left. Four rows to a thread; a reduction instruction instead of a
+// read and a write, so that sequences which share a page add up. Rows that take no
+// part have the score -inf and receive 0.
 constexpr int kWThreads = 256;
+constexpr int kWTiles = kWThreads / 4;  // tiles of one pass of a CTA
 
 __global__ void __launch_bounds__(kWThreads) paged_weight_kernel(const __grid_constant__ PagedAttnParams p) {
   extern __shared__ __align__(16) uint8_t smem[];
@@ -415,23 +417,30 @@ __global__ void __launch_bounds__(kWThreads) paged_weight_kernel(const __grid_co
   pdl_wait();
   tile_prefix(p, pre);
   const int U = pre[p.n_seqs], tpp = p.page_size / kTile, G = p.groups;
-  const int i = threadIdx.x % kTile;
-  for (long long uu = (long long)blockIdx.x * (kWThreads / kTile) + threadIdx.x / kTile; uu < U;
-       uu += (long long)gridDim.x * (kWThreads / kTile)) {
+  const int i = (threadIdx.x & 3) * 4;
+  for (long long uu = (long long)blockIdx.x * kWTiles + (threadIdx.x >> 2); uu < U;
+       uu += (long long)gridDim.x * kWTiles) {
     const int u = (int)uu;
     const int b = seq_of(pre, p.n_seqs, u);
     const int T = (pre[b + 1] - pre[b]) / p.n_kv;
     const int h = (u - pre[b]) / T, tile = (u - pre[b]) - h * T;
     const int pg = p.table[(size_t)b * p.max_pages + tile / tpp];
-    if (pg < 0 || pg >= p.n_pages || tile * kTile + i >= seq_rows(p, b)) continue;
     const float* lse = p.lse + (size_t)b * p.n_head + (size_t)h * G;
     const float* sp = p.scores + (size_t)u * G * kTile + i;
-    float w = 0.f;
+    float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
     for (int head = 0; head < G; ++head) {
-      const float L = lse[head];
-      w += L == -INFINITY ? 0.f : exp2_fast(sp[head * kTile] - L);
+      const float4 x = __ldcs(reinterpret_cast<const float4*>(sp + head * kTile));
+      const float L = lse[head] == -INFINITY ? INFINITY : lse[head];
+      w.x += exp2_fast(x.x - L);
+      w.y += exp2_fast(x.y - L);
+      w.z += exp2_fast(x.z - L);
+      w.w += exp2_fast(x.w - L);
     }
-    atomicAdd(p.weight + ((size_t)pg * p.n_kv + h) * p.page_size + (size_t)(tile % tpp) * kTile + i, w);
+    if (pg < 0 || pg >= p.n_pages) continue;
+    float* out = p.weight + ((size_t)pg * p.n_kv + h) * p.page_size + (size_t)(tile % tpp) * kTile + i;
+    asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(out), "f"(w.x), "f"(w.y), "f"(w.z), "f"(w.w)
+                 : "memory");
   }
   pdl_launch_dependents();
 }
@@ -508,7 +517,7 @@ cudaError_t launch_paged_attention(const PagedAttnParams& p, int grid, int sms, 
     e = f16 ? launch_attention<2, true>(p, grid, stream) : launch_attention<2, false>(p, grid, stream);
   if (e != cudaSuccess || p.weight == nullptr) return e;
   const long long tiles = most_tiles(p.n_seqs, p.n_kv, (long long)p.max_pages * p.page_size);
-  const long long n = (tiles + kWThreads / kTile - 1) / (kWThreads / kTile);
+  const long long n = (tiles + kWTiles - 1) / kWTiles;
   return launch(paged_weight_kernel, (int)(n < 8LL * sms ? n : 8LL * sms), kWThreads,
                 (size_t)(p.n_seqs + 1) * sizeof(int), p, stream);
 }
