@@ -474,10 +474,11 @@ int nf4b_qkv_attention_ex(const void* qkv, const void* q_norm_w, const void* k_n
  *                has received, summed over the query heads of its KV head and over
  *                all tokens since the row was written; NULL where it is not kept
  *   position     int32 [n_pages, n_kv, page_size]: each row's token position; or NULL
- * page_size is a multiple of 16, n_seqs at most 4096, n_seqs * n_kv at most 65535
- * and a sequence's capacity max_pages * page_size below 2^31 rows. int32
- * arrays are 4-byte aligned, fp32 pools 16-byte. Lengths, rows and tables are read on the device, so a
- * captured graph serves every state of the cache.
+ * page_size is a multiple of 16, n_seqs at most 4096, n_seqs * n_kv at most 65535;
+ * the pools, and the capacity max_pages * page_size of a sequence, are below 2^31
+ * rows. weight and position are 16-byte aligned, other int32 arrays 4-byte.
+ * Lengths, rows and tables are read on the device, so a captured graph serves every
+ * state of the cache.
  */
 typedef struct nf4b_paged_kv {
   void* k;

@@ -1001,8 +1001,10 @@ int check_paged(const nf4b_paged_kv* c, bool* f16) {
       (long long)c->n_seqs * c->n_kv * c->max_pages * (c->page_size / PAGED_TILE) >= (1LL << 31))
     return fail(NF4B_ERR_SHAPE, "%d pages, %d of %d rows for each sequence", c->n_pages, c->max_pages, c->page_size);
   if (!aligned(c->k, 16) || !aligned(c->v, 16)) return fail(NF4B_ERR_ALIGN, "pools not 16-byte aligned");
-  if (!aligned(c->block_table, 4) || !aligned(c->weight, 16) || !aligned(c->position, 4))
-    return fail(NF4B_ERR_ALIGN, "weights not 16-byte or block table or positions not 4-byte aligned");
+  if ((long long)c->n_pages * c->n_kv * c->page_size >= (1LL << 31))
+    return fail(NF4B_ERR_SHAPE, "pools of %d x %d x %d rows (below 2^31)", c->n_pages, c->n_kv, c->page_size);
+  if (!aligned(c->block_table, 4) || !aligned(c->weight, 16) || !aligned(c->position, 16))
+    return fail(NF4B_ERR_ALIGN, "block table not 4-byte or weights or positions not 16-byte aligned");
   return NF4B_OK;
 }
 
@@ -1145,8 +1147,8 @@ int nf4b_paged_evict(const nf4b_paged_kv* cache, const int32_t* lens, int budget
   if (!lens || !weight_out || !position_out || !lens_out) return fail(NF4B_ERR_ARG, "null pointer");
   if (budget < 1 || recent < 0 || sink < 0 || (long long)recent + sink > budget)
     return fail(NF4B_ERR_ARG, "budget %d of which %d recent and %d first rows are protected", budget, recent, sink);
-  if (!aligned(lens, 4) || !aligned(weight_out, 4) || !aligned(position_out, 4) || !aligned(lens_out, 4))
-    return fail(NF4B_ERR_ALIGN, "lens, weight_out, position_out or lens_out not 4-byte aligned");
+  if (!aligned(lens, 4) || !aligned(weight_out, 16) || !aligned(position_out, 16) || !aligned(lens_out, 4))
+    return fail(NF4B_ERR_ALIGN, "lengths not 4-byte or weight_out or position_out not 16-byte aligned");
   PagedEvictPlan plan;
   paged_evict_plan(cache->n_seqs, cache->n_kv, (long long)cache->max_pages * cache->page_size, budget, &plan);
   if ((st = check_workspace(workspace, workspace_bytes, plan.bytes))) return st;

@@ -455,8 +455,8 @@ struct PagedEvictParams {
   int n_seqs, n_kv, page_size, max_pages, n_pages;
   int* count;    // [n_seqs, n_kv] moves
   int* left;     // [n_seqs] rows left
-  int32_t* to;   // [n_seqs, n_kv, max_moves] rows that are overwritten
-  int32_t* src;  // [n_seqs, n_kv, max_moves] rows that move there
+  int32_t* to;   // [n_seqs, n_kv, max_moves] pool rows that are overwritten
+  int32_t* src;  // [n_seqs, n_kv, max_moves] pool rows that move there
   int max_moves;
 };
 struct PagedEvictPlan {

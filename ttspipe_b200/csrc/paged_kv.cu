@@ -1,6 +1,8 @@
 // The paged KV cache's other two operators: tokens entering their pages (q/k norm,
 // rotary, scatter), and the eviction of the rows that were attended to least.
 
+#include <limits.h>
+
 #include "common.cuh"
 #include "kernels.cuh"
 
@@ -86,202 +88,304 @@ __global__ void __launch_bounds__(kWriteWarps * 32) paged_write_kernel(const __g
 // equally many, the two sets are disjoint, and attention does not depend on the order of rows
 // (the rotary is in the keys), so nothing else has to move.
 //
-// paged_select_kernel finds the smallest kept key by four 8-bit steps from the top
-// (a histogram each) and lists the moves; paged_move_kernel makes them.
+// paged_select_kernel, one CTA a list, finds the smallest kept key digit by digit from
+// the top (11, 11 and 10 bits, a histogram each) and lists the moves;
+// paged_move_kernel makes them.
 constexpr int kSelThreads = 1024;
 constexpr int kSelWarps = kSelThreads / 32;
+constexpr int kBins = 2048;
+constexpr int kMaxStaged = 48 * 1024;  // rows whose keys lie in shared memory; longer lists are read again for each digit
 
 // Weights in rising order as unsigned integers; 0xFFFFFFFF (no weight maps there,
-// NaN being taken as -inf) is for the protected rows.
+// NaN being taken as -inf) is for the protected rows, 0 for rows without a page.
 __device__ __forceinline__ uint32_t weight_key(float w) {
   if (!(w == w)) w = -INFINITY;
   const uint32_t u = __float_as_uint(w + 0.0f);  // -0 as 0
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-struct SelectView {
-  const PagedEvictParams& p;
-  int b, h;
-  __device__ __forceinline__ long long slot(int row) const {  // -1: the row's page is not assigned
-    const int pg = p.table[(size_t)b * p.max_pages + row / p.page_size];
-    if (pg < 0 || pg >= p.n_pages) return -1;
-    return ((long long)pg * p.n_kv + h) * p.page_size + row % p.page_size;
-  }
-};
+// The pool row of a cache row; -1 where its page is not assigned. Four rows from a
+// multiple of four lie in one page.
+__device__ __forceinline__ int pool_row(const PagedEvictParams& p, int b, int h, int row) {
+  const int page = row / p.page_size;
+  const int pg = p.table[(size_t)b * p.max_pages + page];
+  if (pg < 0 || pg >= p.n_pages) return -1;
+  return (pg * p.n_kv + h) * p.page_size + (row - page * p.page_size);
+}
 
-__device__ __forceinline__ int block_reduce_max(int v, int* red) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  v = __reduce_max_sync(0xffffffffu, v);
-  if (lane == 0) red[warp] = v;
-  __syncthreads();
-  v = __reduce_max_sync(0xffffffffu, red[lane]);
-  __syncthreads();
+__device__ __forceinline__ int warp_scan(int v, int lane) {  // inclusive
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, v, off);
+    if (lane >= off) v += o;
+  }
   return v;
 }
 
-// Exclusive prefix of two counts packed in 16 bits each (at most 1024 of either), and their totals.
-__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* red, uint32_t* total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t x = v;
-#pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const uint32_t o = __shfl_up_sync(0xffffffffu, x, off);
-    if (lane >= off) x += o;
-  }
-  if (lane == 31) red[warp] = x;
-  __syncthreads();
-  uint32_t y = red[lane];
-#pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const uint32_t o = __shfl_up_sync(0xffffffffu, y, off);
-    if (lane >= off) y += o;
-  }
-  const uint32_t before = warp ? __shfl_sync(0xffffffffu, y, warp - 1) : 0u;
-  *total = __shfl_sync(0xffffffffu, y, 31);
-  __syncthreads();
-  return before + x - v;
+// Add one to hist[digit] for every lane with `take`: the lanes that share the first
+// one's digit as one addition (all weights may be equal), the others each.
+__device__ __forceinline__ void count_digit(int* hist, int digit, bool take, int lane) {
+  const uint32_t m = __ballot_sync(0xffffffffu, take);
+  if (m == 0) return;
+  const int first = __ffs(m) - 1;
+  const int theirs = __shfl_sync(0xffffffffu, digit, first);  // by every lane, taking part or not
+  const bool same = take && digit == theirs;
+  const uint32_t sm = __ballot_sync(0xffffffffu, same);
+  if (lane == first) atomicAdd(&hist[digit], __popc(sm));
+  if (take && !same) atomicAdd(&hist[digit], 1);
 }
 
-__global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const __grid_constant__ PagedEvictParams p) {
-  __shared__ int hist[256];
-  __shared__ int red[kSelWarps];
+__global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const __grid_constant__ PagedEvictParams p,
+                                                                  int staged_rows) {
+  extern __shared__ __align__(16) uint32_t keys[];
+  __shared__ int hist[kBins];
+  __shared__ int part[5][kSelWarps];
   __shared__ uint32_t s_prefix;
-  __shared__ int s_need;
-  static_assert(kSelWarps == 32, "the block reductions read one value a lane");
+  __shared__ int s_need, s_newest;
+  static_assert(kSelWarps == 32, "the block's sums read one value a lane");
   pdl_wait();
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = blockIdx.x / p.n_kv, h = blockIdx.x - b * p.n_kv;
-  const SelectView view{p, b, h};
   const int cap = p.max_pages * p.page_size;
   const int rows = min(max(p.lens[b], 0), cap), left = min(rows, p.budget);
+  const bool all = rows <= p.budget, staged = rows <= staged_rows;
   if (tid == 0) {
-    p.count[blockIdx.x] = 0;
     if (h == 0) p.left[b] = left;
+    if (all) p.count[blockIdx.x] = 0;
+    s_newest = INT_MIN;
   }
-  const bool copied = p.weight_out != p.weight || p.position_out != p.position;
-  if (rows <= p.budget) {  // all stay
-    if (copied)
-      for (int i = tid; i < rows; i += kSelThreads) {
-        const long long at = view.slot(i);
-        if (at < 0) continue;
-        p.weight_out[at] = p.weight[at];
-        p.position_out[at] = p.position[at];
+  hist[tid] = hist[tid + kSelThreads] = 0;
+  __syncthreads();
+
+  if (!all && p.recent > 0) {
+    int newest = INT_MIN;
+    for (int i = tid * 4; i < rows; i += kSelThreads * 4) {
+      const int at = pool_row(p, b, h, i);
+      if (at < 0) continue;
+      const int4 x = *reinterpret_cast<const int4*>(p.position + at);
+      newest = max(newest, x.x);
+      if (i + 1 < rows) newest = max(newest, x.y);
+      if (i + 2 < rows) newest = max(newest, x.z);
+      if (i + 3 < rows) newest = max(newest, x.w);
+    }
+    newest = __reduce_max_sync(0xffffffffu, newest);
+    if (lane == 0) atomicMax(&s_newest, newest);
+    __syncthreads();
+  }
+  // positions above this are among the newest (no position is above INT_MAX)
+  const int guard = p.recent == 0 ? INT_MAX : s_newest < INT_MIN + p.recent ? INT_MIN : s_newest - p.recent;
+  auto keys_of = [&](int i, int at) -> uint4 {  // of rows i .. i + 3 < rows, else 0
+    if (at < 0) return make_uint4(0, 0, 0, 0);
+    const float4 w = *reinterpret_cast<const float4*>(p.weight + at);
+    const int4 x = *reinterpret_cast<const int4*>(p.position + at);
+    auto key = [&](float wt, int pos, int row) -> uint32_t {
+      return row >= rows ? 0u : pos < p.sink || pos > guard ? 0xFFFFFFFFu : weight_key(wt);
+    };
+    return make_uint4(key(w.x, x.x, i), key(w.y, x.y, i + 1), key(w.z, x.z, i + 2), key(w.w, x.w, i + 3));
+  };
+  auto keys_at = [&](int i) -> uint4 {
+    return staged ? *reinterpret_cast<const uint4*>(keys + i) : keys_of(i, pool_row(p, b, h, i));
+  };
+
+  // the first digit's histogram, and the weights and positions of the first rows into
+  // their output (rows that move overwrite theirs afterwards)
+  const bool copy_w = p.weight_out != p.weight, copy_p = p.position_out != p.position;
+  for (int i0 = 0; i0 < rows; i0 += kSelThreads * 4) {
+    const int i = i0 + tid * 4;
+    const int at = i < rows ? pool_row(p, b, h, i) : -1;
+    if (i < left && at >= 0) {
+      const int n = min(4, left - i);
+      if (copy_w) {
+        if (n == 4)
+          *reinterpret_cast<float4*>(p.weight_out + at) = *reinterpret_cast<const float4*>(p.weight + at);
+        else
+          for (int j = 0; j < n; ++j) p.weight_out[at + j] = p.weight[at + j];
       }
+      if (copy_p) {
+        if (n == 4)
+          *reinterpret_cast<int4*>(p.position_out + at) = *reinterpret_cast<const int4*>(p.position + at);
+        else
+          for (int j = 0; j < n; ++j) p.position_out[at + j] = p.position[at + j];
+      }
+    }
+    if (all) continue;
+    const uint4 k = keys_of(i, at);
+    if (staged && i < rows) *reinterpret_cast<uint4*>(keys + i) = k;
+    count_digit(hist, k.x >> 21, i < rows, lane);
+    count_digit(hist, k.y >> 21, i + 1 < rows, lane);
+    count_digit(hist, k.z >> 21, i + 2 < rows, lane);
+    count_digit(hist, k.w >> 21, i + 3 < rows, lane);
+  }
+  if (all) {
     pdl_launch_dependents();
     return;
   }
-  int newest = -1;
-  if (p.recent > 0) {
-    for (int i = tid; i < rows; i += kSelThreads) {
-      const long long at = view.slot(i);
-      if (at >= 0) newest = max(newest, p.position[at]);
-    }
-    newest = block_reduce_max(newest, red);
-  }
-  auto key = [&](int row) -> uint32_t {
-    const long long at = view.slot(row);
-    if (at < 0) return 0u;
-    const int pos = p.position[at];
-    if (pos < p.sink || (p.recent > 0 && (long long)pos > (long long)newest - p.recent)) return 0xFFFFFFFFu;
-    return weight_key(p.weight[at]);
-  };
+  __syncthreads();
+
   uint32_t prefix = 0;  // the smallest kept key's leading digits
-  int need = left;      // rows of the remaining candidates that stay
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
-    __syncthreads();
-    for (int i = tid; i < rows; i += kSelThreads) {
-      const uint32_t k = key(i);
-      if (shift == 24 || (k >> (shift + 8)) == prefix) atomicAdd(&hist[(k >> shift) & 255u], 1);
+  int need = left;      // rows that stay among those with these digits
+#pragma unroll 1
+  for (int step = 0; step < 3; ++step) {
+    if (step > 0) {
+      const int shift = step == 1 ? 10 : 0;
+      const uint32_t mask = step == 1 ? 2047u : 1023u;
+      hist[tid] = hist[tid + kSelThreads] = 0;
+      __syncthreads();
+      for (int i0 = 0; i0 < rows; i0 += kSelThreads * 4) {
+        const int i = i0 + tid * 4;
+        const uint4 k = i < rows ? keys_at(i) : make_uint4(0, 0, 0, 0);
+        const int up = step == 1 ? 21 : 10;
+        count_digit(hist, (k.x >> shift) & mask, i < rows && (k.x >> up) == prefix, lane);
+        count_digit(hist, (k.y >> shift) & mask, i + 1 < rows && (k.y >> up) == prefix, lane);
+        count_digit(hist, (k.z >> shift) & mask, i + 2 < rows && (k.z >> up) == prefix, lane);
+        count_digit(hist, (k.w >> shift) & mask, i + 3 < rows && (k.w >> up) == prefix, lane);
+      }
+      __syncthreads();
     }
+    // thread t: digits 2047 - 2 t and 2046 - 2 t, falling
+    const int hi = hist[kBins - 1 - 2 * tid], lo = hist[kBins - 2 - 2 * tid];
+    const int mine = warp_scan(hi + lo, lane);
+    if (lane == 31) part[0][warp] = mine;
     __syncthreads();
-    if (tid < 32) {  // lane l: digits 255 - 8 l down to 248 - 8 l
-      int n = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) n += hist[255 - tid * 8 - i];
-      int x = n;
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, x, off);
-        if (tid >= off) x += o;
-      }
-      int above = x - n;
-      if (above < need && need <= x) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int digit = 255 - tid * 8 - i;
-          if (above < need && need <= above + hist[digit]) {
-            s_prefix = (prefix << 8) | (uint32_t)digit;
-            s_need = need - above;
-          }
-          above += hist[digit];
-        }
-      }
+    const int upto = warp_scan(part[0][lane], lane);
+    int above = (warp ? __shfl_sync(0xffffffffu, upto, warp - 1) : 0) + mine - hi - lo;
+    const int digit = above < need && need <= above + hi ? 0 : above + hi < need && need <= above + hi + lo ? 1 : -1;
+    if (digit >= 0) {
+      s_prefix = (prefix << (step == 2 ? 10 : 11)) | (uint32_t)(kBins - 1 - 2 * tid - digit);
+      s_need = need - above - (digit ? hi : 0);
     }
     __syncthreads();
     prefix = s_prefix;
     need = s_need;
-    __syncthreads();
   }
-  // key > prefix stays; of those equal to it the first `need` do
-  uint32_t* ured = reinterpret_cast<uint32_t*>(red);
-  int equal = 0, holes = 0, moved = 0;
+
+  // A key above prefix stays, and of the equal ones the first `need` do. Each warp
+  // takes a run of rows: it counts, the counts are summed up, then it writes.
+  const int run = ((rows + kSelThreads * 4 - 1) / (kSelThreads * 4)) * 128;  // rows of a warp
+  const int r0 = warp * run, r1 = min(rows, r0 + run);
+  int gt[2] = {0, 0}, eq[2] = {0, 0};  // below `left`, and from it on
+  for (int i = r0 + lane * 4; i < r1; i += 128) {
+    const uint4 k4 = keys_at(i);
+    const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (i + j >= rows) continue;
+      const int s = i + j >= left;
+      gt[s] += k[j] > prefix;
+      eq[s] += k[j] == prefix;
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    gt[s] = __reduce_add_sync(0xffffffffu, gt[s]);
+    eq[s] = __reduce_add_sync(0xffffffffu, eq[s]);
+  }
+  if (lane == 0) part[0][warp] = eq[0] + eq[1];
+  __syncthreads();
+  const int eqs = warp_scan(part[0][lane], lane);
+  int eq_at = warp ? __shfl_sync(0xffffffffu, eqs, warp - 1) : 0;
+  const bool ties = __shfl_sync(0xffffffffu, eqs, 31) != need;  // some equal rows go
+  {
+    const int eq_low = min(max(need - eq_at, 0), eq[0]), eq_high = min(max(need - eq_at - eq[0], 0), eq[1]);
+    const int low = max(min(r1, left) - r0, 0);
+    if (lane == 0) {
+      part[1][warp] = low - gt[0] - eq_low;
+      part[2][warp] = gt[1] + eq_high;
+    }
+  }
+  __syncthreads();
+  const int holes = warp_scan(part[1][lane], lane), outs = warp_scan(part[2][lane], lane);
+  int hole_at = warp ? __shfl_sync(0xffffffffu, holes, warp - 1) : 0;
+  int out_at = warp ? __shfl_sync(0xffffffffu, outs, warp - 1) : 0;
+  const int moved = __shfl_sync(0xffffffffu, outs, 31);
+  if (tid == 0) p.count[blockIdx.x] = moved;
   int32_t* to = p.to + (size_t)blockIdx.x * p.max_moves;
   int32_t* src = p.src + (size_t)blockIdx.x * p.max_moves;
-  for (int i0 = 0; i0 < rows; i0 += kSelThreads) {
-    const int i = i0 + tid;
-    const uint32_t k = i < rows ? key(i) : 0u;
-    uint32_t total;
-    const bool eq = i < rows && k == prefix;
-    const int rank = equal + (int)block_scan(eq ? 1u : 0u, ured, &total);
-    equal += (int)total;
-    const bool kept = i < rows && (k > prefix || (eq && rank < need));
-    const bool hole = i < left && !kept, out = i >= left && kept;
-    const uint32_t at = block_scan((hole ? 1u : 0u) | (out ? 0x10000u : 0u), ured, &total);
-    if (hole) to[holes + (int)(at & 0xFFFFu)] = i;
-    if (out) src[moved + (int)(at >> 16)] = i;
-    holes += (int)(total & 0xFFFFu);
-    moved += (int)(total >> 16);
-    if (copied && kept && i < left) {
-      const long long s = view.slot(i);
-      if (s >= 0) {
-        p.weight_out[s] = p.weight[s];
-        p.position_out[s] = p.position[s];
+  for (int i0 = r0; i0 < r1; i0 += 128) {
+    const int i = i0 + lane * 4;
+    const uint4 k4 = i < r1 ? keys_at(i) : make_uint4(0, 0, 0, 0);
+    const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+    int rank = eq_at;
+    if (ties) {
+      int n = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) n += i + j < r1 && k[j] == prefix;
+      const int upto = warp_scan(n, lane);
+      rank += upto - n;
+      eq_at += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    bool hole[4], out[4];
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool is_eq = k[j] == prefix;
+      const bool kept = k[j] > prefix || (is_eq && (!ties || rank < need));
+      if (is_eq) ++rank;
+      hole[j] = i + j < r1 && i + j < left && !kept;
+      out[j] = i + j < r1 && i + j >= left && kept;
+      n += (hole[j] ? 1 : 0) + (out[j] ? 0x10000 : 0);
+    }
+    const int upto = warp_scan(n, lane);
+    int hole_to = hole_at + ((upto - n) & 0xFFFF), out_to = out_at + ((upto - n) >> 16);
+    const int total = __shfl_sync(0xffffffffu, upto, 31);
+    hole_at += total & 0xFFFF;
+    out_at += total >> 16;
+    if (n != 0) {
+      const int at = pool_row(p, b, h, i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (hole[j]) to[hole_to++] = at < 0 ? -1 : at + j;
+        if (out[j]) src[out_to++] = at < 0 ? -1 : at + j;
       }
     }
   }
-  if (tid == 0) p.count[blockIdx.x] = moved;
   pdl_launch_dependents();
 }
 
 constexpr int kMoveWarps = 8;
+constexpr int kMoveRows = 8;  // rows that a warp has in flight
 
-// One warp a row: half of it copies the key row, half the value row, 16 bytes a lane.
+// Eight rows to a warp at a time: half of it copies the key rows, half the value rows,
+// 16 bytes a lane.
 __global__ void __launch_bounds__(kMoveWarps * 32) paged_move_kernel(const __grid_constant__ PagedEvictParams p) {
   pdl_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int b = blockIdx.y / p.n_kv, h = blockIdx.y - b * p.n_kv;
-  const SelectView view{p, b, h};
-  if (h == 0 && blockIdx.x == 0 && threadIdx.x == 0) p.lens_out[b] = p.left[b];
+  const int b = blockIdx.y / p.n_kv;
+  if (blockIdx.y == b * p.n_kv && blockIdx.x == 0 && threadIdx.x == 0) p.lens_out[b] = p.left[b];
   const int n = p.count[blockIdx.y];
   const int32_t* to = p.to + (size_t)blockIdx.y * p.max_moves;
   const int32_t* src = p.src + (size_t)blockIdx.y * p.max_moves;
-  for (int i = blockIdx.x * kMoveWarps + warp; i < n; i += gridDim.x * kMoveWarps) {
-    const long long from = view.slot(src[i]), at = view.slot(to[i]);
-    if (from < 0 || at < 0) continue;
-    uint16_t* pool = lane < 16 ? p.k : p.v;
-    reinterpret_cast<uint4*>(pool + at * kD)[lane & 15] = reinterpret_cast<const uint4*>(pool + from * kD)[lane & 15];
-    if (lane == 0) {
+  uint4* pool = reinterpret_cast<uint4*>(lane < 16 ? p.k : p.v) + (lane & 15);
+  for (int i = (blockIdx.x * kMoveWarps + warp) * kMoveRows; i < n; i += gridDim.x * kMoveWarps * kMoveRows) {
+    int from = -1, at = -1;
+    if (lane < kMoveRows && i + lane < n) {
+      from = src[i + lane];
+      at = to[i + lane];
+    }
+    if (from < 0 || at < 0) from = at = -1;
+    uint4 x[kMoveRows];
+#pragma unroll
+    for (int j = 0; j < kMoveRows; ++j) {
+      const int f = __shfl_sync(0xffffffffu, from, j);
+      if (f >= 0) x[j] = pool[(size_t)f * (kD / 8)];
+    }
+    if (at >= 0) {
       p.weight_out[at] = p.weight[from];
       p.position_out[at] = p.position[from];
+    }
+#pragma unroll
+    for (int j = 0; j < kMoveRows; ++j) {
+      const int t = __shfl_sync(0xffffffffu, at, j);
+      if (t >= 0) pool[(size_t)t * (kD / 8)] = x[j];
     }
   }
   pdl_launch_dependents();
 }
 
-template <typename P>
-cudaError_t launch(void (*kernel)(P), dim3 grid, int threads, const P& p, cudaStream_t stream) {
+template <typename... A>
+cudaError_t launch(void (*kernel)(A...), dim3 grid, int threads, size_t smem, cudaStream_t stream, A... args) {
   cudaLaunchConfig_t cfg = {};
+  cfg.dynamicSmemBytes = smem;
   cfg.gridDim = grid;
   cfg.blockDim = dim3((unsigned)threads);
   cfg.stream = stream;
@@ -290,7 +394,7 @@ cudaError_t launch(void (*kernel)(P), dim3 grid, int threads, const P& p, cudaSt
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -301,7 +405,7 @@ cudaError_t launch_paged_write(const PagedWriteParams& p, int sms, bool f16, cud
   const long long items = (long long)p.n_tokens * (p.n_head + 2 * p.n_kv);
   const long long want = (items + kWriteWarps - 1) / kWriteWarps, most = 16LL * sms;
   return launch(f16 ? paged_write_kernel<true> : paged_write_kernel<false>, dim3((unsigned)(want < most ? want : most)),
-                kWriteWarps * 32, p, stream);
+                kWriteWarps * 32, 0, stream, p);
 }
 
 void paged_evict_plan(int n_seqs, int n_kv, long long max_rows, int budget, PagedEvictPlan* plan) {
@@ -318,13 +422,25 @@ void paged_evict_plan(int n_seqs, int n_kv, long long max_rows, int budget, Page
 }
 
 cudaError_t launch_paged_evict(const PagedEvictParams& p, int sms, cudaStream_t stream) {
-  const int lists = p.n_seqs * p.n_kv;
-  cudaError_t e = launch(paged_select_kernel, dim3((unsigned)lists), kSelThreads, p, stream);
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!configured[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(paged_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         kMaxStaged * (int)sizeof(uint32_t));
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
+  }
+  const int lists = p.n_seqs * p.n_kv, cap = p.max_pages * p.page_size;
+  const int staged = cap < kMaxStaged ? cap : kMaxStaged;
+  cudaError_t e = launch(paged_select_kernel, dim3((unsigned)lists), kSelThreads, staged * sizeof(uint32_t), stream, p,
+                         staged);
   if (e != cudaSuccess) return e;
-  long long x = (p.max_moves + kMoveWarps - 1) / kMoveWarps;
-  const long long most = (8LL * sms + lists - 1) / lists;
-  x = x > most ? most : x < 1 ? 1 : x;
-  return launch(paged_move_kernel, dim3((unsigned)x, (unsigned)lists), kMoveWarps * 32, p, stream);
+  // as many CTAs as are resident (4 an SM), no more than a list has rows for
+  const int want = (p.max_moves + kMoveWarps * kMoveRows - 1) / (kMoveWarps * kMoveRows), most = 4 * sms / lists;
+  const int x = want < most ? want : most;
+  return launch(paged_move_kernel, dim3((unsigned)(x < 1 ? 1 : x), (unsigned)lists), kMoveWarps * 32, 0, stream, p);
 }
 
 }  // namespace nf4b
