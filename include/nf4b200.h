@@ -475,8 +475,8 @@ int nf4b_qkv_attention_ex(const void* qkv, const void* q_norm_w, const void* k_n
  *                all tokens since the row was written; NULL where it is not kept
  *   position     int32 [n_pages, n_kv, page_size]: each row's token position; or NULL
  * page_size is a multiple of 16, n_seqs at most 4096, n_seqs * n_kv at most 65535;
- * the pools, and the capacity max_pages * page_size of a sequence, are below 2^31
- * rows. weight and position are 16-byte aligned, other int32 arrays 4-byte.
+ * the pools are below 2^31 rows and a sequence's capacity max_pages * page_size
+ * below 2^30. weight and position are 16-byte aligned, other int32 arrays 4-byte.
  * Lengths, rows and tables are read on the device, so a captured graph serves every
  * state of the cache.
  */

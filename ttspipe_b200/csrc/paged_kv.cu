@@ -91,9 +91,9 @@ __global__ void __launch_bounds__(kWriteWarps * 32) paged_write_kernel(const __g
 // paged_select_kernel, one CTA a list, finds the smallest kept key digit by digit from
 // the top (11, 11 and 10 bits, a histogram each) and lists the moves;
 // paged_move_kernel makes them.
-constexpr int kSelThreads = 1024;
-constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kBins = 2048;
+constexpr int kSelDeep = 4;  // groups of four rows that a thread requests at once
+constexpr int kShortList = 8192;  // lists up to this get 256 threads, so that several share an SM; longer ones 1024
 constexpr int kMaxStaged = 48 * 1024;  // rows whose keys lie in shared memory; longer lists are read again for each digit
 
 // Weights in rising order as unsigned integers; 0xFFFFFFFF (no weight maps there,
@@ -104,14 +104,31 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// The pool row of a cache row; -1 where its page is not assigned. Four rows from a
-// multiple of four lie in one page.
-__device__ __forceinline__ int pool_row(const PagedEvictParams& p, int b, int h, int row) {
-  const int page = row / p.page_size;
-  const int pg = p.table[(size_t)b * p.max_pages + page];
-  if (pg < 0 || pg >= p.n_pages) return -1;
-  return (pg * p.n_kv + h) * p.page_size + (row - page * p.page_size);
-}
+// Walks a list four rows at a time (they lie in one page) with a constant step, the
+// page and the row in it carried along instead of divided out.
+struct Quads {
+  const int32_t* table;
+  int h, n_kv, n_pages, page_size, step_pages, step_rows;
+  int row, page, at;
+  __device__ __forceinline__ Quads(const PagedEvictParams& p, int b, int head, int first, int step)
+      : table(p.table + (size_t)b * p.max_pages), h(head), n_kv(p.n_kv), n_pages(p.n_pages), page_size(p.page_size),
+        step_pages(step / p.page_size), step_rows(step % p.page_size), row(first), page(first / p.page_size),
+        at(first % p.page_size) {}
+  __device__ __forceinline__ void next(int step) {
+    row += step;
+    page += step_pages;
+    at += step_rows;
+    if (at >= page_size) {
+      at -= page_size;
+      ++page;
+    }
+  }
+  // The pool row of `row`; -1 where its page is not assigned.
+  __device__ __forceinline__ int pool() const {
+    const int pg = table[page];
+    return pg < 0 || pg >= n_pages ? -1 : (pg * n_kv + h) * page_size + at;
+  }
+};
 
 __device__ __forceinline__ int warp_scan(int v, int lane) {  // inclusive
 #pragma unroll
@@ -122,27 +139,28 @@ __device__ __forceinline__ int warp_scan(int v, int lane) {  // inclusive
   return v;
 }
 
-// Add one to hist[digit] for every lane with `take`: the lanes that share the first
-// one's digit as one addition (all weights may be equal), the others each.
-__device__ __forceinline__ void count_digit(int* hist, int digit, bool take, int lane) {
-  const uint32_t m = __ballot_sync(0xffffffffu, take);
-  if (m == 0) return;
-  const int first = __ffs(m) - 1;
-  const int theirs = __shfl_sync(0xffffffffu, digit, first);  // by every lane, taking part or not
-  const bool same = take && digit == theirs;
-  const uint32_t sm = __ballot_sync(0xffffffffu, same);
-  if (lane == first) atomicAdd(&hist[digit], __popc(sm));
-  if (take && !same) atomicAdd(&hist[digit], 1);
+// Add one to hist[digit] for every lane with `take`. `crowded`: most rows may share a
+// digit (new rows all have weight 0); then the lanes that share the first one's are one addition.
+__device__ __forceinline__ void count_digit(int* hist, int digit, bool take, bool crowded, int lane) {
+  if (crowded) {
+    const int theirs = __shfl_sync(0xffffffffu, digit, 0);  // by every lane, taking part or not
+    const bool same = take && digit == theirs;
+    const uint32_t m = __ballot_sync(0xffffffffu, same);
+    if (lane == __ffs(m) - 1) atomicAdd(&hist[digit], __popc(m));
+    take = take && !same;
+  }
+  if (take) atomicAdd(&hist[digit], 1);
 }
 
-__global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const __grid_constant__ PagedEvictParams p,
-                                                                  int staged_rows) {
+template <int kSelThreads>
+__global__ void __launch_bounds__(kSelThreads, kSelThreads == 1024 ? 1 : 4)
+    paged_select_kernel(const __grid_constant__ PagedEvictParams p, int staged_rows) {
   extern __shared__ __align__(16) uint32_t keys[];
   __shared__ int hist[kBins];
-  __shared__ int part[5][kSelWarps];
+  __shared__ int part[3][32];
   __shared__ uint32_t s_prefix;
-  __shared__ int s_need, s_newest;
-  static_assert(kSelWarps == 32, "the block's sums read one value a lane");
+  __shared__ int s_need, s_among, s_newest;
+  constexpr int kStep = kSelThreads * 4, kWarps = kSelThreads / 32, kMine = kBins / kSelThreads;
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = blockIdx.x / p.n_kv, h = blockIdx.x - b * p.n_kv;
@@ -154,19 +172,39 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const __grid_
     if (all) p.count[blockIdx.x] = 0;
     s_newest = INT_MIN;
   }
-  hist[tid] = hist[tid + kSelThreads] = 0;
+  auto clear = [&]() {
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) hist[tid + j * kSelThreads] = 0;
+  };
+  // of one value a warp: the sum up to the warp before this one's, and of all
+  auto warps_before = [&](const int* v, int* total) -> int {
+    const int upto = warp_scan(lane < kWarps ? v[lane] : 0, lane);
+    *total = __shfl_sync(0xffffffffu, upto, 31);
+    return warp ? __shfl_sync(0xffffffffu, upto, warp - 1) : 0;
+  };
+  clear();
   __syncthreads();
 
   if (!all && p.recent > 0) {
     int newest = INT_MIN;
-    for (int i = tid * 4; i < rows; i += kSelThreads * 4) {
-      const int at = pool_row(p, b, h, i);
-      if (at < 0) continue;
-      const int4 x = *reinterpret_cast<const int4*>(p.position + at);
-      newest = max(newest, x.x);
-      if (i + 1 < rows) newest = max(newest, x.y);
-      if (i + 2 < rows) newest = max(newest, x.z);
-      if (i + 3 < rows) newest = max(newest, x.w);
+    for (Quads q(p, b, h, tid * 4, kStep); q.row < rows;) {
+      int at[kSelDeep];
+      int4 x[kSelDeep];
+      const int first = q.row;
+#pragma unroll
+      for (int u = 0; u < kSelDeep; ++u, q.next(kStep)) at[u] = q.row < rows ? q.pool() : -1;
+#pragma unroll
+      for (int u = 0; u < kSelDeep; ++u)
+        if (at[u] >= 0) x[u] = *reinterpret_cast<const int4*>(p.position + at[u]);
+#pragma unroll
+      for (int u = 0; u < kSelDeep; ++u) {
+        if (at[u] < 0) continue;
+        const int n = rows - first - u * kStep;  // at least one
+        newest = max(newest, x[u].x);
+        if (n > 1) newest = max(newest, x[u].y);
+        if (n > 2) newest = max(newest, x[u].z);
+        if (n > 3) newest = max(newest, x[u].w);
+      }
     }
     newest = __reduce_max_sync(0xffffffffu, newest);
     if (lane == 0) atomicMax(&s_newest, newest);
@@ -174,47 +212,61 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const __grid_
   }
   // positions above this are among the newest (no position is above INT_MAX)
   const int guard = p.recent == 0 ? INT_MAX : s_newest < INT_MIN + p.recent ? INT_MIN : s_newest - p.recent;
-  auto keys_of = [&](int i, int at) -> uint4 {  // of rows i .. i + 3 < rows, else 0
-    if (at < 0) return make_uint4(0, 0, 0, 0);
-    const float4 w = *reinterpret_cast<const float4*>(p.weight + at);
-    const int4 x = *reinterpret_cast<const int4*>(p.position + at);
-    auto key = [&](float wt, int pos, int row) -> uint32_t {
-      return row >= rows ? 0u : pos < p.sink || pos > guard ? 0xFFFFFFFFu : weight_key(wt);
+  auto keys_from = [&](const float4& w, const int4& x) -> uint4 {
+    auto key = [&](float wt, int pos) -> uint32_t {
+      return pos < p.sink || pos > guard ? 0xFFFFFFFFu : weight_key(wt);
     };
-    return make_uint4(key(w.x, x.x, i), key(w.y, x.y, i + 1), key(w.z, x.z, i + 2), key(w.w, x.w, i + 3));
+    return make_uint4(key(w.x, x.x), key(w.y, x.y), key(w.z, x.z), key(w.w, x.w));
   };
-  auto keys_at = [&](int i) -> uint4 {
-    return staged ? *reinterpret_cast<const uint4*>(keys + i) : keys_of(i, pool_row(p, b, h, i));
+  auto keys_of = [&](int at) -> uint4 {
+    if (at < 0) return make_uint4(0, 0, 0, 0);
+    return keys_from(*reinterpret_cast<const float4*>(p.weight + at),
+                     *reinterpret_cast<const int4*>(p.position + at));
+  };
+  auto keys_at = [&](const Quads& q) -> uint4 {
+    return staged ? *reinterpret_cast<const uint4*>(keys + q.row) : keys_of(q.pool());
   };
 
   // the first digit's histogram, and the weights and positions of the first rows into
   // their output (rows that move overwrite theirs afterwards)
   const bool copy_w = p.weight_out != p.weight, copy_p = p.position_out != p.position;
-  for (int i0 = 0; i0 < rows; i0 += kSelThreads * 4) {
-    const int i = i0 + tid * 4;
-    const int at = i < rows ? pool_row(p, b, h, i) : -1;
-    if (i < left && at >= 0) {
-      const int n = min(4, left - i);
-      if (copy_w) {
-        if (n == 4)
-          *reinterpret_cast<float4*>(p.weight_out + at) = *reinterpret_cast<const float4*>(p.weight + at);
-        else
-          for (int j = 0; j < n; ++j) p.weight_out[at + j] = p.weight[at + j];
+  Quads q0(p, b, h, tid * 4, kStep);
+  for (int i0 = 0; i0 < rows; i0 += kSelDeep * kStep) {
+    int at[kSelDeep];
+    float4 w[kSelDeep];
+    int4 x[kSelDeep];
+    const int first = q0.row;
+#pragma unroll
+    for (int u = 0; u < kSelDeep; ++u, q0.next(kStep)) at[u] = q0.row < rows ? q0.pool() : -1;
+#pragma unroll
+    for (int u = 0; u < kSelDeep; ++u)
+      if (at[u] >= 0) {
+        w[u] = *reinterpret_cast<const float4*>(p.weight + at[u]);
+        x[u] = *reinterpret_cast<const int4*>(p.position + at[u]);
       }
-      if (copy_p) {
-        if (n == 4)
-          *reinterpret_cast<int4*>(p.position_out + at) = *reinterpret_cast<const int4*>(p.position + at);
-        else
-          for (int j = 0; j < n; ++j) p.position_out[at + j] = p.position[at + j];
+#pragma unroll
+    for (int u = 0; u < kSelDeep; ++u) {
+      const int i = first + u * kStep;
+      if (i0 + u * kStep >= rows) break;
+      if (i < left && at[u] >= 0 && (copy_w || copy_p)) {
+        if (i + 4 <= left) {
+          if (copy_w) *reinterpret_cast<float4*>(p.weight_out + at[u]) = w[u];
+          if (copy_p) *reinterpret_cast<int4*>(p.position_out + at[u]) = x[u];
+        } else {
+          for (int j = 0; j < left - i; ++j) {
+            if (copy_w) p.weight_out[at[u] + j] = p.weight[at[u] + j];
+            if (copy_p) p.position_out[at[u] + j] = p.position[at[u] + j];
+          }
+        }
       }
+      if (all) continue;
+      const uint4 k = at[u] < 0 ? make_uint4(0, 0, 0, 0) : keys_from(w[u], x[u]);
+      if (staged && i < rows) *reinterpret_cast<uint4*>(keys + i) = k;
+      count_digit(hist, k.x >> 21, i < rows, true, lane);
+      count_digit(hist, k.y >> 21, i + 1 < rows, true, lane);
+      count_digit(hist, k.z >> 21, i + 2 < rows, true, lane);
+      count_digit(hist, k.w >> 21, i + 3 < rows, true, lane);
     }
-    if (all) continue;
-    const uint4 k = keys_of(i, at);
-    if (staged && i < rows) *reinterpret_cast<uint4*>(keys + i) = k;
-    count_digit(hist, k.x >> 21, i < rows, lane);
-    count_digit(hist, k.y >> 21, i + 1 < rows, lane);
-    count_digit(hist, k.z >> 21, i + 2 < rows, lane);
-    count_digit(hist, k.w >> 21, i + 3 < rows, lane);
   }
   if (all) {
     pdl_launch_dependents();
@@ -227,52 +279,75 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const __grid_
 #pragma unroll 1
   for (int step = 0; step < 3; ++step) {
     if (step > 0) {
-      const int shift = step == 1 ? 10 : 0;
+      const int shift = step == 1 ? 10 : 0, up = step == 1 ? 21 : 10;
       const uint32_t mask = step == 1 ? 2047u : 1023u;
-      hist[tid] = hist[tid + kSelThreads] = 0;
+      const bool crowded = s_among > rows / 8;
+      clear();
       __syncthreads();
-      for (int i0 = 0; i0 < rows; i0 += kSelThreads * 4) {
-        const int i = i0 + tid * 4;
-        const uint4 k = i < rows ? keys_at(i) : make_uint4(0, 0, 0, 0);
-        const int up = step == 1 ? 21 : 10;
-        count_digit(hist, (k.x >> shift) & mask, i < rows && (k.x >> up) == prefix, lane);
-        count_digit(hist, (k.y >> shift) & mask, i + 1 < rows && (k.y >> up) == prefix, lane);
-        count_digit(hist, (k.z >> shift) & mask, i + 2 < rows && (k.z >> up) == prefix, lane);
-        count_digit(hist, (k.w >> shift) & mask, i + 3 < rows && (k.w >> up) == prefix, lane);
+      Quads q(p, b, h, tid * 4, kStep);
+      for (int i0 = 0; i0 < rows; i0 += kStep, q.next(kStep)) {
+        const int i = q.row;
+        const uint4 k = i < rows ? keys_at(q) : make_uint4(0, 0, 0, 0);
+        count_digit(hist, (k.x >> shift) & mask, i < rows && (k.x >> up) == prefix, crowded, lane);
+        count_digit(hist, (k.y >> shift) & mask, i + 1 < rows && (k.y >> up) == prefix, crowded, lane);
+        count_digit(hist, (k.z >> shift) & mask, i + 2 < rows && (k.z >> up) == prefix, crowded, lane);
+        count_digit(hist, (k.w >> shift) & mask, i + 3 < rows && (k.w >> up) == prefix, crowded, lane);
       }
       __syncthreads();
     }
-    // thread t: digits 2047 - 2 t and 2046 - 2 t, falling
-    const int hi = hist[kBins - 1 - 2 * tid], lo = hist[kBins - 2 - 2 * tid];
-    const int mine = warp_scan(hi + lo, lane);
+    // falling digits, kMine to a thread
+    int n[kMine], sum = 0, all_of;
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) sum += n[j] = hist[kBins - 1 - kMine * tid - j];
+    const int mine = warp_scan(sum, lane);
     if (lane == 31) part[0][warp] = mine;
     __syncthreads();
-    const int upto = warp_scan(part[0][lane], lane);
-    int above = (warp ? __shfl_sync(0xffffffffu, upto, warp - 1) : 0) + mine - hi - lo;
-    const int digit = above < need && need <= above + hi ? 0 : above + hi < need && need <= above + hi + lo ? 1 : -1;
-    if (digit >= 0) {
-      s_prefix = (prefix << (step == 2 ? 10 : 11)) | (uint32_t)(kBins - 1 - 2 * tid - digit);
-      s_need = need - above - (digit ? hi : 0);
+    int above = warps_before(part[0], &all_of) + mine - sum;
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) {
+      if (above < need && need <= above + n[j]) {
+        s_prefix = (prefix << (step == 2 ? 10 : 11)) | (uint32_t)(kBins - 1 - kMine * tid - j);
+        s_need = need - above;
+        s_among = n[j];
+      }
+      above += n[j];
     }
     __syncthreads();
     prefix = s_prefix;
     need = s_need;
   }
 
-  // A key above prefix stays, and of the equal ones the first `need` do. Each warp
-  // takes a run of rows: it counts, the counts are summed up, then it writes.
-  const int run = ((rows + kSelThreads * 4 - 1) / (kSelThreads * 4)) * 128;  // rows of a warp
+  // A key above prefix stays, and of the s_among equal ones the first `need` do. Each
+  // warp takes a run of rows: it counts, the counts are summed up, then it writes.
+  const bool ties = s_among != need;  // some equal rows go
+  const int run = ((rows + kStep - 1) / kStep) * 128;
   const int r0 = warp * run, r1 = min(rows, r0 + run);
   int gt[2] = {0, 0}, eq[2] = {0, 0};  // below `left`, and from it on
-  for (int i = r0 + lane * 4; i < r1; i += 128) {
-    const uint4 k4 = keys_at(i);
-    const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
+  for (Quads q(p, b, h, r0 + lane * 4, 128); q.row < r1; q.next(128)) {
+    const uint4 k = keys_at(q);
+    const int i = q.row;
+    if (i + 4 <= left || (i >= left && i + 4 <= rows)) {
+      const int n = (k.x > prefix) + (k.y > prefix) + (k.z > prefix) + (k.w > prefix);
+      const int e = (k.x == prefix) + (k.y == prefix) + (k.z == prefix) + (k.w == prefix);
+      if (i < left) {
+        gt[0] += n;
+        eq[0] += e;
+      } else {
+        gt[1] += n;
+        eq[1] += e;
+      }
+    } else {
+      const uint32_t kk[4] = {k.x, k.y, k.z, k.w};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (i + j >= rows) continue;
-      const int s = i + j >= left;
-      gt[s] += k[j] > prefix;
-      eq[s] += k[j] == prefix;
+      for (int j = 0; j < 4; ++j) {
+        if (i + j < left) {
+          gt[0] += kk[j] > prefix;
+          eq[0] += kk[j] == prefix;
+        } else if (i + j < rows) {
+          gt[1] += kk[j] > prefix;
+          eq[1] += kk[j] == prefix;
+        }
+      }
     }
   }
 #pragma unroll
@@ -280,62 +355,63 @@ __global__ void __launch_bounds__(kSelThreads) paged_select_kernel(const __grid_
     gt[s] = __reduce_add_sync(0xffffffffu, gt[s]);
     eq[s] = __reduce_add_sync(0xffffffffu, eq[s]);
   }
-  if (lane == 0) part[0][warp] = eq[0] + eq[1];
-  __syncthreads();
-  const int eqs = warp_scan(part[0][lane], lane);
-  int eq_at = warp ? __shfl_sync(0xffffffffu, eqs, warp - 1) : 0;
-  const bool ties = __shfl_sync(0xffffffffu, eqs, 31) != need;  // some equal rows go
-  {
-    const int eq_low = min(max(need - eq_at, 0), eq[0]), eq_high = min(max(need - eq_at - eq[0], 0), eq[1]);
-    const int low = max(min(r1, left) - r0, 0);
-    if (lane == 0) {
-      part[1][warp] = low - gt[0] - eq_low;
-      part[2][warp] = gt[1] + eq_high;
-    }
+  int eq_at = 0;
+  if (ties) {
+    if (lane == 0) part[0][warp] = eq[0] + eq[1];
+    __syncthreads();
+    int all_of;
+    eq_at = warps_before(part[0], &all_of);
+    eq[1] = min(max(need - eq_at - eq[0], 0), eq[1]);
+    eq[0] = min(max(need - eq_at, 0), eq[0]);
+  }
+  if (lane == 0) {
+    part[1][warp] = max(min(r1, left) - r0, 0) - gt[0] - eq[0];
+    part[2][warp] = gt[1] + eq[1];
   }
   __syncthreads();
-  const int holes = warp_scan(part[1][lane], lane), outs = warp_scan(part[2][lane], lane);
-  int hole_at = warp ? __shfl_sync(0xffffffffu, holes, warp - 1) : 0;
-  int out_at = warp ? __shfl_sync(0xffffffffu, outs, warp - 1) : 0;
-  const int moved = __shfl_sync(0xffffffffu, outs, 31);
+  int holes, moved;  // equally many
+  int hole_at = warps_before(part[1], &holes), out_at = warps_before(part[2], &moved);
   if (tid == 0) p.count[blockIdx.x] = moved;
   int32_t* to = p.to + (size_t)blockIdx.x * p.max_moves;
   int32_t* src = p.src + (size_t)blockIdx.x * p.max_moves;
-  for (int i0 = r0; i0 < r1; i0 += 128) {
-    const int i = i0 + lane * 4;
-    const uint4 k4 = i < r1 ? keys_at(i) : make_uint4(0, 0, 0, 0);
+  Quads q(p, b, h, r0 + lane * 4, 128);
+  for (int i0 = r0; i0 < r1; i0 += 128, q.next(128)) {
+    const int i = q.row;
+    const uint4 k4 = i < r1 ? keys_at(q) : make_uint4(0, 0, 0, 0);
     const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
-    int rank = eq_at;
+    uint32_t kept = 0;
     if (ties) {
       int n = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) n += i + j < r1 && k[j] == prefix;
       const int upto = warp_scan(n, lane);
-      rank += upto - n;
+      int rank = eq_at + upto - n;
       eq_at += __shfl_sync(0xffffffffu, upto, 31);
-    }
-    bool hole[4], out[4];
-    int n = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const bool is_eq = k[j] == prefix;
-      const bool kept = k[j] > prefix || (is_eq && (!ties || rank < need));
-      if (is_eq) ++rank;
-      hole[j] = i + j < r1 && i + j < left && !kept;
-      out[j] = i + j < r1 && i + j >= left && kept;
-      n += (hole[j] ? 1 : 0) + (out[j] ? 0x10000 : 0);
+      for (int j = 0; j < 4; ++j) {
+        if (k[j] > prefix || (k[j] == prefix && rank < need)) kept |= 1u << j;
+        rank += k[j] == prefix;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (k[j] >= prefix) kept |= 1u << j;
     }
+    // bits of the rows below `left`, and of those in the list
+    const uint32_t low = (1u << min(max(left - i, 0), 4)) - 1u, in = (1u << min(max(r1 - i, 0), 4)) - 1u;
+    const uint32_t hole = low & in & ~kept, out = ~low & in & kept;
+    const int n = __popc(hole) + (__popc(out) << 16);
     const int upto = warp_scan(n, lane);
     int hole_to = hole_at + ((upto - n) & 0xFFFF), out_to = out_at + ((upto - n) >> 16);
     const int total = __shfl_sync(0xffffffffu, upto, 31);
     hole_at += total & 0xFFFF;
     out_at += total >> 16;
     if (n != 0) {
-      const int at = pool_row(p, b, h, i);
+      const int at = q.pool();
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (hole[j]) to[hole_to++] = at < 0 ? -1 : at + j;
-        if (out[j]) src[out_to++] = at < 0 ? -1 : at + j;
+        if (hole >> j & 1) to[hole_to++] = at < 0 ? -1 : at + j;
+        if (out >> j & 1) src[out_to++] = at < 0 ? -1 : at + j;
       }
     }
   }
@@ -397,6 +473,22 @@ cudaError_t launch(void (*kernel)(A...), dim3 grid, int threads, size_t smem, cu
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+template <int THREADS>
+cudaError_t launch_select(const PagedEvictParams& p, int lists, int staged, cudaStream_t stream) {
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (!configured[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(paged_select_kernel<THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         kMaxStaged * (int)sizeof(uint32_t));
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
+  }
+  return launch(paged_select_kernel<THREADS>, dim3((unsigned)lists), THREADS, staged * sizeof(uint32_t), stream, p,
+                staged);
+}
+
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 }  // namespace
@@ -422,20 +514,10 @@ void paged_evict_plan(int n_seqs, int n_kv, long long max_rows, int budget, Page
 }
 
 cudaError_t launch_paged_evict(const PagedEvictParams& p, int sms, cudaStream_t stream) {
-  static bool configured[64] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  if (!configured[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(paged_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         kMaxStaged * (int)sizeof(uint32_t));
-    if (e != cudaSuccess) return e;
-    configured[dev] = true;
-  }
   const int lists = p.n_seqs * p.n_kv, cap = p.max_pages * p.page_size;
   const int staged = cap < kMaxStaged ? cap : kMaxStaged;
-  cudaError_t e = launch(paged_select_kernel, dim3((unsigned)lists), kSelThreads, staged * sizeof(uint32_t), stream, p,
-                         staged);
+  cudaError_t e = cap <= kShortList ? launch_select<256>(p, lists, staged, stream)
+                                    : launch_select<1024>(p, lists, staged, stream);
   if (e != cudaSuccess) return e;
   // as many CTAs as are resident (4 an SM), no more than a list has rows for
   const int want = (p.max_moves + kMoveWarps * kMoveRows - 1) / (kMoveWarps * kMoveRows), most = 4 * sms / lists;
