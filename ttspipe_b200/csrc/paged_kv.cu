@@ -139,55 +139,66 @@ __device__ __forceinline__ int warp_scan(int v, int lane) {  // inclusive
   return v;
 }
 
-// Add one to hist[digit] for every lane with `take`. `crowded`: most rows may share a
-// digit (new rows all have weight 0); then the lanes that share the first one's are one addition.
-__device__ __forceinline__ void count_digit(int* hist, int digit, bool take, bool crowded, int lane) {
-  if (crowded) {
-    const int theirs = __shfl_sync(0xffffffffu, digit, 0);  // by every lane, taking part or not
-    const bool same = take && digit == theirs;
-    const uint32_t m = __ballot_sync(0xffffffffu, same);
-    if (lane == __ffs(m) - 1) atomicAdd(&hist[digit], __popc(m));
-    take = take && !same;
-  }
-  if (take) atomicAdd(&hist[digit], 1);
+// Counts of digits that many rows may share (weight 0 of new rows, protected rows, a
+// digit 0 below a common prefix) are kept by each thread and added once a warp: as
+// single additions to one counter they would run one after another.
+__device__ __forceinline__ void add_shared(int* to, int n, int lane) {
+  n = __reduce_add_sync(0xffffffffu, n);
+  if (lane == 0 && n != 0) atomicAdd(to, n);
 }
 
+__device__ __forceinline__ int* cluster_peer(int* p, unsigned rank) {  // the same place in another CTA of the cluster
+  uint64_t out;
+  asm("mapa.u64 %0, %1, %2;" : "=l"(out) : "l"(reinterpret_cast<uint64_t>(p)), "r"(rank));
+  return reinterpret_cast<int*>(out);
+}
+
+// A list belongs to a cluster of `size` CTAs, each with an equal run of its rows.
 template <int kSelThreads>
 __global__ void __launch_bounds__(kSelThreads, kSelThreads == 1024 ? 1 : 4)
-    paged_select_kernel(const __grid_constant__ PagedEvictParams p, int staged_rows) {
+    paged_select_kernel(const __grid_constant__ PagedEvictParams p, int staged_rows, int size) {
   extern __shared__ __align__(16) uint32_t keys[];
-  __shared__ int hist[kBins];
+  __shared__ alignas(16) int hists[3][kBins];  // of each step: other CTAs of the cluster may still read the last one's
   __shared__ int part[3][32];
   __shared__ uint32_t s_prefix;
-  __shared__ int s_need, s_among, s_newest;
+  __shared__ int s_need, s_among, s_newest, s_sum[3];
   constexpr int kStep = kSelThreads * 4, kWarps = kSelThreads / 32, kMine = kBins / kSelThreads;
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int b = blockIdx.x / p.n_kv, h = blockIdx.x - b * p.n_kv;
+  const int list = blockIdx.x / size, rank = blockIdx.x - list * size;
+  const int b = list / p.n_kv, h = list - b * p.n_kv;
   const int cap = p.max_pages * p.page_size;
-  const int rows = min(max(p.lens[b], 0), cap), left = min(rows, p.budget);
-  const bool all = rows <= p.budget, staged = rows <= staged_rows;
-  if (tid == 0) {
+  const int total = min(max(p.lens[b], 0), cap), left = min(total, p.budget);
+  const bool all = total <= p.budget;
+  // this CTA's rows: [base, rows), in steps of the warps' runs
+  const int share = (total + size * kStep - 1) / (size * kStep) * kStep;
+  const int base = min(total, rank * share), rows = min(total, base + share);
+  const bool staged = share <= staged_rows;
+  if (tid == 0 && rank == 0) {
     if (h == 0) p.left[b] = left;
-    if (all) p.count[blockIdx.x] = 0;
-    s_newest = INT_MIN;
+    if (all) p.count[list] = 0;
   }
-  auto clear = [&]() {
-#pragma unroll
-    for (int j = 0; j < kMine; ++j) hist[tid + j * kSelThreads] = 0;
-  };
+  if (tid == 0) s_newest = INT_MIN;
   // of one value a warp: the sum up to the warp before this one's, and of all
   auto warps_before = [&](const int* v, int* total) -> int {
     const int upto = warp_scan(lane < kWarps ? v[lane] : 0, lane);
     *total = __shfl_sync(0xffffffffu, upto, 31);
     return warp ? __shfl_sync(0xffffffffu, upto, warp - 1) : 0;
   };
-  clear();
-  __syncthreads();
+  auto sync = [&]() {
+    if (size == 1) {
+      __syncthreads();
+    } else {
+      asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+      asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    }
+  };
+  for (int j = tid; j < 3 * kBins / 4; j += kSelThreads) reinterpret_cast<int4*>(hists)[j] = make_int4(0, 0, 0, 0);
+  sync();
 
   if (!all && p.recent > 0) {
     int newest = INT_MIN;
-    for (Quads q(p, b, h, tid * 4, kStep); q.row < rows;) {
+    for (Quads q(p, b, h, base + tid * 4, kStep); q.row < rows;) {
       int at[kSelDeep];
       int4 x[kSelDeep];
       const int first = q.row;
@@ -207,8 +218,9 @@ __global__ void __launch_bounds__(kSelThreads, kSelThreads == 1024 ? 1 : 4)
       }
     }
     newest = __reduce_max_sync(0xffffffffu, newest);
-    if (lane == 0) atomicMax(&s_newest, newest);
-    __syncthreads();
+    if (lane == 0)
+      for (int r = 0; r < size; ++r) atomicMax(size == 1 ? &s_newest : cluster_peer(&s_newest, r), newest);
+    sync();
   }
   // positions above this are among the newest (no position is above INT_MAX)
   const int guard = p.recent == 0 ? INT_MAX : s_newest < INT_MIN + p.recent ? INT_MIN : s_newest - p.recent;
@@ -224,14 +236,16 @@ __global__ void __launch_bounds__(kSelThreads, kSelThreads == 1024 ? 1 : 4)
                      *reinterpret_cast<const int4*>(p.position + at));
   };
   auto keys_at = [&](const Quads& q) -> uint4 {
-    return staged ? *reinterpret_cast<const uint4*>(keys + q.row) : keys_of(q.pool());
+    return staged ? *reinterpret_cast<const uint4*>(keys + (q.row - base)) : keys_of(q.pool());
   };
 
   // the first digit's histogram, and the weights and positions of the first rows into
   // their output (rows that move overwrite theirs afterwards)
   const bool copy_w = p.weight_out != p.weight, copy_p = p.position_out != p.position;
-  Quads q0(p, b, h, tid * 4, kStep);
-  for (int i0 = 0; i0 < rows; i0 += kSelDeep * kStep) {
+  int zeros = 0, guarded = 0;
+  const uint32_t kZero = weight_key(0.f);
+  Quads q0(p, b, h, base + tid * 4, kStep);
+  for (int i0 = base; i0 < rows; i0 += kSelDeep * kStep) {
     int at[kSelDeep];
     float4 w[kSelDeep];
     int4 x[kSelDeep];
@@ -261,44 +275,69 @@ __global__ void __launch_bounds__(kSelThreads, kSelThreads == 1024 ? 1 : 4)
       }
       if (all) continue;
       const uint4 k = at[u] < 0 ? make_uint4(0, 0, 0, 0) : keys_from(w[u], x[u]);
-      if (staged && i < rows) *reinterpret_cast<uint4*>(keys + i) = k;
-      count_digit(hist, k.x >> 21, i < rows, true, lane);
-      count_digit(hist, k.y >> 21, i + 1 < rows, true, lane);
-      count_digit(hist, k.z >> 21, i + 2 < rows, true, lane);
-      count_digit(hist, k.w >> 21, i + 3 < rows, true, lane);
+      if (staged && i < rows) *reinterpret_cast<uint4*>(keys + (i - base)) = k;
+      auto count = [&](uint32_t key, bool take) {
+        if (!take) return;
+        if (key == kZero)
+          ++zeros;
+        else if (key == 0xFFFFFFFFu)
+          ++guarded;
+        else
+          atomicAdd(&hists[0][key >> 21], 1);
+      };
+      count(k.x, i < rows);
+      count(k.y, i + 1 < rows);
+      count(k.z, i + 2 < rows);
+      count(k.w, i + 3 < rows);
     }
   }
-  if (all) {
+  if (all) {  // the whole cluster returns
     pdl_launch_dependents();
     return;
   }
-  __syncthreads();
+  add_shared(&hists[0][kZero >> 21], zeros, lane);
+  add_shared(&hists[0][kBins - 1], guarded, lane);
+  sync();
 
   uint32_t prefix = 0;  // the smallest kept key's leading digits
   int need = left;      // rows that stay among those with these digits
 #pragma unroll 1
   for (int step = 0; step < 3; ++step) {
+    int* hist = hists[step];
     if (step > 0) {
       const int shift = step == 1 ? 10 : 0, up = step == 1 ? 21 : 10;
       const uint32_t mask = step == 1 ? 2047u : 1023u;
-      const bool crowded = s_among > rows / 8;
-      clear();
-      __syncthreads();
-      Quads q(p, b, h, tid * 4, kStep);
-      for (int i0 = 0; i0 < rows; i0 += kStep, q.next(kStep)) {
+      int lowest = 0;
+      Quads q(p, b, h, base + tid * 4, kStep);
+      for (; q.row < rows; q.next(kStep)) {
         const int i = q.row;
-        const uint4 k = i < rows ? keys_at(q) : make_uint4(0, 0, 0, 0);
-        count_digit(hist, (k.x >> shift) & mask, i < rows && (k.x >> up) == prefix, crowded, lane);
-        count_digit(hist, (k.y >> shift) & mask, i + 1 < rows && (k.y >> up) == prefix, crowded, lane);
-        count_digit(hist, (k.z >> shift) & mask, i + 2 < rows && (k.z >> up) == prefix, crowded, lane);
-        count_digit(hist, (k.w >> shift) & mask, i + 3 < rows && (k.w >> up) == prefix, crowded, lane);
+        const uint4 k = keys_at(q);
+        auto count = [&](uint32_t key, bool take) {
+          if (!take || (key >> up) != prefix) return;
+          const uint32_t digit = (key >> shift) & mask;
+          if (digit == 0)
+            ++lowest;
+          else
+            atomicAdd(&hist[digit], 1);
+        };
+        count(k.x, true);
+        count(k.y, i + 1 < rows);
+        count(k.z, i + 2 < rows);
+        count(k.w, i + 3 < rows);
       }
-      __syncthreads();
+      __syncwarp();
+      add_shared(&hist[0], lowest, lane);
+      sync();
     }
     // falling digits, kMine to a thread
     int n[kMine], sum = 0, all_of;
 #pragma unroll
-    for (int j = 0; j < kMine; ++j) sum += n[j] = hist[kBins - 1 - kMine * tid - j];
+    for (int j = 0; j < kMine; ++j) {
+      const int at = kBins - 1 - kMine * tid - j;
+      n[j] = hist[at];
+      for (int r = 1; r < size; ++r) n[j] += *cluster_peer(&hist[at], (rank + r) % size);
+      sum += n[j];
+    }
     const int mine = warp_scan(sum, lane);
     if (lane == 31) part[0][warp] = mine;
     __syncthreads();
@@ -315,13 +354,17 @@ __global__ void __launch_bounds__(kSelThreads, kSelThreads == 1024 ? 1 : 4)
     __syncthreads();
     prefix = s_prefix;
     need = s_need;
+    if (s_among == need) {  // all of them stay, whatever their other digits
+      prefix <<= step == 0 ? 21 : step == 1 ? 10 : 0;
+      break;
+    }
   }
 
   // A key above prefix stays, and of the s_among equal ones the first `need` do. Each
   // warp takes a run of rows: it counts, the counts are summed up, then it writes.
   const bool ties = s_among != need;  // some equal rows go
-  const int run = ((rows + kStep - 1) / kStep) * 128;
-  const int r0 = warp * run, r1 = min(rows, r0 + run);
+  const int run = share / kWarps;
+  const int r0 = base + warp * run, r1 = min(rows, r0 + run);
   int gt[2] = {0, 0}, eq[2] = {0, 0};  // below `left`, and from it on
   for (Quads q(p, b, h, r0 + lane * 4, 128); q.row < r1; q.next(128)) {
     const uint4 k = keys_at(q);
@@ -355,12 +398,31 @@ __global__ void __launch_bounds__(kSelThreads, kSelThreads == 1024 ? 1 : 4)
     gt[s] = __reduce_add_sync(0xffffffffu, gt[s]);
     eq[s] = __reduce_add_sync(0xffffffffu, eq[s]);
   }
+  // of one value a warp: the sum up to this warp's, over the CTAs before this one too, and of all
+  auto before = [&](int k, int* of_all) -> int {
+    int mine;
+    const int at = warps_before(part[k], &mine);
+    if (size == 1) {
+      *of_all = mine;
+      return at;
+    }
+    if (tid == 0) s_sum[k] = mine;
+    sync();
+    int less = 0, sum = 0;
+    for (int r = 0; r < size; ++r) {
+      const int v = *cluster_peer(&s_sum[k], r);
+      if (r < rank) less += v;
+      sum += v;
+    }
+    *of_all = sum;
+    return less + at;
+  };
   int eq_at = 0;
   if (ties) {
     if (lane == 0) part[0][warp] = eq[0] + eq[1];
     __syncthreads();
     int all_of;
-    eq_at = warps_before(part[0], &all_of);
+    eq_at = before(0, &all_of);
     eq[1] = min(max(need - eq_at - eq[0], 0), eq[1]);
     eq[0] = min(max(need - eq_at, 0), eq[0]);
   }
@@ -370,111 +432,152 @@ __global__ void __launch_bounds__(kSelThreads, kSelThreads == 1024 ? 1 : 4)
   }
   __syncthreads();
   int holes, moved;  // equally many
-  int hole_at = warps_before(part[1], &holes), out_at = warps_before(part[2], &moved);
-  if (tid == 0) p.count[blockIdx.x] = moved;
-  int32_t* to = p.to + (size_t)blockIdx.x * p.max_moves;
-  int32_t* src = p.src + (size_t)blockIdx.x * p.max_moves;
+  int hole_at = before(1, &holes), out_at = before(2, &moved);
+  if (tid == 0 && rank == 0) p.count[list] = moved;
+  int32_t* to = p.to + (size_t)list * p.max_moves;
+  int32_t* src = p.src + (size_t)list * p.max_moves;
   Quads q(p, b, h, r0 + lane * 4, 128);
-  for (int i0 = r0; i0 < r1; i0 += 128, q.next(128)) {
-    const int i = q.row;
-    const uint4 k4 = i < r1 ? keys_at(q) : make_uint4(0, 0, 0, 0);
-    const uint32_t k[4] = {k4.x, k4.y, k4.z, k4.w};
-    uint32_t kept = 0;
-    if (ties) {
-      int n = 0;
+  for (int i0 = r0; i0 < r1; i0 += kSelDeep * 128) {
+    uint4 k[kSelDeep];
+    int at[kSelDeep];
+    const int first = q.row;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) n += i + j < r1 && k[j] == prefix;
-      const int upto = warp_scan(n, lane);
-      int rank = eq_at + upto - n;
-      eq_at += __shfl_sync(0xffffffffu, upto, 31);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (k[j] > prefix || (k[j] == prefix && rank < need)) kept |= 1u << j;
-        rank += k[j] == prefix;
+    for (int u = 0; u < kSelDeep; ++u, q.next(128)) {
+      k[u] = make_uint4(0, 0, 0, 0);
+      at[u] = -1;
+      if (q.row < r1) {
+        k[u] = keys_at(q);
+        at[u] = q.pool();
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (k[j] >= prefix) kept |= 1u << j;
     }
-    // bits of the rows below `left`, and of those in the list
-    const uint32_t low = (1u << min(max(left - i, 0), 4)) - 1u, in = (1u << min(max(r1 - i, 0), 4)) - 1u;
-    const uint32_t hole = low & in & ~kept, out = ~low & in & kept;
-    const int n = __popc(hole) + (__popc(out) << 16);
-    const int upto = warp_scan(n, lane);
-    int hole_to = hole_at + ((upto - n) & 0xFFFF), out_to = out_at + ((upto - n) >> 16);
-    const int total = __shfl_sync(0xffffffffu, upto, 31);
-    hole_at += total & 0xFFFF;
-    out_at += total >> 16;
-    if (n != 0) {
-      const int at = q.pool();
+    uint32_t hole[kSelDeep], out[kSelDeep];  // a bit for each row
+    int upto[kSelDeep];
+#pragma unroll
+    for (int u = 0; u < kSelDeep; ++u) {
+      const int i = first + u * 128;
+      const uint32_t kk[4] = {k[u].x, k[u].y, k[u].z, k[u].w};
+      const uint32_t low = (1u << min(max(left - i, 0), 4)) - 1u, in = (1u << min(max(r1 - i, 0), 4)) - 1u;
+      uint32_t kept = 0;
+      if (ties) {
+        uint32_t same = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) same |= (kk[j] == prefix ? 1u : 0u) << j;
+        same &= in;
+        const int n = __popc(same), before_me = warp_scan(n, lane);
+        int left_of = need - (eq_at + before_me - n);  // how many of the equal rows from here on stay
+        eq_at += __shfl_sync(0xffffffffu, before_me, 31);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (kk[j] > prefix || ((same >> j & 1) && left_of > 0)) kept |= 1u << j;
+          left_of -= same >> j & 1;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) kept |= (kk[j] >= prefix ? 1u : 0u) << j;
+      }
+      hole[u] = low & in & ~kept;
+      out[u] = ~low & in & kept;
+      upto[u] = warp_scan(__popc(hole[u]) + (__popc(out[u]) << 16), lane);
+    }
+#pragma unroll
+    for (int u = 0; u < kSelDeep; ++u) {
+      const int mine = upto[u] - (__popc(hole[u]) + (__popc(out[u]) << 16)), sum = __shfl_sync(0xffffffffu, upto[u], 31);
+      int hole_to = hole_at + (mine & 0xFFFF), out_to = out_at + (mine >> 16);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (hole >> j & 1) to[hole_to++] = at < 0 ? -1 : at + j;
-        if (out >> j & 1) src[out_to++] = at < 0 ? -1 : at + j;
+        if (hole[u] >> j & 1) to[hole_to++] = at[u] < 0 ? -1 : at[u] + j;
+        if (out[u] >> j & 1) src[out_to++] = at[u] < 0 ? -1 : at[u] + j;
       }
+      hole_at += sum & 0xFFFF;
+      out_at += sum >> 16;
     }
   }
+  if (size > 1) sync();  // no CTA leaves while another may read its sums
   pdl_launch_dependents();
 }
 
 constexpr int kMoveWarps = 8;
 constexpr int kMoveRows = 8;  // rows that a warp has in flight
+constexpr int kMovePiece = kMoveWarps * kMoveRows;
 
 // Eight rows to a warp at a time: half of it copies the key rows, half the value rows,
-// 16 bytes a lane.
-__global__ void __launch_bounds__(kMoveWarps * 32) paged_move_kernel(const __grid_constant__ PagedEvictParams p) {
+// 16 bytes a lane; the next eight are looked up meanwhile. The lists' pieces of 64 rows
+// are dealt out to the CTAs one list after another, so that lists of unequal length spread.
+__global__ void __launch_bounds__(kMoveWarps * 32, 4)
+    paged_move_kernel(const __grid_constant__ PagedEvictParams p) {
   pdl_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int b = blockIdx.y / p.n_kv;
-  if (blockIdx.y == b * p.n_kv && blockIdx.x == 0 && threadIdx.x == 0) p.lens_out[b] = p.left[b];
-  const int n = p.count[blockIdx.y];
-  const int32_t* to = p.to + (size_t)blockIdx.y * p.max_moves;
-  const int32_t* src = p.src + (size_t)blockIdx.y * p.max_moves;
+  const int lane = threadIdx.x & 31, mine = (threadIdx.x >> 5) * kMoveRows + lane;
+  const int lists = p.n_seqs * p.n_kv;
+  for (int b = blockIdx.x * kMoveWarps * 32 + threadIdx.x; b < p.n_seqs; b += gridDim.x * kMoveWarps * 32)
+    p.lens_out[b] = p.left[b];
   uint4* pool = reinterpret_cast<uint4*>(lane < 16 ? p.k : p.v) + (lane & 15);
-  for (int i = (blockIdx.x * kMoveWarps + warp) * kMoveRows; i < n; i += gridDim.x * kMoveWarps * kMoveRows) {
-    int from = -1, at = -1;
-    if (lane < kMoveRows && i + lane < n) {
-      from = src[i + lane];
-      at = to[i + lane];
+  const int step_list = gridDim.x % lists, step_row = gridDim.x / lists * kMovePiece;
+  int list = blockIdx.x % lists, row = blockIdx.x / lists * kMovePiece;
+  auto fetch = [&](int& from, int& at) {  // the next rows of the warp, one to a lane
+    from = at = -1;
+    if (lane < kMoveRows && row + mine < p.max_moves && row + mine < p.count[list]) {
+      from = p.src[(size_t)list * p.max_moves + row + mine];
+      at = p.to[(size_t)list * p.max_moves + row + mine];
+      if (from < 0 || at < 0) from = at = -1;
     }
-    if (from < 0 || at < 0) from = at = -1;
+    list += step_list;
+    row += step_row;
+    if (list >= lists) {
+      list -= lists;
+      row += kMovePiece;
+    }
+  };
+  int from, at, from1, at1;
+  bool more = row < p.max_moves;
+  for (fetch(from, at); more; from = from1, at = at1) {
+    more = row < p.max_moves;
     uint4 x[kMoveRows];
+    float w;
+    int pos;
+    if (at >= 0) {
+      w = p.weight[from];
+      pos = p.position[from];
+    }
 #pragma unroll
     for (int j = 0; j < kMoveRows; ++j) {
       const int f = __shfl_sync(0xffffffffu, from, j);
-      if (f >= 0) x[j] = pool[(size_t)f * (kD / 8)];
+      if (f >= 0) x[j] = ld_stream_u4(pool + (size_t)f * (kD / 8));  // no row is both read and written
     }
+    fetch(from1, at1);
     if (at >= 0) {
-      p.weight_out[at] = p.weight[from];
-      p.position_out[at] = p.position[from];
+      p.weight_out[at] = w;
+      p.position_out[at] = pos;
     }
 #pragma unroll
     for (int j = 0; j < kMoveRows; ++j) {
       const int t = __shfl_sync(0xffffffffu, at, j);
-      if (t >= 0) pool[(size_t)t * (kD / 8)] = x[j];
+      if (t >= 0) __stcs(pool + (size_t)t * (kD / 8), x[j]);
     }
   }
   pdl_launch_dependents();
 }
 
 template <typename... A>
-cudaError_t launch(void (*kernel)(A...), dim3 grid, int threads, size_t smem, cudaStream_t stream, A... args) {
+cudaError_t launch(void (*kernel)(A...), int grid, int threads, size_t smem, int cluster, cudaStream_t stream,
+                   A... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.dynamicSmemBytes = smem;
-  cfg.gridDim = grid;
+  cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3((unsigned)threads);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 template <int THREADS>
-cudaError_t launch_select(const PagedEvictParams& p, int lists, int staged, cudaStream_t stream) {
+cudaError_t launch_select(const PagedEvictParams& p, int lists, int staged, int cluster, cudaStream_t stream) {
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -485,8 +588,8 @@ cudaError_t launch_select(const PagedEvictParams& p, int lists, int staged, cuda
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
-  return launch(paged_select_kernel<THREADS>, dim3((unsigned)lists), THREADS, staged * sizeof(uint32_t), stream, p,
-                staged);
+  return launch(paged_select_kernel<THREADS>, lists * cluster, THREADS, staged * sizeof(uint32_t), cluster, stream, p,
+                staged, cluster);
 }
 
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -496,8 +599,8 @@ size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 cudaError_t launch_paged_write(const PagedWriteParams& p, int sms, bool f16, cudaStream_t stream) {
   const long long items = (long long)p.n_tokens * (p.n_head + 2 * p.n_kv);
   const long long want = (items + kWriteWarps - 1) / kWriteWarps, most = 16LL * sms;
-  return launch(f16 ? paged_write_kernel<true> : paged_write_kernel<false>, dim3((unsigned)(want < most ? want : most)),
-                kWriteWarps * 32, 0, stream, p);
+  return launch(f16 ? paged_write_kernel<true> : paged_write_kernel<false>, (int)(want < most ? want : most),
+                kWriteWarps * 32, 0, 1, stream, p);
 }
 
 void paged_evict_plan(int n_seqs, int n_kv, long long max_rows, int budget, PagedEvictPlan* plan) {
@@ -515,14 +618,18 @@ void paged_evict_plan(int n_seqs, int n_kv, long long max_rows, int budget, Page
 
 cudaError_t launch_paged_evict(const PagedEvictParams& p, int sms, cudaStream_t stream) {
   const int lists = p.n_seqs * p.n_kv, cap = p.max_pages * p.page_size;
-  const int staged = cap < kMaxStaged ? cap : kMaxStaged;
-  cudaError_t e = cap <= kShortList ? launch_select<256>(p, lists, staged, stream)
-                                    : launch_select<1024>(p, lists, staged, stream);
+  // a cluster for a list while there are SMs for it and each of its CTAs has rows for all its threads
+  int cluster = 1;
+  while (cluster < 8 && lists * cluster * 2 <= sms && cap >= cluster * 2 * kShortList) cluster *= 2;
+  const int threads = cap <= kShortList ? 256 : 1024;
+  const int step = cluster * threads * 4, share = (cap + step - 1) / step * threads * 4;
+  const int staged = share < kMaxStaged ? share : kMaxStaged;
+  cudaError_t e = threads == 256 ? launch_select<256>(p, lists, staged, cluster, stream)
+                                 : launch_select<1024>(p, lists, staged, cluster, stream);
   if (e != cudaSuccess) return e;
-  // as many CTAs as are resident (4 an SM), no more than a list has rows for
-  const int want = (p.max_moves + kMoveWarps * kMoveRows - 1) / (kMoveWarps * kMoveRows), most = 4 * sms / lists;
-  const int x = want < most ? want : most;
-  return launch(paged_move_kernel, dim3((unsigned)(x < 1 ? 1 : x), (unsigned)lists), kMoveWarps * 32, 0, stream, p);
+  const long long want = (long long)lists * ((p.max_moves + kMovePiece - 1) / kMovePiece), most = 4LL * sms;  // all resident
+  return launch(paged_move_kernel, (int)(want < 1 ? 1 : want < most ? want : most), kMoveWarps * 32, 0, 1,
+                stream, p);
 }
 
 }  // namespace nf4b
