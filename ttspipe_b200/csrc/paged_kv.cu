@@ -88,13 +88,11 @@ __global__ void __launch_bounds__(kWriteWarps * 32) paged_write_kernel(const __g
 // equally many, the two sets are disjoint, and attention does not depend on the order of rows
 // (the rotary is in the keys), so nothing else has to move.
 //
-// paged_select_kernel, one CTA a list, finds the smallest kept key digit by digit from
-// the top (11, 11 and 10 bits, a histogram each) and lists the moves;
+// paged_select_kernel, one CTA or one cluster of CTAs a list, finds the smallest kept key digit by digit
+// from the top (11, 11 and 10 bits, a histogram each) and lists the moves;
 // paged_move_kernel makes them.
 constexpr int kBins = 2048;
-constexpr int kSelDeep = 4;  // groups of four rows that a thread requests at once
-constexpr int kShortList = 8192;  // lists up to this get 256 threads, so that several share an SM; longer ones 1024
-constexpr int kMaxStaged = 48 * 1024;  // rows whose keys lie in shared memory; longer lists are read again for each digit
+constexpr int kDeep = 4;  // groups of 128 rows that a warp requests at once
 
 // Weights in rising order as unsigned integers; 0xFFFFFFFF (no weight maps there,
 // NaN being taken as -inf) is for the protected rows, 0 for rows without a page.
@@ -104,18 +102,18 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// Walks a list four rows at a time (they lie in one page) with a constant step, the
-// page and the row in it carried along instead of divided out.
+// Walks a list in groups of 128 rows, four consecutive ones (they lie in one page) to a
+// lane; the page and the row in it are carried along instead of divided out.
 struct Quads {
   const int32_t* table;
   int h, n_kv, n_pages, page_size, step_pages, step_rows;
   int row, page, at;
-  __device__ __forceinline__ Quads(const PagedEvictParams& p, int b, int head, int first, int step)
+  __device__ __forceinline__ Quads(const PagedEvictParams& p, int b, int head, int first)
       : table(p.table + (size_t)b * p.max_pages), h(head), n_kv(p.n_kv), n_pages(p.n_pages), page_size(p.page_size),
-        step_pages(step / p.page_size), step_rows(step % p.page_size), row(first), page(first / p.page_size),
+        step_pages(128 / p.page_size), step_rows(128 % p.page_size), row(first), page(first / p.page_size),
         at(first % p.page_size) {}
-  __device__ __forceinline__ void next(int step) {
-    row += step;
+  __device__ __forceinline__ void next() {
+    row += 128;
     page += step_pages;
     at += step_rows;
     if (at >= page_size) {
@@ -153,16 +151,17 @@ __device__ __forceinline__ int* cluster_peer(int* p, unsigned rank) {  // the sa
   return reinterpret_cast<int*>(out);
 }
 
-// A list belongs to a cluster of `size` CTAs, each with an equal run of its rows.
-template <int kSelThreads>
-__global__ void __launch_bounds__(kSelThreads, kSelThreads == 1024 ? 1 : 4)
-    paged_select_kernel(const __grid_constant__ PagedEvictParams p, int staged_rows, int size) {
-  extern __shared__ __align__(16) uint32_t keys[];
+// A list belongs to a cluster of `size` CTAs, each with an equal share of its rows, and
+// each warp of them with a run of that. kOnce: a run is at most kDeep * 128 rows, whose
+// keys stay in registers; longer runs are read again (from L2) for every step.
+template <int kThreads, bool kOnce>
+__global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : 4)
+    paged_select_kernel(const __grid_constant__ PagedEvictParams p, int size) {
   __shared__ alignas(16) int hists[3][kBins];  // of each step: other CTAs of the cluster may still read the last one's
   __shared__ int part[3][32];
   __shared__ uint32_t s_prefix;
   __shared__ int s_need, s_among, s_newest, s_sum[3];
-  constexpr int kStep = kSelThreads * 4, kWarps = kSelThreads / 32, kMine = kBins / kSelThreads;
+  constexpr int kWarps = kThreads / 32, kMine = kBins / kThreads;
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int list = blockIdx.x / size, rank = blockIdx.x - list * size;
@@ -170,47 +169,75 @@ __global__ void __launch_bounds__(kSelThreads, kSelThreads == 1024 ? 1 : 4)
   const int cap = p.max_pages * p.page_size;
   const int total = min(max(p.lens[b], 0), cap), left = min(total, p.budget);
   const bool all = total <= p.budget;
-  // this CTA's rows: [base, rows), in steps of the warps' runs
-  const int share = (total + size * kStep - 1) / (size * kStep) * kStep;
-  const int base = min(total, rank * share), rows = min(total, base + share);
-  const bool staged = share <= staged_rows;
-  if (tid == 0 && rank == 0) {
-    if (h == 0) p.left[b] = left;
-    if (all) p.count[list] = 0;
+  const int run = (total + size * kWarps * 128 - 1) / (size * kWarps * 128) * 128;
+  const int r0 = min(total, (rank * kWarps + warp) * run), r1 = min(total, r0 + run);  // this warp's rows
+  if (tid == 0) {
+    s_newest = INT_MIN;
+    if (rank == 0 && h == 0) p.left[b] = left;
+    if (rank == 0 && all) p.count[list] = 0;
   }
-  if (tid == 0) s_newest = INT_MIN;
-  // of one value a warp: the sum up to the warp before this one's, and of all
-  auto warps_before = [&](const int* v, int* total) -> int {
-    const int upto = warp_scan(lane < kWarps ? v[lane] : 0, lane);
-    *total = __shfl_sync(0xffffffffu, upto, 31);
-    return warp ? __shfl_sync(0xffffffffu, upto, warp - 1) : 0;
-  };
   auto sync = [&]() {
     if (size == 1) {
       __syncthreads();
     } else {
-      asm volatile("barrier.cluster.arrive.release;" ::: "memory");
-      asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+      __syncwarp();
+      asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+      asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
   };
-  for (int j = tid; j < 3 * kBins / 4; j += kSelThreads) reinterpret_cast<int4*>(hists)[j] = make_int4(0, 0, 0, 0);
-  sync();
+  for (int j = tid; j < 3 * kBins / 4; j += kThreads) reinterpret_cast<int4*>(hists)[j] = make_int4(0, 0, 0, 0);
+
+  // a batch: kDeep groups of four rows of this lane
+  int at[kDeep];  // their pool rows; -1 past the run and where no page is assigned
+  float4 w[kDeep];
+  int4 x[kDeep];
+  uint4 k[kDeep];
+  auto load = [&](Quads& q, bool weights) {
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u, q.next()) at[u] = q.row < r1 ? q.pool() : -1;
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u)
+      if (at[u] >= 0) {
+        x[u] = *reinterpret_cast<const int4*>(p.position + at[u]);
+        if (weights) w[u] = *reinterpret_cast<const float4*>(p.weight + at[u]);
+      }
+  };
+  // the weights and positions of the first rows into their output (rows that move
+  // overwrite theirs afterwards)
+  const bool copy_w = p.weight_out != p.weight, copy_p = p.position_out != p.position;
+  auto copy = [&](int first) {
+    if (!copy_w && !copy_p) return;
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u) {
+      const int i = first + u * 128;
+      if (i >= left || at[u] < 0) continue;
+      if (i + 4 <= left) {
+        if (copy_w) *reinterpret_cast<float4*>(p.weight_out + at[u]) = w[u];
+        if (copy_p) *reinterpret_cast<int4*>(p.position_out + at[u]) = x[u];
+      } else {
+        for (int j = 0; j < left - i; ++j) {
+          if (copy_w) p.weight_out[at[u] + j] = p.weight[at[u] + j];
+          if (copy_p) p.position_out[at[u] + j] = p.position[at[u] + j];
+        }
+      }
+    }
+  };
+  if (kOnce) {
+    Quads q(p, b, h, r0 + lane * 4);
+    load(q, true);
+    copy(r0 + lane * 4);
+  }
+  __syncthreads();
 
   if (!all && p.recent > 0) {
     int newest = INT_MIN;
-    for (Quads q(p, b, h, base + tid * 4, kStep); q.row < rows;) {
-      int at[kSelDeep];
-      int4 x[kSelDeep];
-      const int first = q.row;
+    Quads q(p, b, h, r0 + lane * 4);
+    for (int i0 = r0; i0 < r1; i0 += kDeep * 128) {
+      if (!kOnce) load(q, false);
 #pragma unroll
-      for (int u = 0; u < kSelDeep; ++u, q.next(kStep)) at[u] = q.row < rows ? q.pool() : -1;
-#pragma unroll
-      for (int u = 0; u < kSelDeep; ++u)
-        if (at[u] >= 0) x[u] = *reinterpret_cast<const int4*>(p.position + at[u]);
-#pragma unroll
-      for (int u = 0; u < kSelDeep; ++u) {
+      for (int u = 0; u < kDeep; ++u) {
         if (at[u] < 0) continue;
-        const int n = rows - first - u * kStep;  // at least one
+        const int n = r1 - (i0 + u * 128 + lane * 4);  // at least one
         newest = max(newest, x[u].x);
         if (n > 1) newest = max(newest, x[u].y);
         if (n > 2) newest = max(newest, x[u].z);
@@ -218,64 +245,44 @@ __global__ void __launch_bounds__(kSelThreads, kSelThreads == 1024 ? 1 : 4)
       }
     }
     newest = __reduce_max_sync(0xffffffffu, newest);
-    if (lane == 0)
-      for (int r = 0; r < size; ++r) atomicMax(size == 1 ? &s_newest : cluster_peer(&s_newest, r), newest);
+    if (lane == 0) atomicMax(&s_newest, newest);
     sync();
   }
+  int newest = s_newest;
+  for (int r = 1; r < size && !all && p.recent > 0; ++r) newest = max(newest, *cluster_peer(&s_newest, (rank + r) % size));
   // positions above this are among the newest (no position is above INT_MAX)
-  const int guard = p.recent == 0 ? INT_MAX : s_newest < INT_MIN + p.recent ? INT_MIN : s_newest - p.recent;
-  auto keys_from = [&](const float4& w, const int4& x) -> uint4 {
+  const int guard = p.recent == 0 ? INT_MAX : newest < INT_MIN + p.recent ? INT_MIN : newest - p.recent;
+  auto to_keys = [&]() {
     auto key = [&](float wt, int pos) -> uint32_t {
       return pos < p.sink || pos > guard ? 0xFFFFFFFFu : weight_key(wt);
     };
-    return make_uint4(key(w.x, x.x), key(w.y, x.y), key(w.z, x.z), key(w.w, x.w));
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u)
+      k[u] = at[u] < 0 ? make_uint4(0, 0, 0, 0)
+                       : make_uint4(key(w[u].x, x[u].x), key(w[u].y, x[u].y), key(w[u].z, x[u].z), key(w[u].w, x[u].w));
   };
-  auto keys_of = [&](int at) -> uint4 {
-    if (at < 0) return make_uint4(0, 0, 0, 0);
-    return keys_from(*reinterpret_cast<const float4*>(p.weight + at),
-                     *reinterpret_cast<const int4*>(p.position + at));
+  // f(u, i) for every group of the run, its first row i, with k[u] and at[u]
+  auto each_batch = [&](auto f) {
+    Quads q(p, b, h, r0 + lane * 4);
+    for (int i0 = r0; i0 < r1; i0 += kDeep * 128) {
+      if (!kOnce) {
+        load(q, true);
+        to_keys();
+      }
+      f(i0 + lane * 4);
+    }
   };
-  auto keys_at = [&](const Quads& q) -> uint4 {
-    return staged ? *reinterpret_cast<const uint4*>(keys + (q.row - base)) : keys_of(q.pool());
-  };
+  if (kOnce) to_keys();
 
-  // the first digit's histogram, and the weights and positions of the first rows into
-  // their output (rows that move overwrite theirs afterwards)
-  const bool copy_w = p.weight_out != p.weight, copy_p = p.position_out != p.position;
-  int zeros = 0, guarded = 0;
+  // the first digit's histogram
   const uint32_t kZero = weight_key(0.f);
-  Quads q0(p, b, h, base + tid * 4, kStep);
-  for (int i0 = base; i0 < rows; i0 += kSelDeep * kStep) {
-    int at[kSelDeep];
-    float4 w[kSelDeep];
-    int4 x[kSelDeep];
-    const int first = q0.row;
+  int zeros = 0, guarded = 0;
+  each_batch([&](int first) {
+    if (!kOnce) copy(first);
+    if (all) return;
 #pragma unroll
-    for (int u = 0; u < kSelDeep; ++u, q0.next(kStep)) at[u] = q0.row < rows ? q0.pool() : -1;
-#pragma unroll
-    for (int u = 0; u < kSelDeep; ++u)
-      if (at[u] >= 0) {
-        w[u] = *reinterpret_cast<const float4*>(p.weight + at[u]);
-        x[u] = *reinterpret_cast<const int4*>(p.position + at[u]);
-      }
-#pragma unroll
-    for (int u = 0; u < kSelDeep; ++u) {
-      const int i = first + u * kStep;
-      if (i0 + u * kStep >= rows) break;
-      if (i < left && at[u] >= 0 && (copy_w || copy_p)) {
-        if (i + 4 <= left) {
-          if (copy_w) *reinterpret_cast<float4*>(p.weight_out + at[u]) = w[u];
-          if (copy_p) *reinterpret_cast<int4*>(p.position_out + at[u]) = x[u];
-        } else {
-          for (int j = 0; j < left - i; ++j) {
-            if (copy_w) p.weight_out[at[u] + j] = p.weight[at[u] + j];
-            if (copy_p) p.position_out[at[u] + j] = p.position[at[u] + j];
-          }
-        }
-      }
-      if (all) continue;
-      const uint4 k = at[u] < 0 ? make_uint4(0, 0, 0, 0) : keys_from(w[u], x[u]);
-      if (staged && i < rows) *reinterpret_cast<uint4*>(keys + (i - base)) = k;
+    for (int u = 0; u < kDeep; ++u) {
+      const int i = first + u * 128;
       auto count = [&](uint32_t key, bool take) {
         if (!take) return;
         if (key == kZero)
@@ -285,12 +292,12 @@ __global__ void __launch_bounds__(kSelThreads, kSelThreads == 1024 ? 1 : 4)
         else
           atomicAdd(&hists[0][key >> 21], 1);
       };
-      count(k.x, i < rows);
-      count(k.y, i + 1 < rows);
-      count(k.z, i + 2 < rows);
-      count(k.w, i + 3 < rows);
+      count(k[u].x, i < r1);
+      count(k[u].y, i + 1 < r1);
+      count(k[u].z, i + 2 < r1);
+      count(k[u].w, i + 3 < r1);
     }
-  }
+  });
   if (all) {  // the whole cluster returns
     pdl_launch_dependents();
     return;
@@ -299,6 +306,12 @@ __global__ void __launch_bounds__(kSelThreads, kSelThreads == 1024 ? 1 : 4)
   add_shared(&hists[0][kBins - 1], guarded, lane);
   sync();
 
+  // of one value a warp: the sum up to the warp before this one's, and of all
+  auto warps_before = [&](const int* v, int* sum) -> int {
+    const int upto = warp_scan(lane < kWarps ? v[lane] : 0, lane);
+    *sum = __shfl_sync(0xffffffffu, upto, 31);
+    return warp ? __shfl_sync(0xffffffffu, upto, warp - 1) : 0;
+  };
   uint32_t prefix = 0;  // the smallest kept key's leading digits
   int need = left;      // rows that stay among those with these digits
 #pragma unroll 1
@@ -308,23 +321,24 @@ __global__ void __launch_bounds__(kSelThreads, kSelThreads == 1024 ? 1 : 4)
       const int shift = step == 1 ? 10 : 0, up = step == 1 ? 21 : 10;
       const uint32_t mask = step == 1 ? 2047u : 1023u;
       int lowest = 0;
-      Quads q(p, b, h, base + tid * 4, kStep);
-      for (; q.row < rows; q.next(kStep)) {
-        const int i = q.row;
-        const uint4 k = keys_at(q);
-        auto count = [&](uint32_t key, bool take) {
-          if (!take || (key >> up) != prefix) return;
-          const uint32_t digit = (key >> shift) & mask;
-          if (digit == 0)
-            ++lowest;
-          else
-            atomicAdd(&hist[digit], 1);
-        };
-        count(k.x, true);
-        count(k.y, i + 1 < rows);
-        count(k.z, i + 2 < rows);
-        count(k.w, i + 3 < rows);
-      }
+      each_batch([&](int first) {
+#pragma unroll
+        for (int u = 0; u < kDeep; ++u) {
+          const int i = first + u * 128;
+          auto count = [&](uint32_t key, bool take) {
+            if (!take || (key >> up) != prefix) return;
+            const uint32_t digit = (key >> shift) & mask;
+            if (digit == 0)
+              ++lowest;
+            else
+              atomicAdd(&hist[digit], 1);
+          };
+          count(k[u].x, i < r1);
+          count(k[u].y, i + 1 < r1);
+          count(k[u].z, i + 2 < r1);
+          count(k[u].w, i + 3 < r1);
+        }
+      });
       __syncwarp();
       add_shared(&hist[0], lowest, lane);
       sync();
@@ -332,12 +346,14 @@ __global__ void __launch_bounds__(kSelThreads, kSelThreads == 1024 ? 1 : 4)
     // falling digits, kMine to a thread
     int n[kMine], sum = 0, all_of;
 #pragma unroll
-    for (int j = 0; j < kMine; ++j) {
-      const int at = kBins - 1 - kMine * tid - j;
-      n[j] = hist[at];
-      for (int r = 1; r < size; ++r) n[j] += *cluster_peer(&hist[at], (rank + r) % size);
-      sum += n[j];
+    for (int j = 0; j < kMine; ++j) n[j] = hist[kBins - 1 - kMine * tid - j];
+    for (int r = 1; r < size; ++r) {
+      const int* other = cluster_peer(hist, (rank + r) % size);
+#pragma unroll
+      for (int j = 0; j < kMine; ++j) n[j] += other[kBins - 1 - kMine * tid - j];
     }
+#pragma unroll
+    for (int j = 0; j < kMine; ++j) sum += n[j];
     const int mine = warp_scan(sum, lane);
     if (lane == 31) part[0][warp] = mine;
     __syncthreads();
@@ -360,100 +376,77 @@ __global__ void __launch_bounds__(kSelThreads, kSelThreads == 1024 ? 1 : 4)
     }
   }
 
-  // A key above prefix stays, and of the s_among equal ones the first `need` do. Each
-  // warp takes a run of rows: it counts, the counts are summed up, then it writes.
-  const bool ties = s_among != need;  // some equal rows go
-  const int run = share / kWarps;
-  const int r0 = base + warp * run, r1 = min(rows, r0 + run);
-  int gt[2] = {0, 0}, eq[2] = {0, 0};  // below `left`, and from it on
-  for (Quads q(p, b, h, r0 + lane * 4, 128); q.row < r1; q.next(128)) {
-    const uint4 k = keys_at(q);
-    const int i = q.row;
-    if (i + 4 <= left || (i >= left && i + 4 <= rows)) {
-      const int n = (k.x > prefix) + (k.y > prefix) + (k.z > prefix) + (k.w > prefix);
-      const int e = (k.x == prefix) + (k.y == prefix) + (k.z == prefix) + (k.w == prefix);
-      if (i < left) {
-        gt[0] += n;
-        eq[0] += e;
-      } else {
-        gt[1] += n;
-        eq[1] += e;
-      }
-    } else {
-      const uint32_t kk[4] = {k.x, k.y, k.z, k.w};
+  // A key above prefix stays, and of the s_among ones from it on the first `need` do. Each
+  // warp counts in its run, the counts are summed up, then it writes.
+  const bool ties = s_among != need;  // some of the rows whose key is prefix go
+  int gt[2] = {0, 0}, eq[2] = {0, 0};  // rows above prefix and with it, below `left` and from it on
+  each_batch([&](int first) {
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u) {
+      const int i = first + u * 128;
+      const uint32_t kk[4] = {k[u].x, k[u].y, k[u].z, k[u].w};
+      const uint32_t low = (1u << min(max(left - i, 0), 4)) - 1u, in = (1u << min(max(r1 - i, 0), 4)) - 1u;
+      uint32_t more = 0, same = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (i + j < left) {
-          gt[0] += kk[j] > prefix;
-          eq[0] += kk[j] == prefix;
-        } else if (i + j < rows) {
-          gt[1] += kk[j] > prefix;
-          eq[1] += kk[j] == prefix;
-        }
+        more |= (kk[j] > prefix ? 1u : 0u) << j;
+        same |= (kk[j] == prefix ? 1u : 0u) << j;
       }
+      gt[0] += __popc(more & in & low);
+      gt[1] += __popc(more & in & ~low);
+      eq[0] += __popc(same & in & low);
+      eq[1] += __popc(same & in & ~low);
     }
-  }
+  });
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     gt[s] = __reduce_add_sync(0xffffffffu, gt[s]);
     eq[s] = __reduce_add_sync(0xffffffffu, eq[s]);
   }
-  // of one value a warp: the sum up to this warp's, over the CTAs before this one too, and of all
-  auto before = [&](int k, int* of_all) -> int {
-    int mine;
-    const int at = warps_before(part[k], &mine);
-    if (size == 1) {
-      *of_all = mine;
-      return at;
+  // of part[v] .. part[last], one value a warp: the sums up to this warp's, over the CTAs
+  // before this one too, and of all
+  auto before = [&](int v, int last, int* upto, int* of_all) {
+    for (int j = v; j <= last; ++j) {
+      upto[j - v] = warps_before(part[j], &of_all[j - v]);
+      if (size > 1 && tid == 0) s_sum[j] = of_all[j - v];
     }
-    if (tid == 0) s_sum[k] = mine;
+    if (size == 1) return;
     sync();
-    int less = 0, sum = 0;
-    for (int r = 0; r < size; ++r) {
-      const int v = *cluster_peer(&s_sum[k], r);
-      if (r < rank) less += v;
-      sum += v;
+    for (int j = v; j <= last; ++j) {
+      of_all[j - v] = 0;
+      for (int r = 0; r < size; ++r) {
+        const int theirs = *cluster_peer(&s_sum[j], r);
+        if (r < rank) upto[j - v] += theirs;
+        of_all[j - v] += theirs;
+      }
     }
-    *of_all = sum;
-    return less + at;
   };
   int eq_at = 0;
   if (ties) {
     if (lane == 0) part[0][warp] = eq[0] + eq[1];
     __syncthreads();
     int all_of;
-    eq_at = before(0, &all_of);
+    before(0, 0, &eq_at, &all_of);
     eq[1] = min(max(need - eq_at - eq[0], 0), eq[1]);
     eq[0] = min(max(need - eq_at, 0), eq[0]);
   }
+  // a place that falls free below `left` and a row that moves down there are counted together
   if (lane == 0) {
     part[1][warp] = max(min(r1, left) - r0, 0) - gt[0] - eq[0];
     part[2][warp] = gt[1] + eq[1];
   }
   __syncthreads();
-  int holes, moved;  // equally many
-  int hole_at = before(1, &holes), out_at = before(2, &moved);
-  if (tid == 0 && rank == 0) p.count[list] = moved;
+  int upto[2], of_all[2];  // equally many of both
+  before(1, 2, upto, of_all);
+  int hole_at = upto[0], out_at = upto[1];
+  if (tid == 0 && rank == 0) p.count[list] = of_all[1];
   int32_t* to = p.to + (size_t)list * p.max_moves;
   int32_t* src = p.src + (size_t)list * p.max_moves;
-  Quads q(p, b, h, r0 + lane * 4, 128);
-  for (int i0 = r0; i0 < r1; i0 += kSelDeep * 128) {
-    uint4 k[kSelDeep];
-    int at[kSelDeep];
-    const int first = q.row;
+  each_batch([&](int first) {
+    uint32_t hole[kDeep], out[kDeep];  // a bit for each row
+    int upto[kDeep];
 #pragma unroll
-    for (int u = 0; u < kSelDeep; ++u, q.next(128)) {
-      k[u] = make_uint4(0, 0, 0, 0);
-      at[u] = -1;
-      if (q.row < r1) {
-        k[u] = keys_at(q);
-        at[u] = q.pool();
-      }
-    }
-    uint32_t hole[kSelDeep], out[kSelDeep];  // a bit for each row
-    int upto[kSelDeep];
-#pragma unroll
-    for (int u = 0; u < kSelDeep; ++u) {
+    for (int u = 0; u < kDeep; ++u) {
       const int i = first + u * 128;
       const uint32_t kk[4] = {k[u].x, k[u].y, k[u].z, k[u].w};
       const uint32_t low = (1u << min(max(left - i, 0), 4)) - 1u, in = (1u << min(max(r1 - i, 0), 4)) - 1u;
@@ -480,7 +473,7 @@ __global__ void __launch_bounds__(kSelThreads, kSelThreads == 1024 ? 1 : 4)
       upto[u] = warp_scan(__popc(hole[u]) + (__popc(out[u]) << 16), lane);
     }
 #pragma unroll
-    for (int u = 0; u < kSelDeep; ++u) {
+    for (int u = 0; u < kDeep; ++u) {
       const int mine = upto[u] - (__popc(hole[u]) + (__popc(out[u]) << 16)), sum = __shfl_sync(0xffffffffu, upto[u], 31);
       int hole_to = hole_at + (mine & 0xFFFF), out_to = out_at + (mine >> 16);
 #pragma unroll
@@ -491,7 +484,7 @@ __global__ void __launch_bounds__(kSelThreads, kSelThreads == 1024 ? 1 : 4)
       hole_at += sum & 0xFFFF;
       out_at += sum >> 16;
     }
-  }
+  });
   if (size > 1) sync();  // no CTA leaves while another may read its sums
   pdl_launch_dependents();
 }
@@ -576,22 +569,6 @@ cudaError_t launch(void (*kernel)(A...), int grid, int threads, size_t smem, int
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-template <int THREADS>
-cudaError_t launch_select(const PagedEvictParams& p, int lists, int staged, int cluster, cudaStream_t stream) {
-  static bool configured[64] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-  if (!configured[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(paged_select_kernel<THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         kMaxStaged * (int)sizeof(uint32_t));
-    if (e != cudaSuccess) return e;
-    configured[dev] = true;
-  }
-  return launch(paged_select_kernel<THREADS>, lists * cluster, THREADS, staged * sizeof(uint32_t), cluster, stream, p,
-                staged, cluster);
-}
-
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 }  // namespace
@@ -618,14 +595,17 @@ void paged_evict_plan(int n_seqs, int n_kv, long long max_rows, int budget, Page
 
 cudaError_t launch_paged_evict(const PagedEvictParams& p, int sms, cudaStream_t stream) {
   const int lists = p.n_seqs * p.n_kv, cap = p.max_pages * p.page_size;
-  // a cluster for a list while there are SMs for it and each of its CTAs has rows for all its threads
+  // 256 threads hold the keys of 4096 rows; longer lists get 1024 for each 16384 rows, in
+  // clusters of up to 8 CTAs (131072 rows), and still longer ones those 8 and several reads
   int cluster = 1;
-  while (cluster < 8 && lists * cluster * 2 <= sms && cap >= cluster * 2 * kShortList) cluster *= 2;
-  const int threads = cap <= kShortList ? 256 : 1024;
-  const int step = cluster * threads * 4, share = (cap + step - 1) / step * threads * 4;
-  const int staged = share < kMaxStaged ? share : kMaxStaged;
-  cudaError_t e = threads == 256 ? launch_select<256>(p, lists, staged, cluster, stream)
-                                 : launch_select<1024>(p, lists, staged, cluster, stream);
+  while (cluster < 8 && cap > cluster * 1024 * 4 * kDeep) cluster *= 2;
+  cudaError_t e;
+  if (cap <= 256 * 4 * kDeep)
+    e = launch(paged_select_kernel<256, true>, lists, 256, 0, 1, stream, p, 1);
+  else if (cap <= cluster * 1024 * 4 * kDeep)
+    e = launch(paged_select_kernel<1024, true>, lists * cluster, 1024, 0, cluster, stream, p, cluster);
+  else
+    e = launch(paged_select_kernel<1024, false>, lists * cluster, 1024, 0, cluster, stream, p, cluster);
   if (e != cudaSuccess) return e;
   const long long want = (long long)lists * ((p.max_moves + kMovePiece - 1) / kMovePiece), most = 4LL * sms;  // all resident
   return launch(paged_move_kernel, (int)(want < 1 ? 1 : want < most ? want : most), kMoveWarps * 32, 0, 1,
