@@ -504,7 +504,8 @@ typedef struct nf4b_paged_kv {
  * are apart because an eviction leaves a sequence fewer rows than tokens.
  * A token whose row, sequence or page is out of range writes no cache row; one
  * whose position is outside [0, freqs_rows) writes none and has q = 0 (padding).
- * Two tokens of one call must not name the same row. qkv and q_out 16-byte aligned.
+ * Two tokens of one call must not name the same row. qkv, q_out, freqs and the norm
+ * weights are 16-byte aligned.
  */
 int nf4b_paged_write(const nf4b_paged_kv* cache, const void* qkv, const int32_t* seqs, const int32_t* rows,
                      const int32_t* positions, const void* freqs, int freqs_dtype, int freqs_rows,

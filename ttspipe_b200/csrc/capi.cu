@@ -1045,10 +1045,13 @@ int nf4b_paged_write(const nf4b_paged_kv* cache, const void* qkv, const int32_t*
     return fail(NF4B_ERR_SHAPE, "%d tokens, rotary table of %d rows", n_tokens, freqs_rows);
   if (seqs == nullptr && n_tokens > cache->n_seqs)
     return fail(NF4B_ERR_SHAPE, "%d tokens of %d sequences need seqs", n_tokens, cache->n_seqs);
-  if (!aligned(qkv, 16) || !aligned(q_out, 16)) return fail(NF4B_ERR_ALIGN, "qkv / q_out not 16-byte aligned");
-  if (!aligned(q_norm_w, 2) || !aligned(k_norm_w, 2) || !aligned(seqs, 4) || !aligned(rows, 4) ||
-      !aligned(positions, 4) || !freqs_aligned(freqs, freqs_dtype))
-    return fail(NF4B_ERR_ALIGN, "norm weights, sequences, rows, positions or freqs misaligned");
+  if ((long long)n_tokens * (n_head + 2 * cache->n_kv) >= (1LL << 31))
+    return fail(NF4B_ERR_SHAPE, "%d tokens of %d heads", n_tokens, n_head + 2 * cache->n_kv);
+  if (!aligned(qkv, 16) || !aligned(q_out, 16) || !aligned(freqs, 16) || !aligned(q_norm_w, 16) ||
+      !aligned(k_norm_w, 16))
+    return fail(NF4B_ERR_ALIGN, "qkv, q_out, freqs or norm weights not 16-byte aligned");
+  if (!aligned(seqs, 4) || !aligned(rows, 4) || !aligned(positions, 4))
+    return fail(NF4B_ERR_ALIGN, "sequences, rows or positions not 4-byte aligned");
   if ((st = check_device())) return st;
   PagedWriteParams p;
   p.qkv = static_cast<const uint16_t*>(qkv);

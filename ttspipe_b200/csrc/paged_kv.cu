@@ -13,68 +13,112 @@ namespace {
 constexpr int kD = 128;
 
 // ---- write ------------------------------------------------------------------
-// One warp for each head of each token, four dimensions to a lane (two rotary
-// pairs). The arithmetic is qk_rope_kv_kernel's, rounding point for rounding point
-// (the norm's sum of squares in fp64 is exact in any order), so a row in a page has
-// the bits it would have in a dense cache.
+// Half a warp for each head of a token, 16 bytes (four rotary pairs) to a lane; a warp
+// takes 2 kPairs heads of one token, so that the rotary row, the page and the norm's
+// reciprocal square root (fp64, one lane a head) are had once for all of them. The arithmetic is
+// qk_rope_kv_kernel's, rounding point for rounding point (the norm's sum of squares in
+// fp64 is exact in any order), so a row in a page has the bits it would have in a
+// dense cache.
 constexpr int kWriteWarps = 8;
 
-template <bool F16>
+template <int kPairs, bool F16>
 __global__ void __launch_bounds__(kWriteWarps * 32) paged_write_kernel(const __grid_constant__ PagedWriteParams p) {
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const int heads = p.n_head + 2 * p.n_kv;
-  const long long total = (long long)p.n_tokens * heads;
-  for (long long item = (long long)blockIdx.x * kWriteWarps + (threadIdx.x >> 5); item < total;
-       item += (long long)gridDim.x * kWriteWarps) {
-    const int tok = (int)(item / heads), head = (int)(item - (long long)tok * heads);
+  const int lane = threadIdx.x & 31, half = lane >> 4, piece = lane & 15;
+  const int heads = p.n_head + 2 * p.n_kv, groups = (heads + 2 * kPairs - 1) / (2 * kPairs);
+  const long long item = (long long)blockIdx.x * kWriteWarps + (threadIdx.x >> 5);
+  const int tok = (int)(item / groups), head0 = (int)(item - (long long)tok * groups) * 2 * kPairs + half;
+  if (tok >= p.n_tokens) return;
+  const uint4* in = reinterpret_cast<const uint4*>(p.qkv + (size_t)tok * heads * kD) + piece;
+  uint4 raw[kPairs];
+#pragma unroll
+  for (int u = 0; u < kPairs; ++u)
+    if (head0 + 2 * u < heads) raw[u] = ld_stream_u4(in + (head0 + 2 * u) * (kD / 8));
+  const int pos = p.positions[tok], row = p.rows[tok], seq = p.seqs == nullptr ? tok : p.seqs[tok];
+  const bool turned = pos >= 0 && pos < p.freqs_rows;  // else the token is padding
+  float cs[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) cs[i] = 0.f;
+  if (turned) {
+    const size_t at = (size_t)pos * kD + piece * 8;
+    if (p.ftype == NF4B_F32) {
+      const float4* f = reinterpret_cast<const float4*>(static_cast<const float*>(p.freqs) + at);
+      *reinterpret_cast<float4*>(cs) = f[0];
+      *reinterpret_cast<float4*>(cs + 4) = f[1];
+    } else {
+      const uint4 f = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.freqs) + at);
+      const uint32_t w[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        cs[2 * i] = p.ftype == NF4B_F16 ? act_lo<true>(w[i]) : act_lo<false>(w[i]);
+        cs[2 * i + 1] = p.ftype == NF4B_F16 ? act_hi<true>(w[i]) : act_hi<false>(w[i]);
+      }
+    }
+  }
+  long long slot = -1;  // the token's row in its page, of KV head 0
+  if (turned && row >= 0 && row / p.page_size < p.max_pages && seq >= 0 && seq < p.n_seqs) {
+    const int pg = p.table[(size_t)seq * p.max_pages + row / p.page_size];
+    if (pg >= 0 && pg < p.n_pages) slot = (long long)pg * p.n_kv * p.page_size + row % p.page_size;
+  }
+  float r = 0.f;
+  if (p.qw != nullptr) {
+    double ss[kPairs];
+#pragma unroll
+    for (int u = 0; u < kPairs; ++u) {
+      const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+      ss[u] = 0.0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const double x0 = act_lo<F16>(w[i]), x1 = act_hi<F16>(w[i]);
+        ss[u] = fma(x0, x0, ss[u]);
+        ss[u] = fma(x1, x1, ss[u]);
+      }
+    }
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1)
+#pragma unroll
+      for (int u = 0; u < kPairs; ++u) ss[u] += __shfl_xor_sync(0xffffffffu, ss[u], off);
+    double mine = ss[0];  // lane j of a half: the head of pair j
+#pragma unroll
+    for (int u = 1; u < kPairs; ++u)
+      if (piece == u) mine = ss[u];
+    if (piece < kPairs) r = rsqrt_exact(mine, kD, p.eps);
+  }
+#pragma unroll
+  for (int u = 0; u < kPairs; ++u) {
+    const int head = head0 + 2 * u;
+    const float ru = __shfl_sync(0xffffffffu, r, (lane & 16) | u);
+    if (head >= heads) continue;
     const bool is_q = head < p.n_head, is_v = head >= p.n_head + p.n_kv;
-    const int pos = p.positions[tok];
-    const bool turned = pos >= 0 && pos < p.freqs_rows;  // else the token is padding
-    const uint2 in = *reinterpret_cast<const uint2*>(p.qkv + item * kD + lane * 4);
-    uint2 out = in;
+    uint4 out = raw[u];
     if (!is_v) {
-      float x[4] = {act_lo<F16>(in.x), act_hi<F16>(in.x), act_lo<F16>(in.y), act_hi<F16>(in.y)};
-      const uint16_t* w = is_q ? p.qw : p.kw;
-      if (w != nullptr) {
-        double ss = 0.0;
+      const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+      uint32_t o[4];
+      uint4 nw = make_uint4(0, 0, 0, 0);
+      if (p.qw != nullptr) nw = reinterpret_cast<const uint4*>(is_q ? p.qw : p.kw)[piece];
+      const uint32_t g[4] = {nw.x, nw.y, nw.z, nw.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ss += (double)x[i] * (double)x[i];
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, off);
-        const float r = rsqrt_exact(ss, kD, p.eps);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          x[i] = round_act<F16>(__fmul_rn(__fmul_rn(x[i], r), act2f<F16>(w[lane * 4 + i])));
-      }
-      if (turned) {
-        float y[4];
-#pragma unroll
-        for (int i = 0; i < 4; i += 2) {
-          const long long fi = (long long)pos * kD + lane * 4 + i;
-          const float c = load_freq(p.freqs, fi, p.ftype), sn = load_freq(p.freqs, fi + 1, p.ftype);
-          y[i] = __fsub_rn(__fmul_rn(x[i], c), __fmul_rn(x[i + 1], sn));
-          y[i + 1] = __fadd_rn(__fmul_rn(x[i + 1], c), __fmul_rn(x[i], sn));
+      for (int i = 0; i < 4; ++i) {
+        float x0 = act_lo<F16>(w[i]), x1 = act_hi<F16>(w[i]);
+        if (p.qw != nullptr) {
+          x0 = round_act<F16>(__fmul_rn(__fmul_rn(x0, ru), act_lo<F16>(g[i])));
+          x1 = round_act<F16>(__fmul_rn(__fmul_rn(x1, ru), act_hi<F16>(g[i])));
         }
-        out = make_uint2(pack_act2<F16>(y[0], y[1]), pack_act2<F16>(y[2], y[3]));
-      } else {
-        out = make_uint2(0, 0);
+        const float c = cs[2 * i], sn = cs[2 * i + 1];
+        o[i] = pack_act2<F16>(__fsub_rn(__fmul_rn(x0, c), __fmul_rn(x1, sn)),
+                              __fadd_rn(__fmul_rn(x1, c), __fmul_rn(x0, sn)));
       }
+      out = turned ? make_uint4(o[0], o[1], o[2], o[3]) : make_uint4(0, 0, 0, 0);
     }
     if (is_q) {
-      *reinterpret_cast<uint2*>(p.q_out + ((size_t)tok * p.n_head + head) * kD + lane * 4) = out;
-      continue;
-    }
-    const int seq = p.seqs == nullptr ? tok : p.seqs[tok], row = p.rows[tok];
-    if (!turned || row < 0 || row / p.page_size >= p.max_pages || seq < 0 || seq >= p.n_seqs) continue;
-    const int pg = p.table[(size_t)seq * p.max_pages + row / p.page_size];
-    if (pg < 0 || pg >= p.n_pages) continue;
-    const int kh = head - p.n_head - (is_v ? p.n_kv : 0);
-    const size_t at = ((size_t)pg * p.n_kv + kh) * p.page_size + row % p.page_size;
-    *reinterpret_cast<uint2*>((is_v ? p.v : p.k) + at * kD + lane * 4) = out;
-    if (!is_v && lane == 0) {
-      if (p.weight != nullptr) p.weight[at] = 0.f;
-      if (p.position != nullptr) p.position[at] = pos;
+      reinterpret_cast<uint4*>(p.q_out + ((size_t)tok * p.n_head + head) * kD)[piece] = out;
+    } else if (slot >= 0) {
+      const size_t at = slot + (size_t)(head - p.n_head - (is_v ? p.n_kv : 0)) * p.page_size;
+      reinterpret_cast<uint4*>((is_v ? p.v : p.k) + at * kD)[piece] = out;
+      if (!is_v && piece == 0) {
+        if (p.weight != nullptr) p.weight[at] = 0.f;
+        if (p.position != nullptr) p.position[at] = pos;
+      }
     }
   }
   pdl_launch_dependents();
@@ -574,10 +618,14 @@ size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 }  // namespace
 
 cudaError_t launch_paged_write(const PagedWriteParams& p, int sms, bool f16, cudaStream_t stream) {
-  const long long items = (long long)p.n_tokens * (p.n_head + 2 * p.n_kv);
-  const long long want = (items + kWriteWarps - 1) / kWriteWarps, most = 16LL * sms;
-  return launch(f16 ? paged_write_kernel<true> : paged_write_kernel<false>, (int)(want < most ? want : most),
-                kWriteWarps * 32, 0, 1, stream, p);
+  // eight heads to a warp once that gives every SM a CTA; two until then
+  const int heads = p.n_head + 2 * p.n_kv;
+  const long long eights = (long long)p.n_tokens * ((heads + 7) / 8), pairs = (long long)p.n_tokens * ((heads + 1) / 2);
+  const bool many = eights >= (long long)kWriteWarps * sms;
+  const int grid = (int)(((many ? eights : pairs) + kWriteWarps - 1) / kWriteWarps);
+  auto kernel = many ? (f16 ? paged_write_kernel<4, true> : paged_write_kernel<4, false>)
+                     : (f16 ? paged_write_kernel<1, true> : paged_write_kernel<1, false>);
+  return launch(kernel, grid, kWriteWarps * 32, 0, 1, stream, p);
 }
 
 void paged_evict_plan(int n_seqs, int n_kv, long long max_rows, int budget, PagedEvictPlan* plan) {
