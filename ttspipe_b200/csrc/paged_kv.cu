@@ -21,25 +21,62 @@ constexpr int kD = 128;
 // dense cache.
 constexpr int kWriteWarps = 8;
 
+// Two fp32 numbers in one register pair: sm_100 multiplies and adds both at once, each
+// rounded to nearest as by itself.
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float x, float y) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpack(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+
+// rsqrt_exact of common.cuh for a width of 128 with CUDA's fp64 rsqrt in place of a
+// square root and a division: the rounded results agree for every fp32 t from 0 to
+// infinity (all of them compared).
+__device__ __forceinline__ float rsqrt_128(double ss, float eps) {
+  const float t = __fadd_rn((float)(ss * (1.0 / 128)), eps);
+  return (float)rsqrt((double)t);
+}
+
 template <int kPairs, bool F16>
 __global__ void __launch_bounds__(kWriteWarps * 32) paged_write_kernel(const __grid_constant__ PagedWriteParams p) {
   pdl_wait();
   const int lane = threadIdx.x & 31, half = lane >> 4, piece = lane & 15;
   const int heads = p.n_head + 2 * p.n_kv, groups = (heads + 2 * kPairs - 1) / (2 * kPairs);
-  const long long item = (long long)blockIdx.x * kWriteWarps + (threadIdx.x >> 5);
-  const int tok = (int)(item / groups), head0 = (int)(item - (long long)tok * groups) * 2 * kPairs + half;
+  const unsigned item = blockIdx.x * kWriteWarps + (threadIdx.x >> 5);
+  const int tok = (int)(item / groups), first = (int)(item - (unsigned)tok * groups) * 2 * kPairs, head0 = first + half;
   if (tok >= p.n_tokens) return;
   const uint4* in = reinterpret_cast<const uint4*>(p.qkv + (size_t)tok * heads * kD) + piece;
   uint4 raw[kPairs];
 #pragma unroll
-  for (int u = 0; u < kPairs; ++u)
+  for (int u = 0; u < kPairs; ++u) {
+    raw[u] = make_uint4(0, 0, 0, 0);
     if (head0 + 2 * u < heads) raw[u] = ld_stream_u4(in + (head0 + 2 * u) * (kD / 8));
+  }
   const int pos = p.positions[tok], row = p.rows[tok], seq = p.seqs == nullptr ? tok : p.seqs[tok];
   const bool turned = pos >= 0 && pos < p.freqs_rows;  // else the token is padding
-  float cs[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) cs[i] = 0.f;
-  if (turned) {
+  const bool values = first >= p.n_head + p.n_kv;      // no head of this warp is turned
+  F2 c[2], sn[2], ns[2];  // cos, sin and -sin of pairs 2 i and 2 i + 1
+  float r = 0.f;
+  if (turned && !values) {
+    float cs[8];
     const size_t at = (size_t)pos * kD + piece * 8;
     if (p.ftype == NF4B_F32) {
       const float4* f = reinterpret_cast<const float4*>(static_cast<const float*>(p.freqs) + at);
@@ -54,36 +91,56 @@ __global__ void __launch_bounds__(kWriteWarps * 32) paged_write_kernel(const __g
         cs[2 * i + 1] = p.ftype == NF4B_F16 ? act_hi<true>(w[i]) : act_hi<false>(w[i]);
       }
     }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      c[i] = f2(cs[4 * i], cs[4 * i + 2]);
+      sn[i] = f2(cs[4 * i + 1], cs[4 * i + 3]);
+      ns[i] = f2(-cs[4 * i + 1], -cs[4 * i + 3]);
+    }
+    if (p.qw != nullptr) {
+      double ss[kPairs];
+#pragma unroll
+      for (int u = 0; u < kPairs; ++u) {
+        const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+        ss[u] = 0.0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const double x0 = act_lo<F16>(w[i]), x1 = act_hi<F16>(w[i]);
+          ss[u] = fma(x0, x0, ss[u]);
+          ss[u] = fma(x1, x1, ss[u]);
+        }
+      }
+      // over the half warp; where there are four sums, lanes hand over those that others
+      // finish: lane j ends with the sum of pair j % 4
+      double mine = ss[0];
+      if (kPairs == 4) {
+        double two[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {  // lanes with bit 1 take pairs 2 and 3
+          const bool up = lane & 2;
+          const double keep = up ? ss[2 % kPairs + (i & (kPairs - 1))] : ss[i & (kPairs - 1)];
+          const double give = up ? ss[i & (kPairs - 1)] : ss[2 % kPairs + (i & (kPairs - 1))];
+          two[i] = keep + __shfl_xor_sync(0xffffffffu, give, 2);
+        }
+        const double keep = lane & 1 ? two[1] : two[0], give = lane & 1 ? two[0] : two[1];
+        mine = keep + __shfl_xor_sync(0xffffffffu, give, 1);
+        mine += __shfl_xor_sync(0xffffffffu, mine, 4);
+        mine += __shfl_xor_sync(0xffffffffu, mine, 8);
+      } else {
+#pragma unroll
+        for (int off = 8; off > 0; off >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, off);
+      }
+      r = rsqrt_128(mine, p.eps);
+    }
   }
   long long slot = -1;  // the token's row in its page, of KV head 0
-  if (turned && row >= 0 && row / p.page_size < p.max_pages && seq >= 0 && seq < p.n_seqs) {
+  if (first + 2 * kPairs > p.n_head && turned && row >= 0 && row / p.page_size < p.max_pages && seq >= 0 &&
+      seq < p.n_seqs) {
     const int pg = p.table[(size_t)seq * p.max_pages + row / p.page_size];
     if (pg >= 0 && pg < p.n_pages) slot = (long long)pg * p.n_kv * p.page_size + row % p.page_size;
   }
-  float r = 0.f;
-  if (p.qw != nullptr) {
-    double ss[kPairs];
-#pragma unroll
-    for (int u = 0; u < kPairs; ++u) {
-      const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-      ss[u] = 0.0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const double x0 = act_lo<F16>(w[i]), x1 = act_hi<F16>(w[i]);
-        ss[u] = fma(x0, x0, ss[u]);
-        ss[u] = fma(x1, x1, ss[u]);
-      }
-    }
-#pragma unroll
-    for (int off = 8; off > 0; off >>= 1)
-#pragma unroll
-      for (int u = 0; u < kPairs; ++u) ss[u] += __shfl_xor_sync(0xffffffffu, ss[u], off);
-    double mine = ss[0];  // lane j of a half: the head of pair j
-#pragma unroll
-    for (int u = 1; u < kPairs; ++u)
-      if (piece == u) mine = ss[u];
-    if (piece < kPairs) r = rsqrt_exact(mine, kD, p.eps);
-  }
+  uint4 nw = make_uint4(0, 0, 0, 0);
+  int of = -1;  // whose norm weight nw is: 1 the queries', 0 the keys'
 #pragma unroll
   for (int u = 0; u < kPairs; ++u) {
     const int head = head0 + 2 * u;
@@ -91,27 +148,36 @@ __global__ void __launch_bounds__(kWriteWarps * 32) paged_write_kernel(const __g
     if (head >= heads) continue;
     const bool is_q = head < p.n_head, is_v = head >= p.n_head + p.n_kv;
     uint4 out = raw[u];
-    if (!is_v) {
+    if (!is_v && turned) {
       const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
       uint32_t o[4];
-      uint4 nw = make_uint4(0, 0, 0, 0);
-      if (p.qw != nullptr) nw = reinterpret_cast<const uint4*>(is_q ? p.qw : p.kw)[piece];
+      if (p.qw != nullptr && of != (int)is_q) {
+        of = is_q;
+        nw = reinterpret_cast<const uint4*>(is_q ? p.qw : p.kw)[piece];
+      }
       const uint32_t g[4] = {nw.x, nw.y, nw.z, nw.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float x0 = act_lo<F16>(w[i]), x1 = act_hi<F16>(w[i]);
+      for (int i = 0; i < 2; ++i) {
+        F2 x0 = f2(act_lo<F16>(w[2 * i]), act_lo<F16>(w[2 * i + 1]));
+        F2 x1 = f2(act_hi<F16>(w[2 * i]), act_hi<F16>(w[2 * i + 1]));
         if (p.qw != nullptr) {
-          x0 = round_act<F16>(__fmul_rn(__fmul_rn(x0, ru), act_lo<F16>(g[i])));
-          x1 = round_act<F16>(__fmul_rn(__fmul_rn(x1, ru), act_hi<F16>(g[i])));
+          const F2 rr = f2(ru, ru);
+          const float2 y0 = unpack(mul2(mul2(x0, rr), f2(act_lo<F16>(g[2 * i]), act_lo<F16>(g[2 * i + 1]))));
+          const float2 y1 = unpack(mul2(mul2(x1, rr), f2(act_hi<F16>(g[2 * i]), act_hi<F16>(g[2 * i + 1]))));
+          const uint32_t a = pack_act2<F16>(y0.x, y1.x), b = pack_act2<F16>(y0.y, y1.y);  // the norm's rounding
+          x0 = f2(act_lo<F16>(a), act_lo<F16>(b));
+          x1 = f2(act_hi<F16>(a), act_hi<F16>(b));
         }
-        const float c = cs[2 * i], sn = cs[2 * i + 1];
-        o[i] = pack_act2<F16>(__fsub_rn(__fmul_rn(x0, c), __fmul_rn(x1, sn)),
-                              __fadd_rn(__fmul_rn(x1, c), __fmul_rn(x0, sn)));
+        const float2 z0 = unpack(add2(mul2(x0, c[i]), mul2(x1, ns[i])));
+        const float2 z1 = unpack(add2(mul2(x1, c[i]), mul2(x0, sn[i])));
+        o[2 * i] = pack_act2<F16>(z0.x, z1.x);
+        o[2 * i + 1] = pack_act2<F16>(z0.y, z1.y);
       }
-      out = turned ? make_uint4(o[0], o[1], o[2], o[3]) : make_uint4(0, 0, 0, 0);
+      out = make_uint4(o[0], o[1], o[2], o[3]);
     }
     if (is_q) {
-      reinterpret_cast<uint4*>(p.q_out + ((size_t)tok * p.n_head + head) * kD)[piece] = out;
+      reinterpret_cast<uint4*>(p.q_out + ((size_t)tok * p.n_head + head) * kD)[piece] =
+          turned ? out : make_uint4(0, 0, 0, 0);
     } else if (slot >= 0) {
       const size_t at = slot + (size_t)(head - p.n_head - (is_v ? p.n_kv : 0)) * p.page_size;
       reinterpret_cast<uint4*>((is_v ? p.v : p.k) + at * kD)[piece] = out;
