@@ -14,12 +14,13 @@ constexpr int kD = 128;
 
 // ---- write ------------------------------------------------------------------
 // Half a warp for each head of a token, 16 bytes (four rotary pairs) to a lane; a warp
-// takes 2 kPairs heads of one token, so that the rotary row, the page and the norm's
-// reciprocal square root (fp64, one lane a head) are had once for all of them. The arithmetic is
+// takes kGroups times 2 kPairs heads of one token, so that the rotary row and the page are
+// had once for all of them and the norm's reciprocal square root (fp64, one lane a head) once
+// for each 2 kPairs. The arithmetic is
 // qk_rope_kv_kernel's, rounding point for rounding point (the norm's sum of squares in
 // fp64 is exact in any order), so a row in a page has the bits it would have in a
 // dense cache.
-constexpr int kWriteWarps = 8;
+constexpr int kWriteWarps = 4;
 
 // Two fp32 numbers in one register pair: sm_100 multiplies and adds both at once, each
 // rounded to nearest as by itself.
@@ -55,27 +56,32 @@ __device__ __forceinline__ float rsqrt_128(double ss, float eps) {
   return (float)rsqrt((double)t);
 }
 
-template <int kPairs, bool F16>
+template <int kPairs, int kGroups, bool F16>
 __global__ void __launch_bounds__(kWriteWarps * 32) paged_write_kernel(const __grid_constant__ PagedWriteParams p) {
   pdl_wait();
   const int lane = threadIdx.x & 31, half = lane >> 4, piece = lane & 15;
-  const int heads = p.n_head + 2 * p.n_kv, groups = (heads + 2 * kPairs - 1) / (2 * kPairs);
+  const int heads = p.n_head + 2 * p.n_kv;
+  constexpr int kSpan = 2 * kPairs * kGroups;
+  const int spans = (heads + kSpan - 1) / kSpan;
   const unsigned item = blockIdx.x * kWriteWarps + (threadIdx.x >> 5);
-  const int tok = (int)(item / groups), first = (int)(item - (unsigned)tok * groups) * 2 * kPairs, head0 = first + half;
+  const int tok = (int)(item / spans);
   if (tok >= p.n_tokens) return;
+  int first = (int)(item - (unsigned)tok * spans) * kSpan;
+  const int end = min(heads, first + kSpan);
   const uint4* in = reinterpret_cast<const uint4*>(p.qkv + (size_t)tok * heads * kD) + piece;
-  uint4 raw[kPairs];
+  uint4 raw[kPairs], next[kPairs];
+  auto load = [&](uint4 (&to)[kPairs], int head) {
 #pragma unroll
-  for (int u = 0; u < kPairs; ++u) {
-    raw[u] = make_uint4(0, 0, 0, 0);
-    if (head0 + 2 * u < heads) raw[u] = ld_stream_u4(in + (head0 + 2 * u) * (kD / 8));
-  }
+    for (int u = 0; u < kPairs; ++u) {
+      to[u] = make_uint4(0, 0, 0, 0);
+      if (head + 2 * u < end) to[u] = ld_stream_u4(in + (head + 2 * u) * (kD / 8));
+    }
+  };
+  load(raw, first + half);
   const int pos = p.positions[tok], row = p.rows[tok], seq = p.seqs == nullptr ? tok : p.seqs[tok];
   const bool turned = pos >= 0 && pos < p.freqs_rows;  // else the token is padding
-  const bool values = first >= p.n_head + p.n_kv;      // no head of this warp is turned
   F2 c[2], sn[2], ns[2];  // cos, sin and -sin of pairs 2 i and 2 i + 1
-  float r = 0.f;
-  if (turned && !values) {
+  if (turned && first < p.n_head + p.n_kv) {
     float cs[8];
     const size_t at = (size_t)pos * kD + piece * 8;
     if (p.ftype == NF4B_F32) {
@@ -97,7 +103,21 @@ __global__ void __launch_bounds__(kWriteWarps * 32) paged_write_kernel(const __g
       sn[i] = f2(cs[4 * i + 1], cs[4 * i + 3]);
       ns[i] = f2(-cs[4 * i + 1], -cs[4 * i + 3]);
     }
-    if (p.qw != nullptr) {
+  }
+  long long slot = -1;  // the token's row in its page, of KV head 0
+  if (end > p.n_head && turned && row >= 0 && row / p.page_size < p.max_pages && seq >= 0 &&
+      seq < p.n_seqs) {
+    const int pg = p.table[(size_t)seq * p.max_pages + row / p.page_size];
+    if (pg >= 0 && pg < p.n_pages) slot = (long long)pg * p.n_kv * p.page_size + row % p.page_size;
+  }
+  uint4 nw = make_uint4(0, 0, 0, 0);
+  int of = -1;  // whose norm weight nw is: 1 the queries', 0 the keys'
+#pragma unroll 1
+  for (;; first += 2 * kPairs) {
+    const bool more = first + 2 * kPairs < end;
+    if (more) load(next, first + 2 * kPairs + half);
+    float r = 0.f;
+    if (turned && p.qw != nullptr && first < p.n_head + p.n_kv) {
       double ss[kPairs];
 #pragma unroll
       for (int u = 0; u < kPairs; ++u) {
@@ -132,60 +152,55 @@ __global__ void __launch_bounds__(kWriteWarps * 32) paged_write_kernel(const __g
       }
       r = rsqrt_128(mine, p.eps);
     }
-  }
-  long long slot = -1;  // the token's row in its page, of KV head 0
-  if (first + 2 * kPairs > p.n_head && turned && row >= 0 && row / p.page_size < p.max_pages && seq >= 0 &&
-      seq < p.n_seqs) {
-    const int pg = p.table[(size_t)seq * p.max_pages + row / p.page_size];
-    if (pg >= 0 && pg < p.n_pages) slot = (long long)pg * p.n_kv * p.page_size + row % p.page_size;
-  }
-  uint4 nw = make_uint4(0, 0, 0, 0);
-  int of = -1;  // whose norm weight nw is: 1 the queries', 0 the keys'
 #pragma unroll
-  for (int u = 0; u < kPairs; ++u) {
-    const int head = head0 + 2 * u;
-    const float ru = __shfl_sync(0xffffffffu, r, (lane & 16) | u);
-    if (head >= heads) continue;
-    const bool is_q = head < p.n_head, is_v = head >= p.n_head + p.n_kv;
-    uint4 out = raw[u];
-    if (!is_v && turned) {
-      const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-      uint32_t o[4];
-      if (p.qw != nullptr && of != (int)is_q) {
-        of = is_q;
-        nw = reinterpret_cast<const uint4*>(is_q ? p.qw : p.kw)[piece];
-      }
-      const uint32_t g[4] = {nw.x, nw.y, nw.z, nw.w};
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        F2 x0 = f2(act_lo<F16>(w[2 * i]), act_lo<F16>(w[2 * i + 1]));
-        F2 x1 = f2(act_hi<F16>(w[2 * i]), act_hi<F16>(w[2 * i + 1]));
-        if (p.qw != nullptr) {
-          const F2 rr = f2(ru, ru);
-          const float2 y0 = unpack(mul2(mul2(x0, rr), f2(act_lo<F16>(g[2 * i]), act_lo<F16>(g[2 * i + 1]))));
-          const float2 y1 = unpack(mul2(mul2(x1, rr), f2(act_hi<F16>(g[2 * i]), act_hi<F16>(g[2 * i + 1]))));
-          const uint32_t a = pack_act2<F16>(y0.x, y1.x), b = pack_act2<F16>(y0.y, y1.y);  // the norm's rounding
-          x0 = f2(act_lo<F16>(a), act_lo<F16>(b));
-          x1 = f2(act_hi<F16>(a), act_hi<F16>(b));
+    for (int u = 0; u < kPairs; ++u) {
+      const int head = first + half + 2 * u;
+      const float ru = __shfl_sync(0xffffffffu, r, (lane & 16) | u);
+      if (head >= end) continue;
+      const bool is_q = head < p.n_head, is_v = head >= p.n_head + p.n_kv;
+      uint4 out = raw[u];
+      if (!is_v && turned) {
+        const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+        uint32_t o[4];
+        if (p.qw != nullptr && of != (int)is_q) {
+          of = is_q;
+          nw = reinterpret_cast<const uint4*>(is_q ? p.qw : p.kw)[piece];
         }
-        const float2 z0 = unpack(add2(mul2(x0, c[i]), mul2(x1, ns[i])));
-        const float2 z1 = unpack(add2(mul2(x1, c[i]), mul2(x0, sn[i])));
-        o[2 * i] = pack_act2<F16>(z0.x, z1.x);
-        o[2 * i + 1] = pack_act2<F16>(z0.y, z1.y);
+        const uint32_t g[4] = {nw.x, nw.y, nw.z, nw.w};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          F2 x0 = f2(act_lo<F16>(w[2 * i]), act_lo<F16>(w[2 * i + 1]));
+          F2 x1 = f2(act_hi<F16>(w[2 * i]), act_hi<F16>(w[2 * i + 1]));
+          if (p.qw != nullptr) {
+            const F2 rr = f2(ru, ru);
+            const float2 y0 = unpack(mul2(mul2(x0, rr), f2(act_lo<F16>(g[2 * i]), act_lo<F16>(g[2 * i + 1]))));
+            const float2 y1 = unpack(mul2(mul2(x1, rr), f2(act_hi<F16>(g[2 * i]), act_hi<F16>(g[2 * i + 1]))));
+            const uint32_t a = pack_act2<F16>(y0.x, y1.x), b = pack_act2<F16>(y0.y, y1.y);  // the norm's rounding
+            x0 = f2(act_lo<F16>(a), act_lo<F16>(b));
+            x1 = f2(act_hi<F16>(a), act_hi<F16>(b));
+          }
+          const float2 z0 = unpack(add2(mul2(x0, c[i]), mul2(x1, ns[i])));
+          const float2 z1 = unpack(add2(mul2(x1, c[i]), mul2(x0, sn[i])));
+          o[2 * i] = pack_act2<F16>(z0.x, z1.x);
+          o[2 * i + 1] = pack_act2<F16>(z0.y, z1.y);
+        }
+        out = make_uint4(o[0], o[1], o[2], o[3]);
       }
-      out = make_uint4(o[0], o[1], o[2], o[3]);
-    }
-    if (is_q) {
-      reinterpret_cast<uint4*>(p.q_out + ((size_t)tok * p.n_head + head) * kD)[piece] =
-          turned ? out : make_uint4(0, 0, 0, 0);
-    } else if (slot >= 0) {
-      const size_t at = slot + (size_t)(head - p.n_head - (is_v ? p.n_kv : 0)) * p.page_size;
-      reinterpret_cast<uint4*>((is_v ? p.v : p.k) + at * kD)[piece] = out;
-      if (!is_v && piece == 0) {
-        if (p.weight != nullptr) p.weight[at] = 0.f;
-        if (p.position != nullptr) p.position[at] = pos;
+      if (is_q) {
+        reinterpret_cast<uint4*>(p.q_out + ((size_t)tok * p.n_head + head) * kD)[piece] =
+            turned ? out : make_uint4(0, 0, 0, 0);
+      } else if (slot >= 0) {
+        const size_t at = slot + (size_t)(head - p.n_head - (is_v ? p.n_kv : 0)) * p.page_size;
+        reinterpret_cast<uint4*>((is_v ? p.v : p.k) + at * kD)[piece] = out;
+        if (!is_v && piece == 0) {
+          if (p.weight != nullptr) p.weight[at] = 0.f;
+          if (p.position != nullptr) p.position[at] = pos;
+        }
       }
     }
+    if (!more) break;
+#pragma unroll
+    for (int u = 0; u < kPairs; ++u) raw[u] = next[u];
   }
   pdl_launch_dependents();
 }
@@ -684,13 +699,15 @@ size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 }  // namespace
 
 cudaError_t launch_paged_write(const PagedWriteParams& p, int sms, bool f16, cudaStream_t stream) {
-  // eight heads to a warp once that gives every SM a CTA; two until then
+  // 24 heads to a warp, eight at a time, once that gives the SMs some warps each (8188 tokens
+  // of 48 heads with norm: 41 us, 45 with eight heads to a warp); until then two
+  // (64 tokens: 2.6 us, 4.5 with eight)
   const int heads = p.n_head + 2 * p.n_kv;
-  const long long eights = (long long)p.n_tokens * ((heads + 7) / 8), pairs = (long long)p.n_tokens * ((heads + 1) / 2);
-  const bool many = eights >= (long long)kWriteWarps * sms;
-  const int grid = (int)(((many ? eights : pairs) + kWriteWarps - 1) / kWriteWarps);
-  auto kernel = many ? (f16 ? paged_write_kernel<4, true> : paged_write_kernel<4, false>)
-                     : (f16 ? paged_write_kernel<1, true> : paged_write_kernel<1, false>);
+  const bool many = (long long)p.n_tokens * heads >= 64LL * sms;
+  const long long warps = (long long)p.n_tokens * (many ? (heads + 23) / 24 : (heads + 1) / 2);
+  const int grid = (int)((warps + kWriteWarps - 1) / kWriteWarps);
+  auto kernel = many ? (f16 ? paged_write_kernel<4, 3, true> : paged_write_kernel<4, 3, false>)
+                     : (f16 ? paged_write_kernel<1, 1, true> : paged_write_kernel<1, 1, false>);
   return launch(kernel, grid, kWriteWarps * 32, 0, 1, stream, p);
 }
 
