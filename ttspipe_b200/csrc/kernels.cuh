@@ -389,7 +389,8 @@ cudaError_t launch_qkv_attention(const QkvIn& in, const int64_t* pos, uint16_t* 
 // ---- paged KV cache (paged_attention.cu, paged_kv.cu) ------------------------
 
 constexpr int PAGED_TILE = 16;        // rows of one unit of attention work; page sizes are multiples of it
-constexpr int PAGED_MIN_TILES = 8;    // tiles of one CTA's part, where there are that many
+constexpr int PAGED_MIN_TILES = 8;    // units of one CTA's part, where there are that many
+constexpr int PAGED_SEQ_TILES = 4;    // units that a (sequence, head) costs besides its tiles
 constexpr int PAGED_MAX_SEQS = 4096;  // sequences of one call (their tile counts lie in shared memory)
 constexpr int PAGED_MAX_GROUPS = 16;
 constexpr int PAGED_MAX_LISTS = 65535;  // (sequence, KV head) pairs of one call

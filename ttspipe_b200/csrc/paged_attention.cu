@@ -33,6 +33,7 @@ constexpr int kD = 128;
 constexpr int kTile = PAGED_TILE;
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
+constexpr int kJoin = 32;  // parts whose outputs the joining warp requests at once
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -47,46 +48,79 @@ __device__ __forceinline__ int seq_rows(const PagedAttnParams& p, int b) {
   return n < 0 ? 0 : n > cap ? cap : n;
 }
 
-// pre[b] = tiles of all (sequence < b, head); pre[n_seqs] the total. Ends with a barrier.
-__device__ __forceinline__ void tile_prefix(const PagedAttnParams& p, int* pre) {
-  if (threadIdx.x < 32) {
-    const int lane = threadIdx.x;
-    int base = 0;
-    for (int b0 = 0; b0 < p.n_seqs; b0 += 32) {
-      const int b = b0 + lane;
-      int t = b < p.n_seqs ? (seq_rows(p, b) + kTile - 1) / kTile * p.n_kv : 0;
+// The work of one (sequence, head) on the line: its tiles and what one costs besides
+// (first loads, the joins of its warps and parts), in tiles; 0 where there are none.
+__device__ __forceinline__ int seq_work(const PagedAttnParams& p, int b) {
+  const int tiles = (seq_rows(p, b) + kTile - 1) / kTile;
+  return tiles == 0 ? 0 : tiles + PAGED_SEQ_TILES;
+}
+
+// Where each sequence's work begins on the line, at the start of the kernels' dynamic
+// shared memory: pre[b] = work of all (sequence < b, head), pre[n_seqs] the total, and
+// each[b] = work of one head of sequence b.
+struct Line {
+  int* pre;
+  int* each;
+  __device__ __forceinline__ Line(uint8_t* smem, int n_seqs)
+      : pre(reinterpret_cast<int*>(smem)), each(pre + n_seqs + 1) {}
+  // Ends with a barrier.
+  __device__ __forceinline__ void fill(const PagedAttnParams& p) {
+    if (threadIdx.x < 32) {
+      const int lane = threadIdx.x;
+      int base = 0;
+      for (int b0 = 0; b0 < p.n_seqs; b0 += 32) {
+        const int b = b0 + lane;
+        const int one = b < p.n_seqs ? seq_work(p, b) : 0;
+        int t = one * p.n_kv;
 #pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, t, off);
-        if (lane >= off) t += o;
+        for (int off = 1; off < 32; off <<= 1) {
+          const int o = __shfl_up_sync(0xffffffffu, t, off);
+          if (lane >= off) t += o;
+        }
+        if (b < p.n_seqs) {
+          pre[b + 1] = base + t;
+          each[b] = one;
+        }
+        base += __shfl_sync(0xffffffffu, t, 31);
       }
-      if (b < p.n_seqs) pre[b + 1] = base + t;
-      base += __shfl_sync(0xffffffffu, t, 31);
+      if (lane == 0) pre[0] = 0;
     }
-    if (lane == 0) pre[0] = 0;
+    __syncthreads();
   }
-  __syncthreads();
-}
+  // The sequence of unit u < pre[n]: the last b with pre[b] <= u. By a whole warp, 32
+  // places compared at a time.
+  __device__ __forceinline__ int seq_of(int n, int u) const {
+    const int lane = threadIdx.x & 31;
+    int base = 0;
+    for (int left = n; left > 1;) {
+      const int step = (left + 31) >> 5, at = lane * step;
+      base += (__popc(__ballot_sync(0xffffffffu, at < left && pre[base + at] <= u)) - 1) * step;
+      left = min(step, n - base);
+    }
+    return base;
+  }
+};
 
-// The number of parts: as many CTAs as there are, but PAGED_MIN_TILES tiles for each unless that puts
+constexpr size_t line_bytes(int n_seqs) { return (size_t)(2 * n_seqs + 1) * sizeof(int); }
+
+// The number of parts: as many CTAs as there are, but PAGED_MIN_TILES units of work for each unless that puts
 // several (sequence, head)s into one part while CTAs are left.
-__device__ __forceinline__ int parts(const PagedAttnParams& p, int tiles, int ctas) {
-  const int by_tiles = (tiles + PAGED_MIN_TILES - 1) / PAGED_MIN_TILES;
-  return min(ctas, max(by_tiles, min(p.n_seqs * p.n_kv, tiles)));
+__device__ __forceinline__ int parts(const PagedAttnParams& p, int work, int ctas) {
+  const int by_work = (work + PAGED_MIN_TILES - 1) / PAGED_MIN_TILES;
+  return min(ctas, max(by_work, min(p.n_seqs * p.n_kv, work)));
 }
 
-// The sequence of tile u: the last b with pre[b] <= u.
-__device__ __forceinline__ int seq_of(const int* pre, int n_seqs, int u) {
-  int lo = 0, hi = n_seqs - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (pre[mid] <= u)
-      lo = mid;
-    else
-      hi = mid - 1;
+// Part c of `work` units in n parts: its first unit, the earlier parts one longer where they do not
+// come out even; and the part of a unit.
+struct Parts {
+  int each, longer;
+  __device__ __forceinline__ Parts(int work, int n) : each(work / n), longer(work - work / n * n) {}
+  __device__ __forceinline__ int first(int c) const { return c * each + min(c, longer); }
+  __device__ __forceinline__ int of(int u) const {
+    const int edge = longer * (each + 1);
+    return u < edge ? u / (each + 1) : longer + (u - edge) / each;
   }
-  return lo;
-}
+};
 
 // One (sequence, head) part's running state in a warp. NT: tiles of eight query
 // heads (groups <= 8: one, else two). o is O^T from the MMA: o[nt][j][.] holds
@@ -114,7 +148,8 @@ template <int NT>
 struct AttnShared {
   float o[kWarps][NT * 8][kD];
   float m[kWarps][NT * 8], l[kWarps][NT * 8];
-  int last;
+  int4 joins[2];  // (sequence, head)s that this CTA joins: first and last part, sequence, head
+  int n_joins;
 };
 
 // The finished row of one query head, four dimensions to a lane.
@@ -127,34 +162,100 @@ __device__ __forceinline__ void store_out(const PagedAttnParams& p, size_t head,
   if (lane == 0 && p.lse != nullptr) p.lse[head] = l == 0.f ? -INFINITY : m + log2f(l) - kLift<F16>;
 }
 
+// The states of parts c0 .. c1 of one (sequence, KV head) into the output of its query
+// head `head`, by one warp.
+template <bool F16>
+__device__ __forceinline__ void join(const PagedAttnParams& p, int c0, int c1, size_t head0, int head) {
+  const int lane = threadIdx.x & 31, G = p.groups;
+  float M = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  // kJoin parts at a time, one to a lane, with the sums so far scaled to the new maximum
+  for (int q0 = c0; q0 <= c1; q0 += kJoin) {
+    const int n = min(kJoin, c1 - q0 + 1);
+    auto at = [&](int i) -> size_t { return (size_t)(2 * (q0 + i) + (q0 + i == c0 ? 1 : 0)) * G + head; };
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (lane < n) ml = __ldcg(&p.part_ml[at(lane)]);
+    float4 x[kJoin];
+#pragma unroll
+    for (int i = 0; i < kJoin; ++i)
+      if (i < n) x[i] = __ldcg(reinterpret_cast<const float4*>(&p.part_o[at(i) * kD + lane * 4]));
+    float m = fmaxf(M, ml.x);
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+    const float mu = m == -INFINITY ? 0.f : m, old = exp2_fast(M - mu), f = exp2_fast(ml.x - mu);
+    M = m;
+    l = fmaf(l, old, f * ml.y);
+#pragma unroll
+    for (int d = 0; d < 4; ++d) o[d] *= old;
+#pragma unroll
+    for (int i = 0; i < kJoin; ++i) {
+      if (i >= n) break;
+      const float fi = __shfl_sync(0xffffffffu, f, i);
+      o[0] = fmaf(fi, x[i].x, o[0]);
+      o[1] = fmaf(fi, x[i].y, o[1]);
+      o[2] = fmaf(fi, x[i].z, o[2]);
+      o[3] = fmaf(fi, x[i].w, o[3]);
+    }
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+  store_out<F16>(p, head0 + head, lane, M == -INFINITY ? 0.f : M, l, o);
+}
+
 template <int NT, bool F16>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
     paged_attention_kernel(const __grid_constant__ PagedAttnParams p) {
   extern __shared__ __align__(16) uint8_t smem[];
   AttnShared<NT>& sm = *reinterpret_cast<AttnShared<NT>*>(smem);
-  int* pre = reinterpret_cast<int*>(smem + sizeof(AttnShared<NT>));
+  Line line(smem + sizeof(AttnShared<NT>), p.n_seqs);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int G = p.groups;
 
+  if (tid == 0) sm.n_joins = 0;
   pdl_wait();  // q, the new rows and the lengths come from earlier kernels
-  tile_prefix(p, pre);
+  line.fill(p);
   for (int b = blockIdx.x; b < p.n_seqs; b += gridDim.x)
-    if (pre[b + 1] == pre[b])
+    if (line.each[b] == 0)
       for (int i = tid; i < p.n_head * kD; i += kThreads) p.out[(size_t)b * p.n_head * kD + i] = 0;
-  const int U = pre[p.n_seqs];
+  const int U = line.pre[p.n_seqs];
   const int N = parts(p, U, (int)gridDim.x);
   const int c = blockIdx.x;
   if (c >= N) return;
-  int u = (int)((long long)c * U / N);
-  const int u1 = (int)((long long)(c + 1) * U / N);
+  const Parts cut(U, N);
+  // Where this part and (odd lanes) the next one begin: sequence b, head h, tile t0 of it.
+  // A (sequence, head) of up to PAGED_MIN_TILES tiles is not split (joining it would cost
+  // more): a cut in it moves to its first tile.
+  int u = min(cut.first(c + (lane & 1)), U - 1);
+  int b = line.seq_of(p.n_seqs, __shfl_sync(0xffffffffu, u, 0));
+  const int b1 = line.seq_of(p.n_seqs, __shfl_sync(0xffffffffu, u, 1));
+  if (lane & 1) b = b1;
+  const int from = u - line.pre[b];
+  int h = from / line.each[b], t0 = from - h * line.each[b];
+  if (line.each[b] <= PAGED_MIN_TILES + PAGED_SEQ_TILES) {
+    u -= t0;
+    t0 = 0;
+  }
+  const int u1 = c + 1 < N ? __shfl_sync(0xffffffffu, u, 1) : U;
+  u = __shfl_sync(0xffffffffu, u, 0);
+  b = __shfl_sync(0xffffffffu, b, 0);
+  h = __shfl_sync(0xffffffffu, h, 0);
+  t0 = __shfl_sync(0xffffffffu, t0, 0);
   const int tpp = p.page_size / kTile;
-  int b = seq_of(pre, p.n_seqs, u);
 
-  while (u < u1) {
-    while (pre[b + 1] <= u) ++b;
-    const int T = (pre[b + 1] - pre[b]) / p.n_kv;
-    const int h = (u - pre[b]) / T, t0 = (u - pre[b]) - h * T;
+  auto advance = [&]() {  // to the next (sequence, head) with rows
+    if (++h < p.n_kv) return;
+    h = 0;
+    do ++b;
+    while (b < p.n_seqs && line.each[b] == 0);
+  };
+
+  for (; u < u1; t0 = 0) {
+    const int work = line.each[b], T = work - PAGED_SEQ_TILES;
     const int t1 = min(T, t0 + (u1 - u));
+    if (t0 >= T) {  // only the end of its work: nothing to do
+      u += work - t0;
+      advance();
+      continue;
+    }
     const int rows = seq_rows(p, b);
     const int* table = p.table + (size_t)b * p.max_pages;
     const uint8_t* mask = p.mask == nullptr ? nullptr : p.mask + (size_t)b * p.max_pages * p.page_size;
@@ -357,49 +458,25 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
     }
     if (!whole) {
       // join: the CTAs whose parts hold this (sequence, head), first to last
-      const int s0 = u - t0;
-      const int c0 = (int)(((long long)(s0 + 1) * N - 1) / U), c1 = (int)(((long long)(s0 + T) * N - 1) / U);
-      __threadfence();
+      const int c0 = cut.of(u - t0), c1 = cut.of(u - t0 + T - 1);
       __syncthreads();
-      if (tid == 0) sm.last = atomicAdd(&p.counters[b * p.n_kv + h], 1) == c1 - c0;
-      __syncthreads();
-      if (sm.last) {
+      if (tid == 0) {
         __threadfence();
-        if (tid == 0) p.counters[b * p.n_kv + h] = 0;
-        for (int head = warp; head < G; head += kWarps) {
-          auto at = [&](int q) -> size_t { return (size_t)(2 * q + (q == c0 ? 1 : 0)) * G + head; };
-          float M = -INFINITY;
-          for (int q = c0 + lane; q <= c1; q += 32) M = fmaxf(M, __ldcg(&p.part_ml[at(q)]).x);
-#pragma unroll
-          for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-          const float mu = M == -INFINITY ? 0.f : M;
-          float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-          for (int q0 = c0; q0 <= c1; q0 += 32) {
-            const int n = min(32, c1 - q0 + 1);
-            float f = 0.f;
-            if (lane < n) {
-              const float2 ml = __ldcg(&p.part_ml[at(q0 + lane)]);
-              f = exp2_fast(ml.x - mu);
-              l = fmaf(f, ml.y, l);
-            }
-#pragma unroll 8
-            for (int i = 0; i < n; ++i) {
-              const float4 x = __ldcg(reinterpret_cast<const float4*>(&p.part_o[at(q0 + i) * kD + lane * 4]));
-              const float fi = __shfl_sync(0xffffffffu, f, i);
-              o[0] = fmaf(fi, x.x, o[0]);
-              o[1] = fmaf(fi, x.y, o[1]);
-              o[2] = fmaf(fi, x.z, o[2]);
-              o[3] = fmaf(fi, x.w, o[3]);
-            }
-          }
-#pragma unroll
-          for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
-          store_out<F16>(p, head0 + head, lane, mu, l, o);
+        if (atomicAdd(&p.counters[b * p.n_kv + h], 1) == c1 - c0) {  // this CTA is the last one and joins
+          __threadfence();
+          p.counters[b * p.n_kv + h] = 0;
+          sm.joins[sm.n_joins++] = make_int4(c0, c1, b, h);
         }
       }
     }
     __syncthreads();  // the shared state is free again
-    u += t1 - t0;
+    u += t1 == T ? work - t0 : t1 - t0;
+    advance();
+  }
+  // joins after the main loop, at most two (so that their registers are not the loop's)
+  for (int i = warp; i < sm.n_joins * G; i += kWarps) {
+    const int4 j = sm.joins[i / G];
+    join<F16>(p, j.x, j.y, (size_t)j.z * p.n_head + (size_t)j.w * G, i % G);
   }
   pdl_launch_dependents();
 }
@@ -413,17 +490,19 @@ constexpr int kWTiles = kWThreads / 4;  // tiles of one pass of a CTA
 
 __global__ void __launch_bounds__(kWThreads) paged_weight_kernel(const __grid_constant__ PagedAttnParams p) {
   extern __shared__ __align__(16) uint8_t smem[];
-  int* pre = reinterpret_cast<int*>(smem);
+  Line line(smem, p.n_seqs);
   pdl_wait();
-  tile_prefix(p, pre);
-  const int U = pre[p.n_seqs], tpp = p.page_size / kTile, G = p.groups;
+  line.fill(p);
+  const int U = line.pre[p.n_seqs], tpp = p.page_size / kTile, G = p.groups;
   const int i = (threadIdx.x & 3) * 4;
-  for (long long uu = (long long)blockIdx.x * kWTiles + (threadIdx.x >> 2); uu < U;
-       uu += (long long)gridDim.x * kWTiles) {
-    const int u = (int)uu;
-    const int b = seq_of(pre, p.n_seqs, u);
-    const int T = (pre[b + 1] - pre[b]) / p.n_kv;
-    const int h = (u - pre[b]) / T, tile = (u - pre[b]) - h * T;
+  // a warp takes eight units at a time, four lanes each
+  for (long long u0 = (long long)blockIdx.x * kWTiles + (threadIdx.x >> 5) * 8; u0 < U;
+       u0 += (long long)gridDim.x * kWTiles) {
+    const int u = min((int)u0 + ((threadIdx.x & 31) >> 2), U);
+    int b = line.seq_of(p.n_seqs, (int)u0);
+    while (u < U && line.pre[b + 1] <= u) ++b;
+    const int work = line.each[b], h = (u - line.pre[b]) / max(work, 1), tile = u - line.pre[b] - h * work;
+    if (u == U || tile >= work - PAGED_SEQ_TILES) continue;
     const int pg = p.table[(size_t)b * p.max_pages + tile / tpp];
     const float* lse = p.lse + (size_t)b * p.n_head + (size_t)h * G;
     const float* sp = p.scores + (size_t)u * G * kTile + i;
@@ -462,22 +541,22 @@ cudaError_t launch(K kernel, int grid, int threads, size_t smem, const PagedAttn
 
 template <int NT, bool F16>
 cudaError_t launch_attention(const PagedAttnParams& p, int grid, cudaStream_t stream) {
-  const size_t smem = sizeof(AttnShared<NT>) + (size_t)(p.n_seqs + 1) * sizeof(int);
+  const size_t smem = sizeof(AttnShared<NT>) + line_bytes(p.n_seqs);
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!configured[dev]) {
     cudaError_t e = cudaFuncSetAttribute(paged_attention_kernel<NT, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)(sizeof(AttnShared<NT>) + (PAGED_MAX_SEQS + 1) * sizeof(int)));
+                                         (int)(sizeof(AttnShared<NT>) + line_bytes(PAGED_MAX_SEQS)));
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
   return launch(paged_attention_kernel<NT, F16>, grid, kThreads, smem, p, stream);
 }
 
-long long most_tiles(int n_seqs, int n_kv, long long max_rows) {
-  return (long long)n_seqs * n_kv * ((max_rows + kTile - 1) / kTile);
+long long most_work(int n_seqs, int n_kv, long long max_rows) {
+  return (long long)n_seqs * n_kv * ((max_rows + kTile - 1) / kTile + PAGED_SEQ_TILES);
 }
 
 int grid_for(long long tiles, long long lists, int groups, int sms) {
@@ -492,7 +571,7 @@ size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 void paged_attention_plan(int n_seqs, int n_head, int n_kv, long long max_rows, bool tracked, int sms,
                           PagedAttnPlan* plan) {
-  const long long tiles = most_tiles(n_seqs, n_kv, max_rows);
+  const long long tiles = most_work(n_seqs, n_kv, max_rows);
   const int groups = n_head / n_kv;
   plan->grid = grid_for(tiles, (long long)n_seqs * n_kv, groups, sms);
   size_t at = PAGED_COUNTER_BYTES;
@@ -516,10 +595,10 @@ cudaError_t launch_paged_attention(const PagedAttnParams& p, int grid, int sms, 
   else
     e = f16 ? launch_attention<2, true>(p, grid, stream) : launch_attention<2, false>(p, grid, stream);
   if (e != cudaSuccess || p.weight == nullptr) return e;
-  const long long tiles = most_tiles(p.n_seqs, p.n_kv, (long long)p.max_pages * p.page_size);
+  const long long tiles = most_work(p.n_seqs, p.n_kv, (long long)p.max_pages * p.page_size);
   const long long n = (tiles + kWTiles - 1) / kWTiles;
   return launch(paged_weight_kernel, (int)(n < 8LL * sms ? n : 8LL * sms), kWThreads,
-                (size_t)(p.n_seqs + 1) * sizeof(int), p, stream);
+                line_bytes(p.n_seqs), p, stream);
 }
 
 }  // namespace nf4b
