@@ -21,6 +21,7 @@ from ttspipe_b200 import _lib, fastpath, model, nf4gemv, pagedkv
 
 pytestmark = pytest.mark.gpu
 
+FTYPE = {torch.float32: _lib.NF4B_F32, torch.float16: _lib.NF4B_F16, torch.bfloat16: _lib.NF4B_BF16}
 DT = {"bf16": torch.bfloat16, "fp16": torch.float16}
 U = {"bf16": 2.0 ** -8, "fp16": 2.0 ** -11}  # one rounding to nearest, relative
 
@@ -298,7 +299,7 @@ def test_write_has_the_bits_of_the_dense_cache(name, norm, freqs_dtype):
         at = torch.tensor([t], device="cuda")
         _lib.check(_lib.lib().nf4b_qk_rope_kv_ex(
             qkv[t].data_ptr(), qw.data_ptr() if norm else None, kw.data_ptr() if norm else None, 1e-6,
-            freqs[int(pos[t])].data_ptr(), pagedkv._FTYPE[freqs_dtype], at.data_ptr(), qd[t].data_ptr(),
+            freqs[int(pos[t])].data_ptr(), FTYPE[freqs_dtype], at.data_ptr(), qd[t].data_ptr(),
             kc.data_ptr(), vc.data_ptr(), nh, nkv, 128, n, _lib.act_type(DT[name]),
             torch.cuda.current_stream().cuda_stream))
     torch.cuda.synchronize()

@@ -5,8 +5,9 @@ Each ``csrc/*.cu`` is compiled separately (in parallel) with
 next to this file, so it travels with the source tree. The CUDA runtime is
 linked statically: the library carries its own runtime and shares only the
 driver (and therefore the current context and streams) with the PyTorch that
-calls it. ``python -m ttspipe_b200.build`` rebuilds when a source is newer
-than the library.
+calls it. ``csrc/pagedkv_bind.cpp`` becomes ``_pagedkv.so`` beside it, a Python
+module against this PyTorch's headers. ``python -m ttspipe_b200.build`` rebuilds
+when a source is newer than what was built from it.
 """
 
 from __future__ import annotations
@@ -24,6 +25,8 @@ CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 BUILD = PKG / "_build"
 LIB = PKG / "libnf4b200.so"
+BIND = PKG / "_pagedkv.so"
+BIND_SRC = CSRC / "pagedkv_bind.cpp"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-O3", "--expt-relaxed-constexpr",
@@ -52,8 +55,38 @@ def up_to_date() -> bool:
     return all(p.stat().st_mtime <= t for p in _deps())
 
 
+def build_binding(force: bool = False, verbose: bool = False) -> Path:
+    """Compile the Python binding of the paged KV cache. Returns its path."""
+    deps = [BIND_SRC, *INCLUDE.glob("*.h")]
+    if not force and BIND.exists() and all(p.stat().st_mtime <= BIND.stat().st_mtime for p in deps):
+        return BIND
+    import sysconfig
+
+    import torch
+
+    cxx = os.environ.get("CXX") or shutil.which("g++")
+    if not cxx:
+        raise FileNotFoundError("no C++ compiler (set CXX or install g++)")
+    BUILD.mkdir(exist_ok=True)
+    home = Path(torch.__file__).resolve().parent
+    inc = [INCLUDE, home / "include", home / "include" / "torch" / "csrc" / "api" / "include",
+           sysconfig.get_paths()["include"]]
+    tmp = BIND.with_suffix(".so.tmp")
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{i}" for i in inc), str(BIND_SRC),
+           f"-L{home / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-o", str(tmp)]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True, env=dict(os.environ, TMPDIR=str(BUILD)))
+    if r.returncode != 0:
+        raise RuntimeError(f"{cxx} failed on {BIND_SRC.name}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, BIND)
+    return BIND
+
+
 def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> Path:
-    """Compile every kernel source and link the shared library. Returns its path."""
+    """Compile the binding and every kernel source and link the shared library. Returns its path."""
+    build_binding(force=force, verbose=verbose)
     if not force and up_to_date() and not ptxas_info:
         return LIB
     BUILD.mkdir(exist_ok=True)

@@ -34,16 +34,29 @@ import torch
 from ttspipe_b200 import _lib
 
 HEAD_DIM = 128
-_FTYPE = {torch.float32: _lib.NF4B_F32, torch.float16: _lib.NF4B_F16, torch.bfloat16: _lib.NF4B_BF16}
-_ACT = {torch.bfloat16: _lib.NF4B_BF16, torch.float16: _lib.NF4B_F16}
 _stats = {"write": 0, "attention": 0, "evict": 0, "block": 0}
 _workspaces: dict = {}  # (kind, device, stream): (tensor, address, bytes); calls on other streams may overlap
 _retired: list = []  # replaced workspaces: a captured graph may still name them
-
+_native = None
 
 #: The current stream's handle, without the Stream object (2 us a call) torch.cuda.current_stream makes.
 _stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
+def _bound():
+    """The binding (csrc/pagedkv_bind.cpp), handed the library's functions. Raises if it has not been built."""
+    global _native
+    if _native is None:
+        lib = _lib.lib()
+        try:
+            from ttspipe_b200 import _pagedkv
+        except ImportError as exc:
+            raise RuntimeError("_pagedkv.so is not built; run `python -m ttspipe_b200.build`") from exc
+        _pagedkv.bind(*(ctypes.cast(getattr(lib, f"nf4b_paged_{name}"), ctypes.c_void_p).value
+                        for name in ("write", "attention", "evict")))
+        _native = _pagedkv
+    return _native
 
 
 def stats() -> dict:
@@ -62,31 +75,8 @@ def _grow(kind: str, device, stream: int, need: int):
     return got
 
 
-def _take(name: str, t, dtype, shape, device: int):
-    """The tensor's address; refused if it is not of this type, shape and device, or not contiguous."""
-    if t.dtype is not dtype or t.shape != shape or t.get_device() != device or not t.is_contiguous():
-        raise ValueError(f"{name}: contiguous {dtype} {tuple(shape)} on cuda:{device} needed, got {t.dtype} "
-                         f"{tuple(t.shape)} on {t.device}{'' if t.is_contiguous() else ', not contiguous'}")
-    return t.data_ptr()
-
-
-def _cache(k, v, block_table, weight=None, position=None):
-    """The library's description of a paged cache, the shape of its rows and its device, after their checks."""
-    dtype, shape, device = k.dtype, k.shape, k.get_device()
-    dt = _ACT.get(dtype)
-    if dt is None or device < 0:
-        raise ValueError(f"pools of {dtype} on {k.device} are not served")
-    table = block_table.shape
-    if len(shape) != 4 or shape[3] != HEAD_DIM or len(table) != 2 or 0 in shape or 0 in table:
-        raise ValueError(f"pools [n_pages, n_kv, page_size, {HEAD_DIM}] and a table [n_seqs, max_pages] needed, got "
-                         f"{tuple(shape)} and {tuple(table)}")
-    slots = shape[:3]
-    return _lib.PagedKv(
-        _take("k", k, dtype, shape, device), _take("v", v, dtype, shape, device),
-        _take("block_table", block_table, torch.int32, table, device),
-        None if weight is None else _take("weight", weight, torch.float32, slots, device),
-        None if position is None else _take("position", position, torch.int32, slots, device),
-        *table, *slots, dt), slots, device
+def _raise(status: int):
+    raise _lib.Nf4bError(status, _lib.last_error())
 
 
 def write(qkv, k, v, block_table, rows, positions, freqs, *, n_head: int, seqs=None, q_norm=None, k_norm=None,
@@ -100,26 +90,12 @@ def write(qkv, k, v, block_table, rows, positions, freqs, *, n_head: int, seqs=N
     `weight` is set to 0 and `position` to the token's position at the new rows. A
     token whose row or position is out of range (-1, say) is padding: nothing of it
     enters the cache. No two tokens of a call may name the same row."""
-    c, (_, n_kv, _), dev = _cache(k, v, block_table, weight, position)
-    dtype, width = k.dtype, (n_head + 2 * n_kv) * HEAD_DIM
-    if qkv.dim() != 2 or n_head < 1:
-        raise ValueError(f"qkv: [tokens, {width}] and n_head >= 1 needed, got {tuple(qkv.shape)} and {n_head}")
-    n = qkv.shape[0]
-    ft = _FTYPE.get(freqs.dtype)
-    if ft is None or freqs.dim() != 3:
-        raise ValueError(f"freqs: (rows, 64, 2) of fp32, fp16 or bf16 needed, got {freqs.dtype} {tuple(freqs.shape)}")
-    n_freqs = freqs.shape[0]
-    if out is None:
-        out = qkv.new_empty((n, n_head, HEAD_DIM))
-    _lib.check(_lib.lib().nf4b_paged_write(
-        c, _take("qkv", qkv, dtype, (n, width), dev), None if seqs is None else _take("seqs", seqs, torch.int32, (n,), dev),
-        _take("rows", rows, torch.int32, (n,), dev), _take("positions", positions, torch.int32, (n,), dev),
-        _take("freqs", freqs, freqs.dtype, (n_freqs, HEAD_DIM // 2, 2), dev), ft, n_freqs,
-        None if q_norm is None else _take("q_norm", q_norm, dtype, (HEAD_DIM,), dev),
-        None if k_norm is None else _take("k_norm", k_norm, dtype, (HEAD_DIM,), dev), eps,
-        _take("out", out, dtype, (n, n_head, HEAD_DIM), dev), n, n_head, _stream(dev)))
+    got = (_native or _bound()).write(qkv, k, v, block_table, rows, positions, freqs, n_head, seqs, q_norm, k_norm, eps,
+                                      weight, position, out, _stream(k.get_device()) if k.is_cuda else 0)
+    if type(got) is int:
+        _raise(got)
     _stats["write"] += 1
-    return out
+    return got
 
 
 def attention(q, k, v, block_table, lens, *, mask=None, scale: float | None = None, weight=None, out=None):
@@ -130,27 +106,21 @@ def attention(q, k, v, block_table, lens, *, mask=None, scale: float | None = No
     whatever they hold; a sequence that sees none gets zeros. `scale` defaults to
     128 ** -0.5. `weight` receives every visible row's weight, summed over the query
     heads of its KV head. Up to 16 query heads to a KV head."""
-    c, (_, n_kv, page_size), dev = _cache(k, v, block_table, weight)
-    dtype, shape = k.dtype, q.shape
-    if len(shape) != 3 or shape[0] != c.n_seqs or shape[2] != HEAD_DIM:
-        raise ValueError(f"q: [{c.n_seqs}, n_head, {HEAD_DIM}] needed, got {tuple(shape)}")
-    if out is None:
-        out = torch.empty_like(q)
-    if mask is not None and mask.dtype is torch.bool:
-        mask = mask.view(torch.uint8)
-    n_head, stream, lib = shape[1], _stream(dev), _lib.lib()
-    args = (_take("q", q, dtype, shape, dev), _take("lens", lens, torch.int32, (shape[0],), dev),
-            None if mask is None else _take("mask", mask, torch.uint8, (shape[0], c.max_pages * page_size), dev),
-            HEAD_DIM ** -0.5 if scale is None else scale, _take("out", out, dtype, shape, dev), n_head)
+    call, dev = (_native or _bound()).attention, k.get_device()
+    stream = _stream(dev) if dev >= 0 else 0
+    scale = HEAD_DIM ** -0.5 if scale is None else scale
     _, ws, size = _workspaces.get(("attention", dev, stream)) or (None, None, 0)
-    status = lib.nf4b_paged_attention(c, *args, ws, size, stream)
-    if status == _lib.NF4B_ERR_WORKSPACE:
-        _, ws, size = _grow("attention", dev, stream, lib.nf4b_paged_attention_workspace_size(
-            shape[0], n_head, n_kv, c.max_pages, page_size, weight is not None))
-        status = lib.nf4b_paged_attention(c, *args, ws, size, stream)
-    _lib.check(status)
+    got = call(q, k, v, block_table, lens, mask, scale, weight, out, ws, size, stream)
+    if type(got) is int:
+        if got != _lib.NF4B_ERR_WORKSPACE:
+            _raise(got)
+        _, ws, size = _grow("attention", dev, stream, _lib.lib().nf4b_paged_attention_workspace_size(
+            q.shape[0], q.shape[1], k.shape[1], block_table.shape[1], k.shape[2], weight is not None))
+        got = call(q, k, v, block_table, lens, mask, scale, weight, out, ws, size, stream)
+        if type(got) is int:
+            _raise(got)
     _stats["attention"] += 1
-    return out
+    return got
 
 
 def evict(k, v, weight, position, block_table, lens, *, budget: int, recent: int = 0, sink: int = 0,
@@ -165,21 +135,20 @@ def evict(k, v, weight, position, block_table, lens, *, budget: int, recent: int
     see - and the pages after them are free. `weight_out`, `position_out` and
     `lens_out` receive the rows' weights and positions and the new lengths; None: in place.
     The sequences must not share pages."""
-    c, slots, dev = _cache(k, v, block_table, weight, position)
-    weight_out = weight if weight_out is None else weight_out
-    position_out = position if position_out is None else position_out
-    lens_out = lens if lens_out is None else lens_out
-    n, stream, lib = c.n_seqs, _stream(dev), _lib.lib()
-    args = (_take("lens", lens, torch.int32, (n,), dev), budget, recent, sink,
-            _take("weight_out", weight_out, torch.float32, slots, dev),
-            _take("position_out", position_out, torch.int32, slots, dev),
-            _take("lens_out", lens_out, torch.int32, (n,), dev))
+    call, dev = (_native or _bound()).evict, k.get_device()
+    stream = _stream(dev) if dev >= 0 else 0
+    args = (k, v, weight, position, block_table, lens, budget, recent, sink,
+            weight if weight_out is None else weight_out, position if position_out is None else position_out,
+            lens if lens_out is None else lens_out)
     _, ws, size = _workspaces.get(("evict", dev, stream)) or (None, None, 0)
-    status = lib.nf4b_paged_evict(c, *args, ws, size, stream)
-    if status == _lib.NF4B_ERR_WORKSPACE:
-        _, ws, size = _grow("evict", dev, stream, lib.nf4b_paged_evict_workspace_size(
-            n, c.n_kv, c.max_pages, c.page_size, budget))
-        status = lib.nf4b_paged_evict(c, *args, ws, size, stream)
-    _lib.check(status)
+    got = call(*args, ws, size, stream)
+    if type(got) is int:
+        if got != _lib.NF4B_ERR_WORKSPACE:
+            _raise(got)
+        _, ws, size = _grow("evict", dev, stream, _lib.lib().nf4b_paged_evict_workspace_size(
+            block_table.shape[0], k.shape[1], block_table.shape[1], k.shape[2], budget))
+        got = call(*args, ws, size, stream)
+        if type(got) is int:
+            _raise(got)
     _stats["evict"] += 1
-    return lens_out
+    return got
