@@ -162,3 +162,66 @@ def test_oracle_kept_rows():
     assert po.kept(w, pos, 3, 1, 1).nonzero()[0].tolist() == [0, 3, 6]
     to, src = po.moves(po.kept(w, pos, 3, 1, 1), 3)
     assert to.tolist() == [1, 2] and src.tolist() == [3, 6]
+
+
+# ---- the cache's pages on the host -------------------------------------------
+
+
+def make_cache(n_pages=6, **kw):
+    return pagedkv.PagedKVCache(2, 3, 64, n_pages, 2, page_size=16, device="cpu", **kw)
+
+
+def test_pages_are_handed_out_and_taken_back():
+    c = make_cache()
+    c.reserve(0, 17)
+    c.reserve(1)
+    assert c.free_pages() == 3 and c.active.tolist() == [1, 1, 0]
+    own = [p for s in range(2) for p in c.block_table[s].tolist() if p >= 0]
+    assert len(set(own)) == 3 and (c.block_table[2] == -1).all()
+    for _ in range(15):
+        c.reserve(1)  # rows 2 to 16 share the page of the first
+    assert c.free_pages() == 3
+    c.reserve(1)
+    assert c.free_pages() == 2 and (c.block_table[1] >= 0).sum() == 2
+    c.trim(0, 16)
+    assert c.free_pages() == 3 and (c.block_table[0] >= 0).tolist() == [True, False, False, False]
+    c.lens[1] = 17
+    c.release(1)
+    assert c.free_pages() == 5 and c.lens[1] == 0 and c.active[1] == 0 and (c.block_table[1] == -1).all()
+
+
+def test_a_reservation_that_does_not_fit_changes_nothing():
+    c = make_cache()
+    c.reserve(0, 64)
+    before = c.block_table.clone()
+    with pytest.raises(ValueError, match="at most 64"):
+        c.reserve(0)
+    with pytest.raises(RuntimeError, match="2 are free"):
+        c.reserve(1, 33)
+    assert torch.equal(c.block_table, before) and c.free_pages() == 2 and c.active.tolist() == [1, 0, 0]
+    c.reserve(1, 32)
+    assert c.free_pages() == 0
+
+
+def test_a_step_counts_the_active_streams_only():
+    c = make_cache(track=False)
+    c.reserve(0, 5)
+    c.reserve(2, 1)
+    c.lens.copy_(torch.tensor([4, 0, 0]))
+    c.next_pos.copy_(torch.tensor([9, 0, 0]))
+    c.begin_step()
+    assert c.rows.tolist() == [4, -1, 0] and c.live.tolist() == [5, 0, 1]
+    c.end_step()
+    assert c.lens.tolist() == [5, 0, 1] and c.next_pos.tolist() == [10, 0, 1]
+    assert c.weight == [None, None]
+
+
+def test_rows_come_back_in_sequence_order():
+    c = make_cache()
+    c.reserve(0, 16)
+    c.reserve(1, 16)
+    c.reserve(0, 10)
+    for r in range(26):
+        c.k[1][int(c.block_table[0, r // 16]), :, r % 16] = r
+    k, v = c.rows_of(1, 0, 26)
+    assert k.shape == (1, 2, 26, 128) and k[0, 1, :, 5].tolist() == list(range(26)) and not v.any()

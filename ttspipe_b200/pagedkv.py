@@ -152,3 +152,191 @@ def evict(k, v, weight, position, block_table, lens, *, budget: int, recent: int
             _raise(got)
     _stats["evict"] += 1
     return got
+
+
+class PagedKVCache:
+    """The paged caches of `n_seqs` streams for `n_layers` blocks: each layer's pools, one
+    block table and one set of lengths for all of them (an eviction leaves every
+    head and layer of a stream equally many rows), and the pages' bookkeeping on the host.
+
+    A decode step: ``reserve(stream)`` for every stream that takes part (its next row needs a
+    page), ``begin_step()``, the blocks (``decode_block``), ``end_step()``; between steps
+    ``evict`` where streams grow past a budget. A stream without ``active`` is passed over.
+    Everything but ``reserve``, ``trim`` and ``release`` runs on the device and can be captured."""
+
+    def __init__(self, n_layers: int, n_seqs: int, max_len: int, n_pages: int, n_kv: int, *, page_size: int = 64,
+                 device, dtype=torch.bfloat16, track: bool = True):
+        self.n_layers, self.n_seqs, self.page_size, self.n_pages = n_layers, n_seqs, page_size, n_pages
+        self.max_pages = -(-max_len // page_size)
+        pool = (n_pages, n_kv, page_size, HEAD_DIM)
+
+        def per_layer(shape, dt):
+            return [torch.zeros(shape, dtype=dt, device=device) for _ in range(n_layers)]
+
+        self.k, self.v = per_layer(pool, dtype), per_layer(pool, dtype)
+        self.weight = per_layer(pool[:3], torch.float32) if track else [None] * n_layers
+        self.position = per_layer(pool[:3], torch.int32) if track else [None] * n_layers
+        self.block_table = torch.full((n_seqs, self.max_pages), -1, dtype=torch.int32, device=device)
+        i32 = dict(dtype=torch.int32, device=device)
+        self.lens = torch.zeros(n_seqs, **i32)       # rows of each stream
+        self.next_pos = torch.zeros(n_seqs, **i32)   # position of its next token
+        self.active = torch.zeros(n_seqs, **i32)     # 1: takes part in the steps
+        self.rows = torch.full((n_seqs,), -1, **i32)  # of a step: the new row of each stream, -1 for none
+        self.live = torch.zeros(n_seqs, **i32)        # of a step: the rows its token attends to
+        self._left = torch.zeros(n_seqs, **i32)
+        self._free = list(range(n_pages - 1, -1, -1))
+        self._pages: list = [[] for _ in range(n_seqs)]
+        self._rows = [0] * n_seqs  # rows promised to each stream
+
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def reserve(self, seq: int, rows: int = 1) -> None:
+        """Pages for `rows` more rows of a stream, which becomes active. Refuses (ValueError) what is past the
+        stream's capacity and (RuntimeError) what the free pages do not hold, changing nothing."""
+        want = self._rows[seq] + rows
+        need = -(-want // self.page_size)
+        if rows < 0 or need > self.max_pages:
+            raise ValueError(f"{want} rows of stream {seq}: at most {self.max_pages * self.page_size}")
+        held = self._pages[seq]
+        if need - len(held) > len(self._free):
+            raise RuntimeError(f"stream {seq} needs {need - len(held)} pages, {len(self._free)} are free")
+        if need > len(held):
+            new = [self._free.pop() for _ in range(need - len(held))]
+            self.block_table[seq, len(held):need] = torch.tensor(new, dtype=torch.int32).to(self.block_table.device)
+            held += new
+        if self._rows[seq] == 0 and rows:
+            self.active[seq] = 1
+        self._rows[seq] = want
+
+    def trim(self, seq: int, rows: int) -> None:
+        """A stream has `rows` rows left (after an eviction): later pages become free."""
+        self._rows[seq] = min(self._rows[seq], rows)
+        keep = -(-self._rows[seq] // self.page_size)
+        held = self._pages[seq]
+        if keep < len(held):
+            self.block_table[seq, keep:len(held)] = -1
+            self._free += held[keep:][::-1]
+            del held[keep:]
+
+    def release(self, seq: int) -> None:
+        """A stream has ended: its pages become free and its place can be used again."""
+        self.trim(seq, 0)
+        self.lens[seq] = 0
+        self.next_pos[seq] = 0
+        self.active[seq] = 0
+
+    def begin_step(self) -> None:
+        """Rows and lengths of one new token of each active stream."""
+        torch.add(self.lens, self.active, out=self.live)
+        torch.add(self.lens, 1, out=self.rows).mul_(self.active).sub_(1)
+
+    def end_step(self) -> None:
+        self.lens.copy_(self.live)
+        self.next_pos.add_(self.active)
+
+    def write(self, layer: int, qkv, rows, positions, freqs, *, n_head: int, **kw):
+        """``write`` into one layer's pools."""
+        return write(qkv, self.k[layer], self.v[layer], self.block_table, rows, positions, freqs, n_head=n_head,
+                     weight=self.weight[layer], position=self.position[layer], **kw)
+
+    def attention(self, layer: int, q, **kw):
+        """``attention`` of a step's tokens over one layer's pools."""
+        return attention(q, self.k[layer], self.v[layer], self.block_table, self.live, weight=self.weight[layer], **kw)
+
+    def evict(self, budget: int, *, recent: int = 0, sink: int = 0) -> None:
+        """``evict`` in every layer (each head by its own weights); afterwards ``trim`` frees the pages."""
+        for i in range(self.n_layers):
+            evict(self.k[i], self.v[i], self.weight[i], self.position[i], self.block_table, self.lens, budget=budget,
+                  recent=recent, sink=sink, lens_out=self._left)
+        self.lens.copy_(self._left)
+
+    def evict_and_trim(self, budget: int, *, recent: int = 0, sink: int = 0) -> None:
+        """``evict``, and the pages that it leaves free are taken back (on the host, from its own count of rows)."""
+        self.evict(budget, recent=recent, sink=sink)
+        for seq in range(self.n_seqs):
+            self.trim(seq, budget)
+
+    def rows_of(self, layer: int, seq: int, rows: int):
+        """(k, v) [1, n_kv, rows, 128]: a copy of a stream's first `rows` rows."""
+        pages = self.block_table[seq, : -(-rows // self.page_size)].long()
+        return tuple(t[pages].transpose(0, 1).flatten(1, 2)[None, :, :rows] for t in (self.k[layer], self.v[layer]))
+
+
+def _norms(a):
+    qn, kn = (a.q_norm, a.k_norm) if a.attention_qk_norm else (None, None)
+    eps = float(qn.eps if qn is not None and qn.eps is not None else 1e-6)
+    return dict(q_norm=None if qn is None else qn.weight, k_norm=None if kn is None else kn.weight, eps=eps)
+
+
+def _linear(module, x, **kw):
+    from ttspipe_b200 import nf4gemv
+
+    if getattr(module, "_nf4_fast", None) is None:
+        nf4gemv.prepare(module)
+    y = nf4gemv.matmul(module, x, **kw)
+    if y is None and "norm" not in kw:
+        raise ValueError(f"the block's {module} does not run on the NF4 kernels for {tuple(x.shape)} {x.dtype}")
+    return y
+
+
+def _normed_linear(norm, module, x):
+    """norm, then the linear: in one launch where the kernel serves that."""
+    from ttspipe_b200 import fusedops
+
+    y = _linear(module, x, norm=(norm.weight, norm.eps))
+    return _linear(module, fusedops.rms_norm(x, norm.weight, norm.eps)) if y is None else y
+
+
+def _feed_forward(block, h):
+    from ttspipe_b200 import fusedops, nf4gemv
+
+    ff, norm = block.feed_forward, block.ffn_norm
+    for module in (ff.w1, ff.w3):
+        if getattr(module, "_nf4_fast", None) is None:
+            nf4gemv.prepare(module)
+    g = nf4gemv.matmul_gated(ff.w1, ff.w3, h, norm=(norm.weight, norm.eps))
+    if g is None:
+        hn = fusedops.rms_norm(h, norm.weight, norm.eps)
+        g = nf4gemv.matmul_gated(ff.w1, ff.w3, hn)
+        if g is None:
+            g = _linear(ff.w3, hn, epi=nf4gemv.EPI_SILU_GATE, operand=_linear(ff.w1, hn))
+    return _linear(ff.w2, g, epi=nf4gemv.EPI_RESIDUAL, operand=h)
+
+
+def decode_block(block, x, freqs, cache: PagedKVCache, layer: int):
+    """One token of every stream through a transformer block: ``fusedlayer.decode_block``
+    for a batch, over a paged cache. `x` is [n_seqs, 1, dim], `freqs` the whole rotary
+    table (rows, 64, 2); between ``cache.begin_step()`` and ``cache.end_step()``. The
+    rows of streams that are not active are computed and mean nothing."""
+    from ttspipe_b200 import nf4gemv
+
+    a = block.attention
+    qkv = _normed_linear(block.attention_norm, a.wqkv, x)
+    q = cache.write(layer, qkv.view(cache.n_seqs, -1), cache.rows, cache.next_pos, freqs, n_head=a.n_head, **_norms(a))
+    y = cache.attention(layer, q).view(cache.n_seqs, 1, -1)
+    h = _linear(a.wo, y, epi=nf4gemv.EPI_RESIDUAL, operand=x)
+    out = _feed_forward(block, h)
+    _stats["block"] += 1
+    return out
+
+
+def prefill_block(block, x, freqs, cache: PagedKVCache, layer: int, seq: int, rows: int = 0, position: int = 0):
+    """The tokens `x` [1, T, dim] of one stream through a transformer block, entering the
+    cache after its `rows` rows, from token position `position` on (both on the host;
+    ``reserve`` T rows first and, after the last layer, add T to ``lens`` and ``next_pos``).
+    Each attends to the rows before it and to itself, by the grouped torch formulation
+    of ``fastpath``; weights are not accumulated here."""
+    from ttspipe_b200 import fastpath, nf4gemv
+
+    a, n = block.attention, x.shape[1]
+    dev = x.device
+    qkv = _normed_linear(block.attention_norm, a.wqkv, x)
+    at = torch.arange(n, dtype=torch.int32, device=dev)
+    q = cache.write(layer, qkv.view(n, -1), at + rows, at + position, freqs, n_head=a.n_head,
+                    seqs=torch.full_like(at, seq), **_norms(a))
+    k, v = cache.rows_of(layer, seq, rows + n)
+    mask = (torch.arange(rows + n, device=dev)[None] <= at[:, None] + rows)[None, None]
+    y = fastpath._grouped_torch(q.transpose(0, 1)[None], k, v, mask, a.n_head, a.n_local_heads, HEAD_DIM)
+    h = _linear(a.wo, y.transpose(1, 2).reshape(1, n, -1), epi=nf4gemv.EPI_RESIDUAL, operand=x)
+    return _feed_forward(block, h)
