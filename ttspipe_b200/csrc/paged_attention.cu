@@ -33,7 +33,7 @@ constexpr int kD = 128;
 constexpr int kTile = PAGED_TILE;
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kJoin = 32;  // parts whose outputs the joining warp requests at once
+constexpr int kJoin = 16;  // parts whose outputs a joining warp requests at once
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -162,43 +162,71 @@ __device__ __forceinline__ void store_out(const PagedAttnParams& p, size_t head,
   if (lane == 0 && p.lse != nullptr) p.lse[head] = l == 0.f ? -INFINITY : m + log2f(l) - kLift<F16>;
 }
 
-// The states of parts c0 .. c1 of one (sequence, KV head) into the output of its query
-// head `head`, by one warp.
+// Parts first .. of one (sequence, query head), one state (maximum, sum) to a lane, and
+// kJoin outputs, four dimensions to a lane.
+struct JoinPiece {
+  float2 ml;
+  float4 o[kJoin];
+};
+
+// The states of the parts of up to two (sequence, KV head)s - joins[.] = (first part, last part,
+// sequence, head) - into their outputs. Each warp takes every fourth query head, kJoin
+// parts at a time, and requests the next ones before it adds up these.
 template <bool F16>
-__device__ __forceinline__ void join(const PagedAttnParams& p, int c0, int c1, size_t head0, int head) {
-  const int lane = threadIdx.x & 31, G = p.groups;
-  float M = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  // kJoin parts at a time, one to a lane, with the sums so far scaled to the new maximum
-  for (int q0 = c0; q0 <= c1; q0 += kJoin) {
-    const int n = min(kJoin, c1 - q0 + 1);
-    auto at = [&](int i) -> size_t { return (size_t)(2 * (q0 + i) + (q0 + i == c0 ? 1 : 0)) * G + head; };
-    float2 ml = make_float2(-INFINITY, 0.f);
-    if (lane < n) ml = __ldcg(&p.part_ml[at(lane)]);
-    float4 x[kJoin];
+__device__ __forceinline__ void join_parts(const PagedAttnParams& p, const int4* joins, int n_joins) {
+  const int lane = threadIdx.x & 31, G = p.groups, n_heads = n_joins * G;
+  int i = threadIdx.x >> 5, q0 = 0;  // the warp's next pieces: query head, first part
+  auto fetch = [&](JoinPiece& x) {
+    const int4 j = joins[i / G];
+    const int head = i % G, first = j.x + q0, n = min(kJoin, j.y - first + 1);
+    auto at = [&](int k) -> size_t { return (size_t)(2 * (first + k) + (first + k == j.x ? 1 : 0)) * G + head; };
+    x.ml = make_float2(-INFINITY, 0.f);
+    if (lane < n) x.ml = __ldcg(&p.part_ml[at(lane)]);
 #pragma unroll
-    for (int i = 0; i < kJoin; ++i)
-      if (i < n) x[i] = __ldcg(reinterpret_cast<const float4*>(&p.part_o[at(i) * kD + lane * 4]));
-    float m = fmaxf(M, ml.x);
+    for (int k = 0; k < kJoin; ++k)
+      if (k < n) x.o[k] = __ldcg(reinterpret_cast<const float4*>(&p.part_o[at(k) * kD + lane * 4]));
+  };
+  JoinPiece x, next;
+  if (i < n_heads) fetch(x);
+  float M = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  while (i < n_heads) {
+    const int4 j = joins[i / G];
+    const int head = i % G, n = min(kJoin, j.y - (j.x + q0) + 1);
+    const bool last = j.x + q0 + kJoin > j.y;
+    if (last) {
+      i += kWarps;
+      q0 = 0;
+    } else {
+      q0 += kJoin;
+    }
+    if (i < n_heads) fetch(next);
+    // the sums so far are scaled to the new maximum
+    float m = fmaxf(M, x.ml.x);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-    const float mu = m == -INFINITY ? 0.f : m, old = exp2_fast(M - mu), f = exp2_fast(ml.x - mu);
+    const float mu = m == -INFINITY ? 0.f : m, old = exp2_fast(M - mu), f = exp2_fast(x.ml.x - mu);
     M = m;
-    l = fmaf(l, old, f * ml.y);
+    l = fmaf(l, old, f * x.ml.y);
 #pragma unroll
     for (int d = 0; d < 4; ++d) o[d] *= old;
 #pragma unroll
-    for (int i = 0; i < kJoin; ++i) {
-      if (i >= n) break;
-      const float fi = __shfl_sync(0xffffffffu, f, i);
-      o[0] = fmaf(fi, x[i].x, o[0]);
-      o[1] = fmaf(fi, x[i].y, o[1]);
-      o[2] = fmaf(fi, x[i].z, o[2]);
-      o[3] = fmaf(fi, x[i].w, o[3]);
+    for (int k = 0; k < kJoin; ++k) {
+      const float fk = __shfl_sync(0xffffffffu, f, k);
+      if (k >= n) continue;
+      o[0] = fmaf(fk, x.o[k].x, o[0]);
+      o[1] = fmaf(fk, x.o[k].y, o[1]);
+      o[2] = fmaf(fk, x.o[k].z, o[2]);
+      o[3] = fmaf(fk, x.o[k].w, o[3]);
     }
-  }
+    if (last) {
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
-  store_out<F16>(p, head0 + head, lane, M == -INFINITY ? 0.f : M, l, o);
+      for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+      store_out<F16>(p, (size_t)j.z * p.n_head + (size_t)j.w * G + head, lane, M == -INFINITY ? 0.f : M, l, o);
+      M = -INFINITY;
+      l = o[0] = o[1] = o[2] = o[3] = 0.f;
+    }
+    x = next;
+  }
 }
 
 template <int NT, bool F16>
@@ -474,10 +502,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
     advance();
   }
   // joins after the main loop, at most two (so that their registers are not the loop's)
-  for (int i = warp; i < sm.n_joins * G; i += kWarps) {
-    const int4 j = sm.joins[i / G];
-    join<F16>(p, j.x, j.y, (size_t)j.z * p.n_head + (size_t)j.w * G, i % G);
-  }
+  join_parts<F16>(p, sm.joins, sm.n_joins);
   pdl_launch_dependents();
 }
 
