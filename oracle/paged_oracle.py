@@ -1,5 +1,5 @@
 """The paged KV cache's operators in NumPy and 64 bits, one sequence and head after
-another (the checker, never the product). Pools are [n_pages, n_kv, page_size, ...]
+another (for the tests, never the product). Pools are [n_pages, n_kv, page_size, ...]
 arrays of values, not bit patterns."""
 
 from __future__ import annotations

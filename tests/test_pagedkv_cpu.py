@@ -145,7 +145,7 @@ def test_python_refuses_tensors_on_the_host():
 
 
 def test_oracle_attention_is_a_softmax():
-    """The checker against itself: weights sum to the group's heads, and one row gives its value."""
+    """The oracle against itself: weights sum to the group's heads, and one row gives its value."""
     rng = np.random.default_rng(0)
     k, v = rng.standard_normal((3, 1, 16, 128)), rng.standard_normal((3, 1, 16, 128))
     table = np.array([[2, 0, -1]])

@@ -12,14 +12,25 @@
 // nothing. Scores are kept in units of log2 (scale * log2 e folded in after the
 // product), products and sums in fp32.
 //
-// Work split. The unit of work is a tile of 16 rows of one (sequence, KV head):
-// page sizes are multiples of 16, so a tile lies in one page. All tiles of all
-// sequences and heads, in that order, are one line that is cut into equal parts,
-// one for each CTA, from the lengths on the device: ragged batches balance, and one
-// captured graph serves every length. A (sequence, head) that lies in one CTA's
-// part is finished there; one that several CTAs share is joined by the CTA that
-// finishes it last (a counter of each (sequence, head), back at 0 afterwards), in
-// the order of the parts, so results do not depend on timing.
+// What bounds it. A row of a KV head is 512 bytes and 4 * 128 * groups operations, so
+// memory does: 64 sequences of 8192 rows (32 query and 8 KV heads, 2.1 GB) take 315 us,
+// 6.8 TB/s, the rate of a plain copy on the same GPU, with the tensor pipe 15-18% busy.
+// Keys and values go from global memory straight into MMA fragments: a lane reads the
+// 16-byte pieces of a row that are its fragment once q's dimensions and v's are taken in
+// that order (a sum does not mind), so there is no staging, no bank conflict and nothing to wait
+// for but the loads; 3 CTAs of 4 warps an SM, each warp a tile of keys and values ahead, keep
+// up to 96 KB of them requested. Few rows are latency: 1 x 19 rows 3.7 us, 1 x 2048 rows
+// 7.9 us (about 1.0 to find the part, 2.3 for its two tiles a warp, 0.4 to join the warps, 1.1
+// for the counter, 2.3 to join the parts).
+//
+// Work split. The unit of work is a tile of 16 rows of one (sequence, KV head): page
+// sizes are multiples of 16, so a tile lies in one page. All tiles of all sequences and
+// heads, in that order, and what each (sequence, head) costs besides, are one line that
+// is cut into equal parts, one for each CTA, from the lengths on the device: ragged
+// batches balance, and one captured graph serves every length. A (sequence, head) that
+// lies in one CTA's part is finished there; one that several CTAs share is joined by the
+// CTA that finishes it last (a counter of each (sequence, head), back at 0 afterwards),
+// in the order of the parts, so results do not depend on timing.
 
 #include "common.cuh"
 #include "gemv_unit.cuh"
@@ -110,15 +121,15 @@ struct Line {
 
 constexpr size_t line_bytes(int n_seqs) { return (size_t)(2 * n_seqs + 1) * sizeof(int); }
 
-// The number of parts: as many CTAs as there are, but paged_min_tiles units of work for each unless that puts
-// several (sequence, head)s into one part while CTAs are left.
+// The number of parts: as many as CTAs, but paged_min_tiles units of work in each unless
+// that puts several (sequence, head)s into one part while CTAs are left.
 __device__ __forceinline__ int parts(const PagedAttnParams& p, int work, int ctas) {
   const int least = paged_min_tiles(p.groups), by_work = (work + least - 1) / least;
   return min(ctas, max(by_work, min(p.n_seqs * p.n_kv, work)));
 }
 
-// Part c of `work` units in n parts: its first unit, the earlier parts one longer where they do not
-// come out even; and the part of a unit.
+// Part c of `work` units in n parts: its first unit, the earlier parts one longer where
+// they do not come out even; and the part of a unit.
 struct Parts {
   int each, longer;
   __device__ __forceinline__ Parts(int work, int n) : each(work / n), longer(work - work / n * n) {}
@@ -176,9 +187,10 @@ struct JoinPiece {
   float4 o[kJoin];
 };
 
-// The states of the parts of up to two (sequence, KV head)s - joins[.] = (first part, last part,
-// sequence, head) - into their outputs. Each warp takes every fourth query head, kJoin
-// parts at a time, and requests the next ones before it adds up these.
+// The states of the parts of up to two (sequence, KV head)s - joins[.] = (first part,
+// last part, sequence, head) - into their outputs. Each warp takes every fourth query
+// head, kJoin parts at a time, and requests the next ones before it adds up these
+// (16 heads of 24 parts: 7 us, 10 when each waited for its own).
 template <bool F16>
 __device__ __forceinline__ void join_parts(const PagedAttnParams& p, const int4* joins, int n_joins) {
   const int lane = threadIdx.x & 31, G = p.groups, n_heads = n_joins * G;
@@ -516,9 +528,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
 }
 
 // weight[row] += sum over the group's heads of 2^(score - lse), from the scores the
-// attention kernel left. Four rows to a thread; a reduction instruction instead of a
-// read and a write, so that sequences which share a page add up. Rows that take no
-// part have the score -inf and receive 0.
+// attention kernel left (a row's weight needs the sum over all rows, which only the
+// joins know). Four rows to a thread; a reduction instruction instead of a read and a
+// write, so that sequences which share a page add up. Rows that take no part have the
+// score -inf and receive 0. Memory bounds it: 4 groups + 8 bytes a row and KV head, 20 us
+// for 64 x 8192 rows (100 MB), about 4 us for small calls.
 constexpr int kWThreads = 256;
 constexpr int kWTiles = kWThreads / 4;  // tiles of one pass of a CTA
 
