@@ -180,11 +180,14 @@ __device__ __forceinline__ void store_out(const PagedAttnParams& p, size_t head,
   if (lane == 0 && p.lse != nullptr) p.lse[head] = l == 0.f ? -INFINITY : m + log2f(l) - kLift<F16>;
 }
 
-// Parts first .. of one (sequence, query head), one state (maximum, sum) to a lane, and
-// kJoin outputs, four dimensions to a lane.
+// Up to kJoin parts of one (sequence, query head): their states (maximum, sum), one to a
+// lane, and their outputs, four dimensions to a lane.
 struct JoinPiece {
   float2 ml;
   float4 o[kJoin];
+  size_t head;  // of all sequences' query heads
+  int n;        // parts; 0: nothing
+  bool last;    // the last ones of this head
 };
 
 // The states of the parts of up to two (sequence, KV head)s - joins[.] = (first part,
@@ -193,59 +196,58 @@ struct JoinPiece {
 // (16 heads of 24 parts: 7 us, 10 when each waited for its own).
 template <bool F16>
 __device__ __forceinline__ void join_parts(const PagedAttnParams& p, const int4* joins, int n_joins) {
-  const int lane = threadIdx.x & 31, G = p.groups, n_heads = n_joins * G;
-  int i = threadIdx.x >> 5, q0 = 0;  // the warp's next pieces: query head, first part
-  auto fetch = [&](JoinPiece& x) {
-    const int4 j = joins[i / G];
-    const int head = i % G, first = j.x + q0, n = min(kJoin, j.y - first + 1);
-    auto at = [&](int k) -> size_t { return (size_t)(2 * (first + k) + (first + k == j.x ? 1 : 0)) * G + head; };
-    x.ml = make_float2(-INFINITY, 0.f);
-    if (lane < n) x.ml = __ldcg(&p.part_ml[at(lane)]);
-#pragma unroll
-    for (int k = 0; k < kJoin; ++k)
-      if (k < n) x.o[k] = __ldcg(reinterpret_cast<const float4*>(&p.part_o[at(k) * kD + lane * 4]));
-  };
+  const int lane = threadIdx.x & 31, G = p.groups;
+  int i = threadIdx.x >> 5, q0 = 0;  // the next pieces: query head, first part
   JoinPiece x, next;
-  if (i < n_heads) fetch(x);
+  x.n = 0;
   float M = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  while (i < n_heads) {
-    const int4 j = joins[i / G];
-    const int head = i % G, n = min(kJoin, j.y - (j.x + q0) + 1);
-    const bool last = j.x + q0 + kJoin > j.y;
-    if (last) {
-      i += kWarps;
-      q0 = 0;
-    } else {
-      q0 += kJoin;
+#pragma unroll 1
+  do {
+    next.n = 0;
+    if (i < n_joins * G) {
+      const int4 j = joins[i / G];
+      const int head = i % G, first = j.x + q0, n = min(kJoin, j.y - first + 1);
+      auto at = [&](int k) -> size_t { return (size_t)(2 * (first + k) + (first + k == j.x ? 1 : 0)) * G + head; };
+      next.ml = make_float2(-INFINITY, 0.f);
+      if (lane < n) next.ml = __ldcg(&p.part_ml[at(lane)]);
+#pragma unroll
+      for (int k = 0; k < kJoin; ++k)
+        if (k < n) next.o[k] = __ldcg(reinterpret_cast<const float4*>(&p.part_o[at(k) * kD + lane * 4]));
+      next.head = (size_t)j.z * p.n_head + (size_t)j.w * G + head;
+      next.n = n;
+      next.last = first + kJoin > j.y;
+      q0 = next.last ? 0 : q0 + kJoin;
+      i += next.last ? kWarps : 0;
     }
-    if (i < n_heads) fetch(next);
-    // the sums so far are scaled to the new maximum
-    float m = fmaxf(M, x.ml.x);
+    if (x.n) {
+      // the sums so far are scaled to the new maximum
+      float m = fmaxf(M, x.ml.x);
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-    const float mu = m == -INFINITY ? 0.f : m, old = exp2_fast(M - mu), f = exp2_fast(x.ml.x - mu);
-    M = m;
-    l = fmaf(l, old, f * x.ml.y);
+      for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+      const float mu = m == -INFINITY ? 0.f : m, old = exp2_fast(M - mu), f = exp2_fast(x.ml.x - mu);
+      M = m;
+      l = fmaf(l, old, f * x.ml.y);
 #pragma unroll
-    for (int d = 0; d < 4; ++d) o[d] *= old;
+      for (int d = 0; d < 4; ++d) o[d] *= old;
 #pragma unroll
-    for (int k = 0; k < kJoin; ++k) {
-      const float fk = __shfl_sync(0xffffffffu, f, k);
-      if (k >= n) continue;
-      o[0] = fmaf(fk, x.o[k].x, o[0]);
-      o[1] = fmaf(fk, x.o[k].y, o[1]);
-      o[2] = fmaf(fk, x.o[k].z, o[2]);
-      o[3] = fmaf(fk, x.o[k].w, o[3]);
-    }
-    if (last) {
+      for (int k = 0; k < kJoin; ++k) {
+        const float fk = __shfl_sync(0xffffffffu, f, k);
+        if (k >= x.n) continue;
+        o[0] = fmaf(fk, x.o[k].x, o[0]);
+        o[1] = fmaf(fk, x.o[k].y, o[1]);
+        o[2] = fmaf(fk, x.o[k].z, o[2]);
+        o[3] = fmaf(fk, x.o[k].w, o[3]);
+      }
+      if (x.last) {
 #pragma unroll
-      for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
-      store_out<F16>(p, (size_t)j.z * p.n_head + (size_t)j.w * G + head, lane, M == -INFINITY ? 0.f : M, l, o);
-      M = -INFINITY;
-      l = o[0] = o[1] = o[2] = o[3] = 0.f;
+        for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+        store_out<F16>(p, x.head, lane, M == -INFINITY ? 0.f : M, l, o);
+        M = -INFINITY;
+        l = o[0] = o[1] = o[2] = o[3] = 0.f;
+      }
     }
     x = next;
-  }
+  } while (x.n);
 }
 
 template <int NT, bool F16>

@@ -221,7 +221,6 @@ __global__ void __launch_bounds__(kWriteWarps * 32, kPairs == 4 ? 7 : 1) paged_w
 // counts), and 104 to move some 524,000 rows, 256 bytes of key and of value each between
 // scattered places, at 5.2 TB/s of DRAM. 1 x 2048 rows are the chain alone, 11 us.
 constexpr int kBins = 2048;
-constexpr int kDeep = 4;  // groups of 128 rows that a warp requests at once
 
 // Weights in rising order as unsigned integers; 0xFFFFFFFF (no weight maps there,
 // NaN being taken as -inf) is for the protected rows, 0 for rows without a page.
@@ -281,10 +280,12 @@ __device__ __forceinline__ int* cluster_peer(int* p, unsigned rank) {  // the sa
 }
 
 // A list belongs to a cluster of `size` CTAs, each with an equal share of its rows, and
-// each warp of them with a run of that. kOnce: a run is at most kDeep * 128 rows, whose
-// keys stay in registers; longer runs are read again (from L2) for every step.
-template <int kThreads, bool kOnce>
-__global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : 4)
+// each warp of them with a run of that, kDeep groups of 128 rows at a time. kOnce: that is
+// the whole run, and its keys stay in registers; longer runs are read again (from L2) for every
+// step. The code is unrolled over the groups and runs once, so where a list is short its
+// fetching costs as much as its work (1 x 2048 rows: 11.1 us with kDeep 4, 8.7 with 2).
+template <int kThreads, int kDeep, bool kOnce>
+__global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : 1024 / kThreads)
     paged_select_kernel(const __grid_constant__ PagedEvictParams p, int size) {
   __shared__ alignas(16) int hists[3][kBins];  // of each step: other CTAs of the cluster may still read the last one's
   __shared__ int part[3][32];
@@ -730,17 +731,20 @@ void paged_evict_plan(int n_seqs, int n_kv, long long max_rows, int budget, Page
 
 cudaError_t launch_paged_evict(const PagedEvictParams& p, int sms, cudaStream_t stream) {
   const int lists = p.n_seqs * p.n_kv, cap = p.max_pages * p.page_size;
-  // 256 threads hold the keys of 4096 rows; longer lists get 1024 for each 16384 rows, in
-  // clusters of up to 8 CTAs (131072 rows), and still longer ones those 8 and several reads
+  // 256 or 512 threads hold the keys of 8 rows each; longer lists get 1024 with 16 rows each
+  // (8 x 32768 rows: 135 us, 149 with 8), in clusters of up to 8 CTAs (131072 rows), and still
+  // longer ones those 8 and several reads
   int cluster = 1;
-  while (cluster < 8 && cap > cluster * 1024 * 4 * kDeep) cluster *= 2;
+  while (cluster < 8 && cap > cluster * 16384) cluster *= 2;
   cudaError_t e;
-  if (cap <= 256 * 4 * kDeep)
-    e = launch(paged_select_kernel<256, true>, lists, 256, 0, 1, stream, p, 1);
-  else if (cap <= cluster * 1024 * 4 * kDeep)
-    e = launch(paged_select_kernel<1024, true>, lists * cluster, 1024, 0, cluster, stream, p, cluster);
+  if (cap <= 2048)
+    e = launch(paged_select_kernel<256, 2, true>, lists, 256, 0, 1, stream, p, 1);
+  else if (cap <= 4096)
+    e = launch(paged_select_kernel<512, 2, true>, lists, 512, 0, 1, stream, p, 1);
+  else if (cap <= cluster * 16384)
+    e = launch(paged_select_kernel<1024, 4, true>, lists * cluster, 1024, 0, cluster, stream, p, cluster);
   else
-    e = launch(paged_select_kernel<1024, false>, lists * cluster, 1024, 0, cluster, stream, p, cluster);
+    e = launch(paged_select_kernel<1024, 4, false>, lists * cluster, 1024, 0, cluster, stream, p, cluster);
   if (e != cudaSuccess) return e;
   const long long want = (long long)lists * ((p.max_moves + kMovePiece - 1) / kMovePiece), most = 4LL * sms;  // all resident
   return launch(paged_move_kernel, (int)(want < 1 ? 1 : want < most ? want : most), kMoveWarps * 32, 0, 1,
