@@ -197,6 +197,18 @@ def test_attention_many_short_sequences():
     check_attention(p, q, "bf16", got=attend(p, q, weight=p.weight), weight=p.weight)
 
 
+@pytest.mark.parametrize("heads,lens", [((16, 1), [30000]), ((13, 1), [17, 12001, 12002]), ((4, 1), [70001]),
+                                        ((32, 2), [9000, 1, 20000])])
+def test_attention_of_sequences_in_very_many_parts(heads, lens):
+    """Few heads of long sequences: so many parts that they are joined in two steps. Twice,
+    with the counters back at zero in between."""
+    p = Pool(lens, n_kv=heads[1], page=128, dtype=torch.bfloat16, seed=len(lens) + heads[0])
+    q = randn_bf16((len(lens), heads[0], 128), seed=31, device="cuda")
+    got = attend(p, q, weight=p.weight)
+    check_attention(p, q, "bf16", got=got, weight=p.weight)
+    assert torch.equal(got, attend(p, q))
+
+
 def test_attention_pages_shared_by_two_sequences_collect_both_weights():
     p = Pool([64, 64], n_kv=1, page=32, dtype=torch.bfloat16, seed=12)
     p.table[1, 0] = p.table[0, 0]  # a common prefix

@@ -1125,6 +1125,7 @@ int nf4b_paged_attention(const nf4b_paged_kv* cache, const void* q, const int32_
   p.max_pages = cache->max_pages;
   p.n_pages = cache->n_pages;
   p.counters = reinterpret_cast<int*>(ws);
+  p.group_counters = p.counters + 65536;
   p.part_o = reinterpret_cast<float*>(ws + plan.part_o);
   p.part_ml = reinterpret_cast<float2*>(ws + plan.part_ml);
   p.lse = cache->weight ? reinterpret_cast<float*>(ws + plan.lse) : nullptr;

@@ -399,7 +399,8 @@ constexpr int PAGED_MAX_SEQS = 4096;  // sequences of one call (their tile count
 constexpr int PAGED_MAX_GROUPS = 16;
 constexpr int PAGED_MAX_LISTS = 65535;  // (sequence, KV head) pairs of one call
 // The workspace's counters, at its start whatever the call's sizes: zero between calls of any sizes.
-constexpr size_t PAGED_COUNTER_BYTES = 65536 * sizeof(int);
+constexpr int PAGED_MAX_PARTS = 2048;  // CTAs of one attention call, two group counters each
+constexpr size_t PAGED_COUNTER_BYTES = (65536 + 2 * PAGED_MAX_PARTS) * sizeof(int);
 
 struct PagedAttnParams {
   const uint16_t* q;     // [n_seqs, n_head, 128]
@@ -411,7 +412,8 @@ struct PagedAttnParams {
   uint16_t* out;         // [n_seqs, n_head, 128]
   float scale_log2;      // scale * log2(e)
   int n_seqs, n_head, n_kv, groups, page_size, max_pages, n_pages;
-  int* counters;    // [n_seqs, n_kv], zero between calls
+  int* counters;        // [n_seqs, n_kv], zero between calls
+  int* group_counters;  // [2 grid], zero between calls
   float* part_o;    // [2 grid, groups, 128]
   float2* part_ml;  // [2 grid, groups]
   float* lse;       // [n_seqs, n_head], log2; null without weight

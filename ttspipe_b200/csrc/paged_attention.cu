@@ -45,6 +45,11 @@ constexpr int kTile = PAGED_TILE;
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kJoin = 16;  // parts whose outputs a joining warp requests at once
+// Parts times query heads from which a join is made in two steps: one CTA reads 512 bytes
+// of each at 64 bytes a clock, a second step costs two more round trips. 16 heads on one,
+// 65536 rows in 296 parts: 23 us in two steps, 67 in one; 8 heads to one, 60 parts: 13.9
+// and 14.9; 16 heads, 22 parts: 16.2 and 13.9.
+constexpr int kWide = 448;
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -161,13 +166,21 @@ struct WarpState {
   float m[NT], l[NT];
 };
 
+// A join: the states of `parts` parts of a (sequence, head), from `first` on in steps of
+// `step`, into its outputs, or (to >= 0) into the place of a part.
+struct Join {
+  int first, parts, step;
+  int b, h, to;
+  int c0, c1;  // its first and last part
+};
+
 // The warps' states of one (sequence, head) part, for the join inside the CTA.
 template <int NT>
 struct AttnShared {
   float o[kWarps][NT * 8][kD];
   float m[kWarps][NT * 8], l[kWarps][NT * 8];
-  int4 joins[2];  // (sequence, head)s that this CTA joins: first and last part, sequence, head
-  int n_joins;
+  Join joins[2];  // what this CTA joins
+  int n_joins, wide;
 };
 
 // The finished row of one query head, four dimensions to a lane.
@@ -180,22 +193,25 @@ __device__ __forceinline__ void store_out(const PagedAttnParams& p, size_t head,
   if (lane == 0 && p.lse != nullptr) p.lse[head] = l == 0.f ? -INFINITY : m + log2f(l) - kLift<F16>;
 }
 
+// Where the state of part q of a (sequence, head) whose first part is c0 lies: a CTA
+// shares at most its first and its last (sequence, head).
+__device__ __forceinline__ int slot_of(int q, int c0) { return 2 * q + (q == c0 ? 1 : 0); }
+
 // Up to kJoin parts of one (sequence, query head): their states (maximum, sum), one to a
 // lane, and their outputs, four dimensions to a lane.
 struct JoinPiece {
   float2 ml;
   float4 o[kJoin];
-  size_t head;  // of all sequences' query heads
-  int n;        // parts; 0: nothing
-  bool last;    // the last ones of this head
+  int join, head;
+  int n;      // parts; 0: nothing
+  bool last;  // the last ones of this head
 };
 
-// The states of the parts of up to two (sequence, KV head)s - joins[.] = (first part,
-// last part, sequence, head) - into their outputs. Each warp takes every fourth query
-// head, kJoin parts at a time, and requests the next ones before it adds up these
-// (16 heads of 24 parts: 7 us, 10 when each waited for its own).
+// The joins of a list of up to two. Each warp takes every fourth query head, kJoin parts
+// at a time, and requests the next ones before it adds up these (16 heads of 24 parts:
+// 7 us, 10 when each waited for its own).
 template <bool F16>
-__device__ __forceinline__ void join_parts(const PagedAttnParams& p, const int4* joins, int n_joins) {
+__device__ __forceinline__ void join_parts(const PagedAttnParams& p, const Join* joins, int n_joins) {
   const int lane = threadIdx.x & 31, G = p.groups;
   int i = threadIdx.x >> 5, q0 = 0;  // the next pieces: query head, first part
   JoinPiece x, next;
@@ -205,17 +221,23 @@ __device__ __forceinline__ void join_parts(const PagedAttnParams& p, const int4*
   do {
     next.n = 0;
     if (i < n_joins * G) {
-      const int4 j = joins[i / G];
-      const int head = i % G, first = j.x + q0, n = min(kJoin, j.y - first + 1);
-      auto at = [&](int k) -> size_t { return (size_t)(2 * (first + k) + (first + k == j.x ? 1 : 0)) * G + head; };
+      next.join = i / G;
+      next.head = i % G;
+      const Join j = joins[next.join];
+      const int n = min(kJoin, j.parts - q0), q = j.first + q0 * j.step;
+      const size_t at0 = (size_t)slot_of(q, j.c0) * G + next.head;  // the others are not c0
+      const size_t at = (size_t)(2 * q) * G + next.head, step = (size_t)(2 * j.step) * G;
       next.ml = make_float2(-INFINITY, 0.f);
-      if (lane < n) next.ml = __ldcg(&p.part_ml[at(lane)]);
+      if (lane < n) next.ml = __ldcg(&p.part_ml[lane == 0 ? at0 : at + lane * step]);
+      const float4* from = reinterpret_cast<const float4*>(p.part_o + at * kD) + lane;
+      next.o[0] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at0 * kD) + lane);
 #pragma unroll
-      for (int k = 0; k < kJoin; ++k)
-        if (k < n) next.o[k] = __ldcg(reinterpret_cast<const float4*>(&p.part_o[at(k) * kD + lane * 4]));
-      next.head = (size_t)j.z * p.n_head + (size_t)j.w * G + head;
+      for (int k = 1; k < kJoin; ++k) {
+        from += step * (kD / 4);
+        if (k < n) next.o[k] = __ldcg(from);
+      }
       next.n = n;
-      next.last = first + kJoin > j.y;
+      next.last = q0 + kJoin >= j.parts;
       q0 = next.last ? 0 : q0 + kJoin;
       i += next.last ? kWarps : 0;
     }
@@ -241,7 +263,14 @@ __device__ __forceinline__ void join_parts(const PagedAttnParams& p, const int4*
       if (x.last) {
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
-        store_out<F16>(p, x.head, lane, M == -INFINITY ? 0.f : M, l, o);
+        const Join j = joins[x.join];
+        if (j.to < 0) {
+          store_out<F16>(p, (size_t)j.b * p.n_head + (size_t)j.h * G + x.head, lane, M == -INFINITY ? 0.f : M, l, o);
+        } else {
+          const size_t to = (size_t)j.to * G + x.head;
+          *reinterpret_cast<float4*>(&p.part_o[to * kD + lane * 4]) = make_float4(o[0], o[1], o[2], o[3]);
+          if (lane == 0) p.part_ml[to] = make_float2(M, l);
+        }
         M = -INFINITY;
         l = o[0] = o[1] = o[2] = o[3] = 0.f;
       }
@@ -259,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int G = p.groups;
 
-  if (tid == 0) sm.n_joins = 0;
+  if (tid == 0) sm.n_joins = sm.wide = 0;
   pdl_wait();  // q, the new rows and the lengths come from earlier kernels
   line.fill(p);
   for (int b = blockIdx.x; b < p.n_seqs; b += gridDim.x)
@@ -481,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
     __syncthreads();
     // a warp joins the states of a query head, four dimensions to a lane
     const bool whole = t0 == 0 && t1 == T;
-    const int slot = 2 * c + (t0 == 0 ? 1 : 0);  // a CTA shares at most its first and its last (sequence, head)
+    const int slot = 2 * c + (t0 == 0 ? 1 : 0);
     const size_t head0 = (size_t)b * p.n_head + (size_t)h * G;
     for (int head = warp; head < G; head += kWarps) {
       float M = -INFINITY;
@@ -508,15 +537,21 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
       }
     }
     if (!whole) {
-      // join: the CTAs whose parts hold this (sequence, head), first to last
+      // The CTAs whose parts hold this (sequence, head) are c0 to c1; the last one to come
+      // here joins them. Where that is much (kWide), each kJoin of them are joined first
+      // by the last of these, and the last of those joins the rest.
       const int c0 = cut.of(u - t0), c1 = cut.of(u - t0 + T - 1);
+      const bool wide = (c1 - c0 + 1) * G >= kWide;
+      const int first = wide ? c - (c - c0) % kJoin : c0, last = wide ? min(first + kJoin - 1, c1) : c1;
       __syncthreads();
       if (tid == 0) {
+        int* counter = wide ? p.group_counters + slot_of(first, c0) : p.counters + b * p.n_kv + h;
         __threadfence();
-        if (atomicAdd(&p.counters[b * p.n_kv + h], 1) == c1 - c0) {  // this CTA is the last one and joins
+        if (atomicAdd(counter, 1) == last - first) {
           __threadfence();
-          p.counters[b * p.n_kv + h] = 0;
-          sm.joins[sm.n_joins++] = make_int4(c0, c1, b, h);
+          *counter = 0;
+          sm.joins[sm.n_joins++] = Join{first, last - first + 1, 1, b, h, wide ? slot_of(first, c0) : -1, c0, c1};
+          if (wide) sm.wide = 1;
         }
       }
     }
@@ -525,7 +560,30 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
     advance();
   }
   // joins after the main loop, at most two (so that their registers are not the loop's)
-  join_parts<F16>(p, sm.joins, sm.n_joins);
+#pragma unroll 1
+  for (bool again = true; again;) {
+    again = sm.wide != 0;
+    join_parts<F16>(p, sm.joins, sm.n_joins);
+    if (!again) break;
+    __syncthreads();
+    if (tid == 0) {  // joins of kJoin parts are parts themselves: the last of them joins these
+      sm.wide = 0;
+      int n = 0;
+      for (int i = 0; i < sm.n_joins; ++i) {
+        Join j = sm.joins[i];
+        if (j.to < 0) continue;  // done
+        const int groups = (j.c1 - j.c0) / kJoin + 1;
+        __threadfence();
+        int* counter = p.counters + j.b * p.n_kv + j.h;
+        if (atomicAdd(counter, 1) != groups - 1) continue;
+        __threadfence();
+        *counter = 0;
+        sm.joins[n++] = Join{j.c0, groups, kJoin, j.b, j.h, -1, j.c0, j.c1};
+      }
+      sm.n_joins = n;
+    }
+    __syncthreads();
+  }
   pdl_launch_dependents();
 }
 
@@ -612,7 +670,8 @@ long long most_work(int n_seqs, int n_kv, long long max_rows) {
 int grid_for(long long tiles, long long lists, int groups, int sms) {
   const int least = paged_min_tiles(groups);
   const long long by_tiles = (tiles + least - 1) / least, n = by_tiles > lists ? by_tiles : lists;
-  const long long most = (long long)sms * (groups <= 8 ? 3 : 2);
+  const long long resident = (long long)sms * (groups <= 8 ? 3 : 2);
+  const long long most = resident < PAGED_MAX_PARTS ? resident : PAGED_MAX_PARTS;
   return (int)(n < most ? n : most);
 }
 
