@@ -435,11 +435,21 @@ def test_evict_ties_signs_nan_and_infinities():
         check_evict(p, w, pos, budget, 0, 0, False)
 
 
-def test_evict_of_a_long_cache():
-    n = 70001
+@pytest.mark.parametrize("n", [6001, 20000, 70001, 140000])
+def test_evict_of_a_long_cache(n):
+    """One CTA, clusters of several, and more rows than a cluster holds at once."""
     p = Pool([n], n_kv=1, page=16, dtype=torch.bfloat16, seed=82)
     rng = np.random.default_rng(83)
-    check_evict(p, [[rng.random(n).astype(np.float32).round(3)]], [[np.arange(n)]], 30001, 1000, 16, True)
+    check_evict(p, [[rng.random(n).astype(np.float32).round(3)]], [[np.arange(n)]], n // 2 - 1, 1000, 16, True)
+
+
+def test_evict_of_many_lists():
+    """More lists than SMs, of a capacity that takes 512 threads each."""
+    lens = [(977 * i) % 5000 for i in range(80)]
+    p = Pool(lens, n_kv=2, page=64, dtype=torch.bfloat16, seed=86, width=96)
+    rng = np.random.default_rng(87)
+    w = [[rng.random(n).astype(np.float32).round(2) for _ in range(2)] for n in lens]
+    check_evict(p, w, [[rng.permutation(n) for _ in range(2)] for n in lens], 1200, 100, 4, False)
 
 
 def test_evict_then_attention_is_attention_over_the_kept_rows():

@@ -287,7 +287,7 @@ __device__ __forceinline__ int* cluster_peer(int* p, unsigned rank) {  // the sa
 template <int kThreads, int kDeep, bool kOnce>
 __global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : 1024 / kThreads)
     paged_select_kernel(const __grid_constant__ PagedEvictParams p, int size) {
-  __shared__ alignas(16) int hists[3][kBins];  // of each step: other CTAs of the cluster may still read the last one's
+  __shared__ alignas(16) int hists[3][kBins];  // of each step; the first CTA's become the cluster's
   __shared__ int part[3][32];
   __shared__ uint32_t s_prefix;
   __shared__ int s_need, s_among, s_newest, s_sum[3];
@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : 1024 / kThrea
     load(q, true);
     copy(r0 + lane * 4);
   }
-  __syncthreads();
+  sync();
 
   if (!all && p.recent > 0) {
     int newest = INT_MIN;
@@ -434,7 +434,17 @@ __global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : 1024 / kThrea
   }
   add_shared(&hists[0][kZero >> 21], zeros, lane);
   add_shared(&hists[0][kBins - 1], guarded, lane);
-  sync();
+  // the cluster's counts into the first CTA's histogram; few digits occur, so few have to go
+  auto merge = [&](int* hist) {
+    if (size > 1) {
+      __syncthreads();
+      if (rank > 0)
+        for (int j = tid; j < kBins; j += kThreads)
+          if (const int n = hist[j]) atomicAdd(cluster_peer(hist, 0) + j, n);
+    }
+    sync();
+  };
+  merge(hists[0]);
 
   // of one value a warp: the sum up to the warp before this one's, and of all
   auto warps_before = [&](const int* v, int* sum) -> int {
@@ -471,16 +481,16 @@ __global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : 1024 / kThrea
       });
       __syncwarp();
       add_shared(&hist[0], lowest, lane);
-      sync();
+      merge(hist);
     }
     // falling digits, kMine to a thread
     int n[kMine], sum = 0, all_of;
+    const int* merged = (size > 1 ? cluster_peer(hist, 0) : hist) + kBins - kMine * (tid + 1);
 #pragma unroll
-    for (int j = 0; j < kMine; ++j) n[j] = hist[kBins - 1 - kMine * tid - j];
-    for (int r = 1; r < size; ++r) {
-      const int* other = cluster_peer(hist, (rank + r) % size);
-#pragma unroll
-      for (int j = 0; j < kMine; ++j) n[j] += other[kBins - 1 - kMine * tid - j];
+    for (int j = 0; j < kMine; j += 2) {
+      const int2 two = *reinterpret_cast<const int2*>(merged + j);
+      n[kMine - 1 - j] = two.x;
+      n[kMine - 2 - j] = two.y;
     }
 #pragma unroll
     for (int j = 0; j < kMine; ++j) sum += n[j];
@@ -731,20 +741,30 @@ void paged_evict_plan(int n_seqs, int n_kv, long long max_rows, int budget, Page
 
 cudaError_t launch_paged_evict(const PagedEvictParams& p, int sms, cudaStream_t stream) {
   const int lists = p.n_seqs * p.n_kv, cap = p.max_pages * p.page_size;
-  // 256 or 512 threads hold the keys of 8 rows each; longer lists get 1024 with 16 rows each
-  // (8 x 32768 rows: 135 us, 149 with 8), in clusters of up to 8 CTAs (131072 rows), and still
-  // longer ones those 8 and several reads
-  int cluster = 1;
-  while (cluster < 8 && cap > cluster * 16384) cluster *= 2;
+  // Lists of up to 4096 rows: 8 rows to each of 256 or 512 threads (1 x 4096: 10.3 us, 12.7 with 16
+  // rows). Longer ones: 1024 threads with 8 rows, in clusters of up to 8 CTAs, while every list's cluster
+  // has SMs of its own (1 x 32768: 29 us, 34 with 16 rows); else 16 rows (8 x 32768: 134 us, 145
+  // with 8), up to 8192 of them to 512 threads (32 x 8192: 127 us, 139 with 1024). Past 131072
+  // rows a cluster of 8 reads its list several times.
+  auto cluster_for = [&](int rows) {
+    int c = 1;
+    while (c < 8 && cap > c * rows) c *= 2;
+    return c;
+  };
+  const int c8 = cluster_for(8192), c16 = cluster_for(16384);
   cudaError_t e;
   if (cap <= 2048)
     e = launch(paged_select_kernel<256, 2, true>, lists, 256, 0, 1, stream, p, 1);
   else if (cap <= 4096)
     e = launch(paged_select_kernel<512, 2, true>, lists, 512, 0, 1, stream, p, 1);
-  else if (cap <= cluster * 16384)
-    e = launch(paged_select_kernel<1024, 4, true>, lists * cluster, 1024, 0, cluster, stream, p, cluster);
+  else if (cap <= c8 * 8192 && lists * c8 <= sms)
+    e = launch(paged_select_kernel<1024, 2, true>, lists * c8, 1024, 0, c8, stream, p, c8);
+  else if (cap <= 8192)
+    e = launch(paged_select_kernel<512, 4, true>, lists, 512, 0, 1, stream, p, 1);
+  else if (cap <= c16 * 16384)
+    e = launch(paged_select_kernel<1024, 4, true>, lists * c16, 1024, 0, c16, stream, p, c16);
   else
-    e = launch(paged_select_kernel<1024, 4, false>, lists * cluster, 1024, 0, cluster, stream, p, cluster);
+    e = launch(paged_select_kernel<1024, 4, false>, lists * c16, 1024, 0, c16, stream, p, c16);
   if (e != cudaSuccess) return e;
   const long long want = (long long)lists * ((p.max_moves + kMovePiece - 1) / kMovePiece), most = 4LL * sms;  // all resident
   return launch(paged_move_kernel, (int)(want < 1 ? 1 : want < most ? want : most), kMoveWarps * 32, 0, 1,
