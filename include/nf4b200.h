@@ -523,7 +523,7 @@ int nf4b_paged_write(const nf4b_paged_kv* cache, const void* qkv, const int32_t*
  * With cache->weight every visible row's weight (the sum over the query heads
  * of its KV head) is added to it, in fp32; a page that several sequences share
  * receives all of theirs, in no fixed order. Otherwise results do not depend on
- * timing. `workspace` (nf4b_paged_attention_workspace_size, tracked = whether
+ * timing. out must not overlap an input. `workspace` (nf4b_paged_attention_workspace_size, tracked = whether
  * weight is given) is zeroed once before its first use and serves calls of any
  * sizes that fit it; calls that overlap on the GPU must not share one.
  */

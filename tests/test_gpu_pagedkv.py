@@ -190,10 +190,11 @@ def test_attention_lengths_and_tables_out_of_range():
     check_attention(p, q, "bf16", got=attend(p, q))
 
 
-def test_attention_many_short_sequences():
-    lens = [(37 * i) % 70 for i in range(400)]
+@pytest.mark.parametrize("n", [400, 4096])
+def test_attention_many_short_sequences(n):
+    lens = [(37 * i) % 70 for i in range(n)]
     p = Pool(lens, n_kv=2, page=16, dtype=torch.bfloat16, seed=6)
-    q = randn_bf16((400, 8, 128), seed=6, device="cuda")
+    q = randn_bf16((n, 8, 128), seed=6, device="cuda")
     check_attention(p, q, "bf16", got=attend(p, q, weight=p.weight), weight=p.weight)
 
 
