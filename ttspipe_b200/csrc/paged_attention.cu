@@ -13,14 +13,14 @@
 // product), products and sums in fp32.
 //
 // What bounds it. A row of a KV head is 512 bytes and 4 * 128 * groups operations, so
-// memory does: 64 sequences of 8192 rows (32 query and 8 KV heads, 2.1 GB) take 315 us,
+// memory does: 64 sequences of 8192 rows (32 query and 8 KV heads, 2.1 GB) take 317 us,
 // 6.8 TB/s, the rate of a plain copy on the same GPU, with the tensor pipe 15-18% busy.
 // Keys and values go from global memory straight into MMA fragments: a lane reads the
 // 16-byte pieces of a row that are its fragment once q's dimensions and v's are taken in
 // that order (a sum does not mind), so there is no staging, no bank conflict and nothing to wait
 // for but the loads; 3 CTAs of 4 warps an SM, each warp a tile of keys and values ahead, keep
-// up to 96 KB of them requested. Few rows are latency: 1 x 19 rows 3.7 us, 1 x 2048 rows
-// 7.9 us (about 1.0 to find the part, 2.3 for its two tiles a warp, 0.4 to join the warps, 1.1
+// up to 96 KB of them requested. Few rows are latency: 1 x 19 rows 3.9 us, 1 x 2048 rows
+// 8.0 us (about 1.0 to find the part, 2.3 for its two tiles a warp, 0.4 to join the warps, 1.1
 // for the counter, 2.3 to join the parts).
 //
 // Work split. The unit of work is a tile of 16 rows of one (sequence, KV head): page

@@ -216,10 +216,10 @@ __global__ void __launch_bounds__(kWriteWarps * 32, kPairs == 4 ? 7 : 1) paged_w
 //
 // paged_select_kernel, one CTA or one cluster of CTAs a list, finds the smallest kept key digit by digit
 // from the top (11, 11 and 10 bits, a histogram each) and lists the moves;
-// paged_move_kernel makes them. 8 x 32768 rows halved (64 lists, 562 MB) take 135 us:
+// paged_move_kernel makes them. 8 x 32768 rows halved (64 lists, 562 MB) take 134 us:
 // about 30 to select, a chain of dependent steps (read, newest, three histograms, two
 // counts), and 104 to move some 524,000 rows, 256 bytes of key and of value each between
-// scattered places, at 5.2 TB/s of DRAM. 1 x 2048 rows are the chain alone, 11 us.
+// scattered places, at 5.2 TB/s of DRAM. 1 x 2048 rows are the chain alone, 9 us.
 constexpr int kBins = 2048;
 
 // Weights in rising order as unsigned integers; 0xFFFFFFFF (no weight maps there,
