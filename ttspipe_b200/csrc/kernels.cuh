@@ -389,9 +389,9 @@ cudaError_t launch_qkv_attention(const QkvIn& in, const int64_t* pos, uint16_t* 
 // ---- paged KV cache (paged_attention.cu, paged_kv.cu) ------------------------
 
 constexpr int PAGED_TILE = 16;        // rows of one unit of attention work; page sizes are multiples of it
-// Units of one CTA's part, where there are that many: a wider join wants fewer parts. 1 x 512 rows
-// of groups of 4: 7.3 us with 8, 8.2 with 12; 5 x 3001 of groups of 16: 14.4 and 13.2.
-constexpr int paged_min_tiles(int groups) { return groups <= 8 ? 8 : 12; }
+// Units of one CTA's part, where there are that many (1 x 512 rows: 7.3 us, 8.2 with 12, 10.5
+// with 16).
+constexpr int PAGED_MIN_TILES = 8;
 // Units that a (sequence, head) costs besides its tiles (32 ragged sequences of up to 4096
 // rows: 56 us with 0, 47 with 4, 42 with 8, 44 with 24).
 constexpr int PAGED_SEQ_TILES = 8;

@@ -20,7 +20,7 @@
 // that order (a sum does not mind), so there is no staging, no bank conflict and nothing to wait
 // for but the loads; 3 CTAs of 4 warps an SM, each warp a tile of keys and values ahead, keep
 // up to 96 KB of them requested. Few rows are latency: 1 x 19 rows 3.9 us, 1 x 2048 rows
-// 8.0 us (about 1.0 to find the part, 2.3 for its two tiles a warp, 0.4 to join the warps, 1.1
+// 7.4 us (about 1.0 to find the part, 1.7 for a tile a warp, 0.4 to join the warps, 1.1
 // for the counter, 2.3 to join the parts).
 //
 // Work split. The unit of work is a tile of 16 rows of one (sequence, KV head): page
@@ -42,14 +42,12 @@ namespace {
 
 constexpr int kD = 128;
 constexpr int kTile = PAGED_TILE;
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
 constexpr int kJoin = 16;  // parts whose outputs a joining warp requests at once
 // Parts times query heads from which a join is made in two steps: one CTA reads 512 bytes
 // of each at 64 bytes a clock, a second step costs two more round trips. 16 heads on one,
-// 65536 rows in 296 parts: 23 us in two steps, 67 in one; 8 heads to one, 60 parts: 13.9
-// and 14.9; 16 heads, 22 parts: 16.2 and 13.9.
-constexpr int kWide = 448;
+// 65536 rows in 148 parts: 17.4 us in two steps, 28 in one; 8 heads to one, 111 parts: 31.3
+// and 37; 16 heads, 33 parts: 13.4 and 11.9.
+constexpr int kWide = 700;
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -126,10 +124,10 @@ struct Line {
 
 constexpr size_t line_bytes(int n_seqs) { return (size_t)(2 * n_seqs + 1) * sizeof(int); }
 
-// The number of parts: as many as CTAs, but paged_min_tiles units of work in each unless
+// The number of parts: as many as CTAs, but PAGED_MIN_TILES units of work in each unless
 // that puts several (sequence, head)s into one part while CTAs are left.
 __device__ __forceinline__ int parts(const PagedAttnParams& p, int work, int ctas) {
-  const int least = paged_min_tiles(p.groups), by_work = (work + least - 1) / least;
+  const int by_work = (work + PAGED_MIN_TILES - 1) / PAGED_MIN_TILES;
   return min(ctas, max(by_work, min(p.n_seqs * p.n_kv, work)));
 }
 
@@ -175,7 +173,7 @@ struct Join {
 };
 
 // The warps' states of one (sequence, head) part, for the join inside the CTA.
-template <int NT>
+template <int NT, int kWarps>
 struct AttnShared {
   float o[kWarps][NT * 8][kD];
   float m[kWarps][NT * 8], l[kWarps][NT * 8];
@@ -207,10 +205,10 @@ struct JoinPiece {
   bool last;  // the last ones of this head
 };
 
-// The joins of a list of up to two. Each warp takes every fourth query head, kJoin parts
+// The joins of a list of up to two. Each warp takes every kWarps-th query head, kJoin parts
 // at a time, and requests the next ones before it adds up these (16 heads of 24 parts:
 // 7 us, 10 when each waited for its own).
-template <bool F16>
+template <int kWarps, bool F16>
 __device__ __forceinline__ void join_parts(const PagedAttnParams& p, const Join* joins, int n_joins) {
   const int lane = threadIdx.x & 31, G = p.groups;
   int i = threadIdx.x >> 5, q0 = 0;  // the next pieces: query head, first part
@@ -279,12 +277,14 @@ __device__ __forceinline__ void join_parts(const PagedAttnParams& p, const Join*
   } while (x.n);
 }
 
-template <int NT, bool F16>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
+template <int NT, int kWarps, bool F16>
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 && kWarps == 4 ? 3 : 1)
     paged_attention_kernel(const __grid_constant__ PagedAttnParams p) {
   extern __shared__ __align__(16) uint8_t smem[];
-  AttnShared<NT>& sm = *reinterpret_cast<AttnShared<NT>*>(smem);
-  Line line(smem + sizeof(AttnShared<NT>), p.n_seqs);
+  constexpr int kThreads = kWarps * 32;
+  using Shared = AttnShared<NT, kWarps>;
+  Shared& sm = *reinterpret_cast<Shared*>(smem);
+  Line line(smem + sizeof(Shared), p.n_seqs);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const int G = p.groups;
 
@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
   if (c >= N) return;
   const Parts cut(U, N);
   // Where this part and (odd lanes) the next one begin: sequence b, head h, tile t0 of it.
-  // A (sequence, head) of up to paged_min_tiles tiles is not split (joining it would cost
+  // A (sequence, head) of up to PAGED_MIN_TILES tiles is not split (joining it would cost
   // more): a cut in it moves to its first tile.
   int u = min(cut.first(c + (lane & 1)), U - 1);
   int b = line.seq_of(p.n_seqs, __shfl_sync(0xffffffffu, u, 0));
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
   if (lane & 1) b = b1;
   const int from = u - line.pre[b];
   int h = from / line.each[b], t0 = from - h * line.each[b];
-  if (line.each[b] <= paged_min_tiles(NT == 1 ? 8 : 16) + PAGED_SEQ_TILES) {
+  if (line.each[b] <= PAGED_MIN_TILES + PAGED_SEQ_TILES) {
     u -= t0;
     t0 = 0;
   }
@@ -563,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2)
 #pragma unroll 1
   for (bool again = true; again;) {
     again = sm.wide != 0;
-    join_parts<F16>(p, sm.joins, sm.n_joins);
+    join_parts<kWarps, F16>(p, sm.joins, sm.n_joins);
     if (!again) break;
     __syncthreads();
     if (tid == 0) {  // joins of kJoin parts are parts themselves: the last of them joins these
@@ -647,30 +647,36 @@ cudaError_t launch(K kernel, int grid, int threads, size_t smem, const PagedAttn
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
-template <int NT, bool F16>
+template <int NT, int kWarps, bool F16>
 cudaError_t launch_attention(const PagedAttnParams& p, int grid, cudaStream_t stream) {
-  const size_t smem = sizeof(AttnShared<NT>) + line_bytes(p.n_seqs);
+  constexpr size_t shared = sizeof(AttnShared<NT, kWarps>);
+  auto kernel = paged_attention_kernel<NT, kWarps, F16>;
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
   if (!configured[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(paged_attention_kernel<NT, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)(sizeof(AttnShared<NT>) + line_bytes(PAGED_MAX_SEQS)));
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)(shared + line_bytes(PAGED_MAX_SEQS)));
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
-  return launch(paged_attention_kernel<NT, F16>, grid, kThreads, smem, p, stream);
+  return launch(kernel, grid, kWarps * 32, shared + line_bytes(p.n_seqs), p, stream);
 }
 
 long long most_work(int n_seqs, int n_kv, long long max_rows) {
   return (long long)n_seqs * n_kv * ((max_rows + kTile - 1) / kTile + PAGED_SEQ_TILES);
 }
 
-int grid_for(long long tiles, long long lists, int groups, int sms) {
-  const int least = paged_min_tiles(groups);
-  const long long by_tiles = (tiles + least - 1) / least, n = by_tiles > lists ? by_tiles : lists;
-  const long long resident = (long long)sms * (groups <= 8 ? 3 : 2);
+// Warps of a CTA: 8 where a join has many heads to share out (16 heads on one, 65536 rows:
+// 17.4 us, 23 with 4) or where the whole cache is so small that a tile a warp is enough (1 x 2048
+// rows: 7.5 us, 8.1 with 4); else 4, three CTAs on an SM.
+int warps_for(long long work, int groups, int sms) { return groups > 8 || work <= 16LL * sms ? 8 : 4; }
+
+// CTAs of a launch, all resident.
+int grid_for(long long work, long long lists, int groups, int sms) {
+  const long long by_work = (work + PAGED_MIN_TILES - 1) / PAGED_MIN_TILES, n = by_work > lists ? by_work : lists;
+  const long long resident = (long long)sms * (warps_for(work, groups, sms) == 4 ? 3 : 1);
   const long long most = resident < PAGED_MAX_PARTS ? resident : PAGED_MAX_PARTS;
   return (int)(n < most ? n : most);
 }
@@ -681,9 +687,9 @@ size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 void paged_attention_plan(int n_seqs, int n_head, int n_kv, long long max_rows, bool tracked, int sms,
                           PagedAttnPlan* plan) {
-  const long long tiles = most_work(n_seqs, n_kv, max_rows);
+  const long long work = most_work(n_seqs, n_kv, max_rows);
   const int groups = n_head / n_kv;
-  plan->grid = grid_for(tiles, (long long)n_seqs * n_kv, groups, sms);
+  plan->grid = grid_for(work, (long long)n_seqs * n_kv, groups, sms);
   size_t at = PAGED_COUNTER_BYTES;
   plan->part_o = at;
   at += up256((size_t)2 * plan->grid * groups * kD * sizeof(float));
@@ -693,20 +699,22 @@ void paged_attention_plan(int n_seqs, int n_head, int n_kv, long long max_rows, 
   if (tracked) {
     at += up256((size_t)n_seqs * n_head * sizeof(float));
     plan->scores = at;
-    at += up256((size_t)tiles * kTile * groups * sizeof(float));
+    at += up256((size_t)work * kTile * groups * sizeof(float));
   }
   plan->bytes = at;
 }
 
 cudaError_t launch_paged_attention(const PagedAttnParams& p, int grid, int sms, bool f16, cudaStream_t stream) {
+  const long long work = most_work(p.n_seqs, p.n_kv, (long long)p.max_pages * p.page_size);
   cudaError_t e;
-  if (p.groups <= 8)
-    e = f16 ? launch_attention<1, true>(p, grid, stream) : launch_attention<1, false>(p, grid, stream);
+  if (p.groups > 8)
+    e = f16 ? launch_attention<2, 8, true>(p, grid, stream) : launch_attention<2, 8, false>(p, grid, stream);
+  else if (warps_for(work, p.groups, sms) == 8)
+    e = f16 ? launch_attention<1, 8, true>(p, grid, stream) : launch_attention<1, 8, false>(p, grid, stream);
   else
-    e = f16 ? launch_attention<2, true>(p, grid, stream) : launch_attention<2, false>(p, grid, stream);
+    e = f16 ? launch_attention<1, 4, true>(p, grid, stream) : launch_attention<1, 4, false>(p, grid, stream);
   if (e != cudaSuccess || p.weight == nullptr) return e;
-  const long long tiles = most_work(p.n_seqs, p.n_kv, (long long)p.max_pages * p.page_size);
-  const long long n = (tiles + kWTiles - 1) / kWTiles;
+  const long long n = (work + kWTiles - 1) / kWTiles;
   return launch(paged_weight_kernel, (int)(n < 8LL * sms ? n : 8LL * sms), kWThreads,
                 line_bytes(p.n_seqs), p, stream);
 }
