@@ -36,8 +36,8 @@ class Alone:
     def error(self, x, y):
         """How far y is from the block of the next token x: max|err| / max|ref|."""
         c = self.cfg
-        want = orc.decode_block(to_bits(x).reshape(-1), self.w, self.k, self.v, self.pos, self.freqs[self.pos], c.n_head,
-                                c.n_local_heads, c.head_dim, c.norm_eps, c.norm_eps)
+        want = orc.decode_block(to_bits(x).reshape(-1), self.w, self.k, self.v, self.pos, self.freqs[self.pos],
+                                c.n_head, c.n_local_heads, c.head_dim, c.norm_eps, c.norm_eps)
         self.pos += 1
         return orc.relative_error(orc.bf16_to_f32(to_bits(y)).ravel(), orc.bf16_to_f32(want).ravel())
 

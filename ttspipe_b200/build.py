@@ -74,7 +74,7 @@ def build_binding(force: bool = False, verbose: bool = False) -> Path:
     tmp = BIND.with_suffix(".so.tmp")
     cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{i}" for i in inc), str(BIND_SRC),
-           f"-L{home / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-o", str(tmp)]
+           f"-L{home / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-o", str(tmp)]
     if verbose:
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True, env=dict(os.environ, TMPDIR=str(BUILD)))

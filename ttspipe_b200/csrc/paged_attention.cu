@@ -186,7 +186,8 @@ template <bool F16>
 __device__ __forceinline__ void store_out(const PagedAttnParams& p, size_t head, int lane, float m, float l,
                                           const float (&o)[4]) {
   const float r = l == 0.f ? 0.f : 1.f / l;
-  const uint2 w = l == 0.f ? make_uint2(0, 0) : make_uint2(pack_act2<F16>(o[0] * r, o[1] * r), pack_act2<F16>(o[2] * r, o[3] * r));
+  uint2 w = make_uint2(0, 0);
+  if (l != 0.f) w = make_uint2(pack_act2<F16>(o[0] * r, o[1] * r), pack_act2<F16>(o[2] * r, o[3] * r));
   *reinterpret_cast<uint2*>(p.out + head * kD + lane * 4) = w;
   if (lane == 0 && p.lse != nullptr) p.lse[head] = l == 0.f ? -INFINITY : m + log2f(l) - kLift<F16>;
 }

@@ -58,7 +58,8 @@ __device__ __forceinline__ float rsqrt_128(double ss, float eps) {
 }
 
 template <int kPairs, int kGroups, bool F16>
-__global__ void __launch_bounds__(kWriteWarps * 32, kPairs == 4 ? 7 : 1) paged_write_kernel(const __grid_constant__ PagedWriteParams p) {
+__global__ void __launch_bounds__(kWriteWarps * 32, kPairs == 4 ? 7 : 1)
+    paged_write_kernel(const __grid_constant__ PagedWriteParams p) {
   pdl_wait();
   const int lane = threadIdx.x & 31, half = lane >> 4, piece = lane & 15;
   const int heads = p.n_head + 2 * p.n_kv;
@@ -211,11 +212,11 @@ __global__ void __launch_bounds__(kWriteWarps * 32, kPairs == 4 ? 7 : 1) paged_w
 // order stay: rows whose position is below `sink` or among the `recent` newest
 // first, then by falling weight (NaN as -inf), equal ones by rising row. Rows at or
 // past `left` that stay move, in order, into the rows below it that do not: there are
-// equally many, the two sets are disjoint, and attention does not depend on the order of rows
-// (the rotary is in the keys), so nothing else has to move.
+// equally many, the two sets are disjoint, and attention does not depend on the order
+// of rows (the rotary is in the keys), so nothing else has to move.
 //
-// paged_select_kernel, one CTA or one cluster of CTAs a list, finds the smallest kept key digit by digit
-// from the top (11, 11 and 10 bits, a histogram each) and lists the moves;
+// paged_select_kernel, one CTA or one cluster of CTAs a list, finds the smallest kept key
+// digit by digit from the top (11, 11 and 10 bits, a histogram each) and lists the moves;
 // paged_move_kernel makes them. 8 x 32768 rows halved (64 lists, 562 MB) take 134 us:
 // about 30 to select, a chain of dependent steps (read, newest, three histograms, two
 // counts), and 104 to move some 524,000 rows, 256 bytes of key and of value each between
@@ -379,7 +380,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : 1024 / kThrea
     sync();
   }
   int newest = s_newest;
-  for (int r = 1; r < size && !all && p.recent > 0; ++r) newest = max(newest, *cluster_peer(&s_newest, (rank + r) % size));
+  if (!all && p.recent > 0)
+    for (int r = 1; r < size; ++r) newest = max(newest, *cluster_peer(&s_newest, (rank + r) % size));
   // positions above this are among the newest (no position is above INT_MAX)
   const int guard = p.recent == 0 ? INT_MAX : newest < INT_MIN + p.recent ? INT_MIN : newest - p.recent;
   auto to_keys = [&]() {
@@ -614,7 +616,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : 1024 / kThrea
     }
 #pragma unroll
     for (int u = 0; u < kDeep; ++u) {
-      const int mine = upto[u] - (__popc(hole[u]) + (__popc(out[u]) << 16)), sum = __shfl_sync(0xffffffffu, upto[u], 31);
+      const int mine = upto[u] - (__popc(hole[u]) + (__popc(out[u]) << 16));
+      const int sum = __shfl_sync(0xffffffffu, upto[u], 31);
       int hole_to = hole_at + (mine & 0xFFFF), out_to = out_at + (mine >> 16);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -766,7 +769,8 @@ cudaError_t launch_paged_evict(const PagedEvictParams& p, int sms, cudaStream_t 
   else
     e = launch(paged_select_kernel<1024, 4, false>, lists * c16, 1024, 0, c16, stream, p, c16);
   if (e != cudaSuccess) return e;
-  const long long want = (long long)lists * ((p.max_moves + kMovePiece - 1) / kMovePiece), most = 4LL * sms;  // all resident
+  const long long want = (long long)lists * ((p.max_moves + kMovePiece - 1) / kMovePiece);
+  const long long most = 4LL * sms;  // all resident
   return launch(paged_move_kernel, (int)(want < 1 ? 1 : want < most ? want : most), kMoveWarps * 32, 0, 1,
                 stream, p);
 }

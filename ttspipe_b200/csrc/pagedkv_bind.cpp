@@ -1,11 +1,10 @@
 // Python binding of the paged KV cache's entry points: the checks of the tensors and
-// the call, 2 us instead of the 9 us that the same steps take in Python. A decode step
-// makes these calls once a layer. The kernels stay behind the C ABI; this module is
+// the call, 4 us with the output's allocation where Python and ctypes take 10. A decode
+// step makes these calls once a layer. The kernels stay behind the C ABI; this module is
 // handed the addresses of its functions.
 
 #include <ATen/core/Tensor.h>
-#include <ATen/ops/empty.h>
-#include <ATen/ops/empty_like.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -125,6 +124,11 @@ void* address(PyObject* o) {
   return o == Py_None ? nullptr : reinterpret_cast<void*>(static_cast<uintptr_t>(PyLong_AsUnsignedLongLong(o)));
 }
 
+// A new tensor on the GPU (the allocator asked directly: 0.6 us less than by at::empty).
+at::Tensor fresh(at::IntArrayRef shape, at::ScalarType type, at::Device device) {
+  return at::Tensor(at::detail::empty_cuda(shape, type, device, std::nullopt));
+}
+
 // The output tensor where the call succeeded, else the library's status.
 PyObject* answer(int status, const at::Tensor& out, PyObject* given) {
   if (status != NF4B_OK) return PyLong_FromLong(status);
@@ -160,7 +164,7 @@ PyObject* write(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   void* f = take("freqs", freqs, ft, {freqs.size(0), kD / 2, 2}, d);
   void* qw = take_or_null("q_norm", a[9], cache.type, {kD}, d);
   void* kw = take_or_null("k_norm", a[10], cache.type, {kD}, d);
-  const at::Tensor out = a[14] == Py_None ? at::empty({n, n_head, kD}, qkv.options()) : tensor("out", a[14]);
+  const at::Tensor out = a[14] == Py_None ? fresh({n, n_head, kD}, cache.type, d) : tensor("out", a[14]);
   void* o = take("out", out, cache.type, {n, n_head, kD}, d);
   const int status =
       g_write(&cache.c, x, static_cast<int32_t*>(seqs), static_cast<int32_t*>(rows), static_cast<int32_t*>(positions),
@@ -188,7 +192,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     mask = take("mask", m, m.scalar_type() == at::kBool ? at::kBool : at::kByte,
                 {n, (int64_t)cache.c.max_pages * cache.c.page_size}, d);
   }
-  const at::Tensor out = a[8] == Py_None ? at::empty_like(q) : tensor("out", a[8]);
+  const at::Tensor out = a[8] == Py_None ? fresh(q.sizes(), cache.type, d) : tensor("out", a[8]);
   void* o = take("out", out, cache.type, q.sizes(), d);
   const int status = g_attention(&cache.c, x, static_cast<int32_t*>(lens), static_cast<uint8_t*>(mask),
                                  (float)number(a[6]), o, (int)q.size(1), address(a[9]), (size_t)integer(a[10]),
