@@ -55,13 +55,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// A store whose line L2 gives up last: the scores of a whole call are read again only
-// after all keys and values have passed through L2 (64 x 8192 rows: the call takes 359 us,
-// 366 with plain stores).
-__device__ __forceinline__ void st_keep(float* p, float x, float y, uint64_t policy) {
-  asm volatile("st.global.L2::cache_hint.v2.f32 [%0], {%1, %2}, %3;" ::"l"(p), "f"(x), "f"(y), "l"(policy) : "memory");
-}
-
 // Tiles of a sequence: its length is brought into [0, capacity].
 __device__ __forceinline__ int seq_rows(const PagedAttnParams& p, int b) {
   const int n = p.lens[b];
@@ -319,8 +312,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 && kWarps == 4 ? 3 : 1)
   h = __shfl_sync(0xffffffffu, h, 0);
   t0 = __shfl_sync(0xffffffffu, t0, 0);
   const int tpp = p.page_size / kTile;
-  uint64_t keep;
-  asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(keep));
 
   auto advance = [&]() {  // to the next (sequence, head) with rows
     if (++h < p.n_kv) return;
@@ -430,8 +421,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 && kWarps == 4 ? 3 : 1)
         for (int r = 0; r < 4; ++r) x[r] = see[r] ? sc[r >> 1][nt * 2 + (r & 1)] * p.scale_log2 : -INFINITY;
         if (scores != nullptr && nt * 8 + g < G) {
           float* sp = scores + ((size_t)tile * G + nt * 8 + g) * kTile + 2 * t;
-          st_keep(sp, x[0], x[1], keep);
-          st_keep(sp + 8, x[2], x[3], keep);
+          *reinterpret_cast<float2*>(sp) = make_float2(x[0], x[1]);
+          *reinterpret_cast<float2*>(sp + 8) = make_float2(x[2], x[3]);
         }
         float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
