@@ -17,8 +17,8 @@ Pools are [n_pages, n_kv, page_size, 128] bf16 or fp16; ``weight`` (fp32) and
 ``position`` (int32) are [n_pages, n_kv, page_size]; ``block_table`` is int32
 [n_seqs, max_pages] (-1: not assigned); lengths, rows and positions are int32. All
 of them stay on the device and are read there, so a CUDA graph of a step serves
-every state of the cache. ``PagedKVCache`` holds one layer's pools and hands out
-pages; ``decode_block`` is a transformer block's decode step for a batch of streams.
+every state of the cache. ``PagedKVCache`` holds the pools of all layers and hands
+out pages; ``decode_block`` is a transformer block's decode step for a batch of streams.
 
 A tensor of a wrong type, shape, layout or device is refused with ValueError,
 what the library refuses (head groups over 16, page sizes that are not a multiple of 16,
@@ -252,7 +252,8 @@ class PagedKVCache:
         self.lens.copy_(self._left)
 
     def evict_and_trim(self, budget: int, *, recent: int = 0, sink: int = 0) -> None:
-        """``evict``, and the pages that it leaves free are taken back (on the host, from its own count of rows)."""
+        """``evict``, and the pages that it leaves free are taken back (on the host, from its own count of
+        rows): after ``end_step``, before rows are reserved for the next step."""
         self.evict(budget, recent=recent, sink=sink)
         for seq in range(self.n_seqs):
             self.trim(seq, budget)
