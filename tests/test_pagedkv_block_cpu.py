@@ -1,0 +1,126 @@
+"""The transformer block over a paged cache, its launches replaced by the products and copies that they
+are documented to be (runs without a GPU): what the block makes of its linears and of the cache."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from ttspipe_b200 import fastpath, fusedops, model, nf4gemv, pagedkv
+
+DIM, HEADS, KV = 64, 2, 1
+CFG = model.ModelArgs(dim=DIM, n_head=HEADS, n_local_heads=KV, intermediate_size=96, max_seq_len=64)
+
+
+def _matmul(module, x, *, epi=nf4gemv.EPI_NONE, operand=None, prefetch=None, norm=None):
+    if norm is not None:
+        x = _rms_norm(x, *norm)
+    y = x @ module.dense.T
+    if epi == nf4gemv.EPI_RESIDUAL:
+        return operand + y
+    return F.silu(operand) * y if epi == nf4gemv.EPI_SILU_GATE else y
+
+
+def _rms_norm(x, weight, eps):
+    xf = x.float()
+    return (xf * torch.rsqrt(xf.square().mean(-1, keepdim=True) + eps)).to(x.dtype) * weight
+
+
+def _write(qkv, k, v, block_table, rows, positions, freqs, *, n_head, seqs=None, weight=None, position=None, **_):
+    heads = qkv.view(len(rows), -1, 128)
+    for t in range(len(rows)):
+        s, r, pos = t if seqs is None else int(seqs[t]), int(rows[t]), int(positions[t])
+        if r < 0 or not 0 <= pos < len(freqs) or r >= block_table.shape[1] * k.shape[2]:
+            continue
+        page, at = int(block_table[s, r // k.shape[2]]), r % k.shape[2]
+        if page < 0:
+            continue
+        k[page, :, at], v[page, :, at] = heads[t, n_head:n_head + k.shape[1]], heads[t, n_head + k.shape[1]:]
+        if weight is not None:
+            weight[page, :, at], position[page, :, at] = 0.0, pos
+    return heads[:, :n_head].clone()
+
+
+def _attention(q, k, v, block_table, lens, *, weight=None, **_):
+    """The mean of the rows; each of them is attended to equally."""
+    out = torch.zeros_like(q)
+    for s, n in enumerate(lens.tolist()):
+        for r in range(n):
+            page, at = int(block_table[s, r // k.shape[2]]), r % k.shape[2]
+            out[s] += v[page, :, at].repeat_interleave(q.shape[1] // k.shape[1], 0) / n
+            if weight is not None:
+                weight[page, :, at] += q[s].sum() * 0 + q.shape[1] / k.shape[1] / n
+    return out
+
+
+@pytest.fixture(autouse=True)
+def launches(monkeypatch):
+    monkeypatch.setattr(nf4gemv, "prepare", lambda module: setattr(module, "_nf4_fast", {}) or True)
+    monkeypatch.setattr(nf4gemv, "matmul", _matmul)
+    monkeypatch.setattr(nf4gemv, "matmul_gated", lambda w1, w3, x, *, prefetch=None, norm=None: _matmul(
+        w3, x, norm=norm, epi=nf4gemv.EPI_SILU_GATE, operand=_matmul(w1, x, norm=norm)))
+    monkeypatch.setattr(fusedops, "rms_norm", _rms_norm)
+    monkeypatch.setattr(pagedkv, "write", _write)
+    monkeypatch.setattr(pagedkv, "attention", _attention)
+
+
+def make_block(biases=()):
+    g = torch.Generator().manual_seed(1)
+    blk = model.TransformerBlock(CFG)
+    for norm in (blk.attention_norm, blk.ffn_norm):
+        norm.weight = torch.nn.Parameter(torch.ones(DIM), requires_grad=False)
+    a, ff = blk.attention, blk.feed_forward
+    for name, lin in (("wqkv", a.wqkv), ("wo", a.wo), ("w1", ff.w1), ("w3", ff.w3), ("w2", ff.w2)):
+        lin.dense = torch.randn(lin.out_features, lin.in_features, generator=g) / lin.in_features ** 0.5
+        bias = torch.randn(lin.out_features, generator=g)
+        lin.bias = torch.nn.Parameter(bias, requires_grad=False) if name in biases else None
+    return blk
+
+
+def make_cache(n_seqs=2, **kw):
+    return pagedkv.PagedKVCache(1, n_seqs, 64, 8, KV, page_size=16, device="cpu", dtype=torch.float32, **kw)
+
+
+def block_alone(blk, x):
+    """The block's own formula for tokens of one stream, each attending to all so far by the mean."""
+    def linear(lin, y):
+        return y @ lin.dense.T + (0 if lin.bias is None else lin.bias)
+
+    v = linear(blk.attention.wqkv, _rms_norm(x, blk.attention_norm.weight, CFG.norm_eps))[..., -128 * KV:]
+    mean = v.cumsum(-2) / torch.arange(1, x.shape[-2] + 1)[:, None]
+    h = x + linear(blk.attention.wo, mean.repeat(1, HEADS // KV))
+    hn, ff = _rms_norm(h, blk.ffn_norm.weight, CFG.norm_eps), blk.feed_forward
+    return h + linear(ff.w2, F.silu(linear(ff.w1, hn)) * linear(ff.w3, hn))
+
+
+FREQS = torch.zeros(64, 64, 2)
+BIASES = [(), ("wqkv",), ("wo",), ("w1",), ("w3",), ("w2",), ("wqkv", "wo", "w1", "w3", "w2")]
+
+
+@pytest.mark.parametrize("biases", BIASES)
+def test_decode_adds_the_biases(biases):
+    blk, cache = make_block(biases), make_cache()
+    x = torch.randn(2, 3, DIM, generator=torch.Generator().manual_seed(2))
+    want = torch.stack([block_alone(blk, x[s]) for s in range(2)])
+    for t in range(3):
+        for s in range(2):
+            cache.reserve(s)
+        cache.begin_step()
+        got = pagedkv.decode_block(blk, x[:, t:t + 1], FREQS, cache, 0)
+        cache.end_step()
+        assert torch.allclose(got[:, 0], want[:, t], atol=1e-4)
+
+
+@pytest.mark.parametrize("biases", BIASES)
+def test_prefill_adds_the_biases(biases, monkeypatch):
+    def mean(q, k, v, mask, n_head, n_kv, d):
+        m = mask[0, 0].float()
+        return (m @ v / m.sum(-1, keepdim=True)).repeat_interleave(n_head // n_kv, 1)
+
+    monkeypatch.setattr(fastpath, "_grouped_torch", mean)
+    blk, cache = make_block(biases), make_cache()
+    x = torch.randn(1, 5, DIM, generator=torch.Generator().manual_seed(3))
+    cache.reserve(1, 5)
+    got = pagedkv.prefill_block(blk, x, FREQS, cache, 0, 1)
+    assert torch.allclose(got[0], block_alone(blk, x[0]), atol=1e-4)

@@ -270,15 +270,26 @@ def _norms(a):
     return dict(q_norm=None if qn is None else qn.weight, k_norm=None if kn is None else kn.weight, eps=eps)
 
 
-def _linear(module, x, **kw):
+def _linear(module, x, *, norm=None, epi: int = 0, operand=None):
+    """``nf4gemv.matmul``, with the bias of a linear that has one: added, as its own forward does, to the rounded
+    product, and the epilogue then applied to that. None where `norm` cannot be fused."""
     from ttspipe_b200 import nf4gemv
 
     if getattr(module, "_nf4_fast", None) is None:
         nf4gemv.prepare(module)
-    y = nf4gemv.matmul(module, x, **kw)
-    if y is None and "norm" not in kw:
-        raise ValueError(f"the block's {module} does not run on the NF4 kernels for {tuple(x.shape)} {x.dtype}")
-    return y
+    bias = getattr(module, "bias", None)
+    y = nf4gemv.matmul(module, x, norm=norm, epi=epi if bias is None else nf4gemv.EPI_NONE,
+                       operand=operand if bias is None else None)
+    if y is None:
+        if norm is None:
+            raise ValueError(f"the block's {module} does not run on the NF4 kernels for {tuple(x.shape)} {x.dtype}")
+        return None
+    if bias is None:
+        return y
+    y = (y + bias).to(y.dtype)
+    if epi == nf4gemv.EPI_RESIDUAL:
+        return operand + y
+    return torch.nn.functional.silu(operand) * y if epi == nf4gemv.EPI_SILU_GATE else y
 
 
 def _normed_linear(norm, module, x):
@@ -296,10 +307,11 @@ def _feed_forward(block, h):
     for module in (ff.w1, ff.w3):
         if getattr(module, "_nf4_fast", None) is None:
             nf4gemv.prepare(module)
-    g = nf4gemv.matmul_gated(ff.w1, ff.w3, h, norm=(norm.weight, norm.eps))
+    gated = all(getattr(module, "bias", None) is None for module in (ff.w1, ff.w3))  # the one launch adds none
+    g = nf4gemv.matmul_gated(ff.w1, ff.w3, h, norm=(norm.weight, norm.eps)) if gated else None
     if g is None:
         hn = fusedops.rms_norm(h, norm.weight, norm.eps)
-        g = nf4gemv.matmul_gated(ff.w1, ff.w3, hn)
+        g = nf4gemv.matmul_gated(ff.w1, ff.w3, hn) if gated else None
         if g is None:
             g = _linear(ff.w3, hn, epi=nf4gemv.EPI_SILU_GATE, operand=_linear(ff.w1, hn))
     return _linear(ff.w2, g, epi=nf4gemv.EPI_RESIDUAL, operand=h)
