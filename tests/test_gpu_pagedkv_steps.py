@@ -68,3 +68,53 @@ def test_prefill_of_a_block_with_biases():
         x = randn_bf16((1, 40, CFG.dim), seed=6, device="cuda")
         cache.reserve(1, 40)
         assert near(pagedkv.prefill_block(blk, x, freqs(), cache, 0, 1), own_forward(blk, x, 0))
+
+
+def step(blk, cache, x, table):
+    cache.begin_step()
+    out = pagedkv.decode_block(blk, x, table, cache, 0)
+    cache.end_step()
+    return out
+
+
+def held_by(cache, seq):
+    pages = cache.block_table[seq]
+    pages = pages[pages >= 0].long()
+    pools = (cache.k[0], cache.v[0], cache.weight[0], cache.position[0])
+    return [t[pages].clone() for t in pools] + [cache.lens[seq].clone(), cache.next_pos[seq].clone()]
+
+
+def unchanged(cache, seq, before):
+    return all(torch.equal(a, b) for a, b in zip(held_by(cache, seq), before))
+
+
+def test_a_stream_that_is_not_active_is_passed_over():
+    """NaN in its slot of x: its rows, weights and lengths stay, and it goes on as one that never paused."""
+    blk, table = model.random_block(CFG, device="cuda", seed=40), freqs()
+    x = randn_bf16((2, 24, CFG.dim), seed=41, device="cuda")
+    caches = [pagedkv.PagedKVCache(1, 2, 128, 8, 2, page_size=16, device="cuda") for _ in range(2)]
+    with torch.inference_mode():
+        want = []
+        for t in range(24):
+            for s in range(2):
+                caches[0].reserve(s)
+            want.append(step(blk, caches[0], x[:, t : t + 1].contiguous(), table)[1])
+        cache, at = caches[1], 0
+        for t in range(34):
+            paused = 8 <= t < 18
+            if t == 8:
+                cache.active[1] = 0
+                before = held_by(cache, 1)
+            if t == 18:
+                cache.active[1] = 1
+            cache.reserve(0)
+            if not paused:
+                cache.reserve(1)
+            xt = torch.stack([x[0, min(t, 23)], torch.full_like(x[1, 0], float("nan")) if paused else x[1, at]])[:, None]
+            got = step(blk, cache, xt, table)
+            if paused:
+                assert unchanged(cache, 1, before)
+            else:
+                assert torch.equal(got[1], want[at]), t
+                at += 1
+        assert at == 24 and cache.lens.tolist() == [34, 24]

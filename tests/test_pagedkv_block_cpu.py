@@ -124,3 +124,44 @@ def test_prefill_adds_the_biases(biases, monkeypatch):
     cache.reserve(1, 5)
     got = pagedkv.prefill_block(blk, x, FREQS, cache, 0, 1)
     assert torch.allclose(got[0], block_alone(blk, x[0]), atol=1e-4)
+
+
+def step(blk, cache, x):
+    cache.begin_step()
+    out = pagedkv.decode_block(blk, x, FREQS, cache, 0)
+    cache.end_step()
+    return out
+
+
+def held_by(cache, seq):
+    """Everything the cache holds of a stream."""
+    pages = [p for p in cache.block_table[seq].tolist() if p >= 0]
+    pools = (cache.k[0], cache.v[0], cache.weight[0], cache.position[0])
+    return [t[pages].clone() for t in pools] + [cache.lens[seq].clone(), cache.next_pos[seq].clone()]
+
+
+def unchanged(cache, seq, before):
+    return all(torch.equal(a, b) for a, b in zip(held_by(cache, seq), before))
+
+
+def test_a_stream_that_is_not_active_is_passed_over():
+    """Whatever its slot of x holds: no row, no weight, no length of it changes, and it goes on as if nothing had been."""
+    blk, cache = make_block(), make_cache()
+    x = torch.randn(2, 9, DIM, generator=torch.Generator().manual_seed(4))
+    for t in range(3):
+        for s in range(2):
+            cache.reserve(s)
+        step(blk, cache, x[:, t:t + 1])
+    cache.active[1] = 0
+    before = held_by(cache, 1)
+    for t in range(3, 6):
+        cache.reserve(0)
+        mixed = x[:, t:t + 1].clone()
+        mixed[1] = float("nan")
+        got = step(blk, cache, mixed)
+        assert torch.allclose(got[0, 0], block_alone(blk, x[0])[t], atol=1e-4)
+        assert cache.live[1] == 0 and unchanged(cache, 1, before)
+    cache.active[1] = 1
+    cache.reserve(1)
+    got = step(blk, cache, x[:, 3:4])
+    assert torch.allclose(got[1, 0], block_alone(blk, x[1])[3], atol=1e-4) and cache.lens.tolist()[1] == 4

@@ -182,7 +182,7 @@ class PagedKVCache:
         self.next_pos = torch.zeros(n_seqs, **i32)   # position of its next token
         self.active = torch.zeros(n_seqs, **i32)     # 1: takes part in the steps
         self.rows = torch.full((n_seqs,), -1, **i32)  # of a step: the new row of each stream, -1 for none
-        self.live = torch.zeros(n_seqs, **i32)        # of a step: the rows its token attends to
+        self.live = torch.zeros(n_seqs, **i32)        # of a step: the rows its token attends to, 0 for none
         self._left = torch.zeros(n_seqs, **i32)
         self._free = list(range(n_pages - 1, -1, -1))
         self._pages: list = [[] for _ in range(n_seqs)]
@@ -227,12 +227,13 @@ class PagedKVCache:
         self.active[seq] = 0
 
     def begin_step(self) -> None:
-        """Rows and lengths of one new token of each active stream."""
-        torch.add(self.lens, self.active, out=self.live)
-        torch.add(self.lens, 1, out=self.rows).mul_(self.active).sub_(1)
+        """Rows and lengths of one new token of each active stream; the others have no row and length 0, so
+        that nothing is written for them, attended to or weighed."""
+        torch.add(self.lens, 1, out=self.live).mul_(self.active)
+        torch.sub(self.live, 1, out=self.rows)
 
     def end_step(self) -> None:
-        self.lens.copy_(self.live)
+        self.lens.add_(self.active)
         self.next_pos.add_(self.active)
 
     def write(self, layer: int, qkv, rows, positions, freqs, *, n_head: int, **kw):
