@@ -118,3 +118,42 @@ def test_a_stream_that_is_not_active_is_passed_over():
                 assert torch.equal(got[1], want[at]), t
                 at += 1
         assert at == 24 and cache.lens.tolist() == [34, 24]
+
+
+def test_replayed_steps_pass_over_streams_that_are_not_reserved():
+    """One captured step: streams join, wait at a full page and in the middle of one, and go on."""
+    blk, table = model.random_block(CFG, device="cuda", seed=50), freqs()
+    x = randn_bf16((3, 40, CFG.dim), seed=51, device="cuda")
+    waits = [set(), set(range(16, 20)) | set(range(25, 28)), set(range(5))]
+    caches = [pagedkv.PagedKVCache(1, 3, 128, 12, 2, page_size=16, device="cuda") for _ in range(2)]
+    xt, out = torch.empty(3, 1, CFG.dim, dtype=torch.bfloat16, device="cuda"), None
+    side = torch.cuda.Stream()
+    with torch.inference_mode():
+        want = []
+        with torch.cuda.stream(side):
+            for t in range(40):
+                for s in range(3):
+                    caches[0].reserve(s)
+                want.append(step(blk, caches[0], x[:, t : t + 1].contiguous(), table)[:, 0].clone())
+            graph, cache = torch.cuda.CUDAGraph(), caches[1]
+            with torch.cuda.graph(graph, stream=side):
+                out = step(blk, cache, xt, table)
+        torch.cuda.synchronize()
+        at = [0, 0, 0]
+        for t in range(40):
+            parts = [t not in w for w in waits]
+            before = [held_by(cache, s) for s in range(3)]
+            for s in range(3):
+                xt[s, 0] = x[s, at[s]] if parts[s] else float("nan")
+                if parts[s]:
+                    cache.reserve(s)
+            graph.replay()
+            for s in range(3):
+                if parts[s]:
+                    assert torch.equal(out[s, 0], want[at[s]][s]), (s, t)
+                    at[s] += 1
+                else:
+                    assert torch.equal(cache.lens[s], before[s][4]) and torch.equal(cache.next_pos[s], before[s][5])
+                    assert all(torch.equal(a[: len(b)], b) for a, b in zip(held_by(cache, s)[:4], before[s][:4]))
+        assert cache.lens.tolist() == at == [40, 33, 35]
+        del graph

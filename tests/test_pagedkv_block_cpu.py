@@ -165,3 +165,109 @@ def test_a_stream_that_is_not_active_is_passed_over():
     cache.reserve(1)
     got = step(blk, cache, x[:, 3:4])
     assert torch.allclose(got[1, 0], block_alone(blk, x[1])[3], atol=1e-4) and cache.lens.tolist()[1] == 4
+
+
+def test_a_stream_that_is_not_reserved_is_passed_over():
+    """A stream of 16 rows, its page full, then steps that reserve only the other one; and one in the middle of a page."""
+    blk, cache = make_block(), make_cache()
+    x = torch.randn(2, 40, DIM, generator=torch.Generator().manual_seed(5))
+    alone = [block_alone(blk, x[s]) for s in range(2)]
+    n = [0, 0]
+    for t in range(40):
+        parts = [True, not (16 <= t < 20 or 25 <= t < 28)]
+        before = held_by(cache, 1)
+        for s in range(2):
+            if parts[s]:
+                cache.reserve(s)
+        got = step(blk, cache, torch.stack([x[s, min(n[s], 39)] for s in range(2)])[:, None])
+        assert cache.part.tolist() == [int(p) for p in parts]
+        for s in range(2):
+            if parts[s]:
+                assert torch.allclose(got[s, 0], alone[s][n[s]], atol=1e-4), (s, t)
+                n[s] += 1
+        assert parts[1] or unchanged(cache, 1, before)
+        assert cache.lens.tolist() == n and cache.next_pos.tolist() == n
+        assert all(cache.lens[s] <= cache._rows[s] for s in range(2))
+
+
+def test_rows_reserved_ahead_last_for_as_many_steps():
+    blk, cache = make_block(), make_cache()
+    x = torch.randn(2, 7, DIM, generator=torch.Generator().manual_seed(6))
+    cache.reserve(0, 5)
+    cache.reserve(1, 7)
+    for t in range(7):
+        got = step(blk, cache, x[:, t:t + 1])
+        assert torch.allclose(got[1, 0], block_alone(blk, x[1])[t], atol=1e-4)
+    assert cache.lens.tolist() == [5, 7]
+
+
+def test_a_prompt_is_filled_in_while_others_decode(monkeypatch):
+    def mean(q, k, v, mask, n_head, n_kv, d):
+        m = mask[0, 0].float()
+        return (m @ v / m.sum(-1, keepdim=True)).repeat_interleave(n_head // n_kv, 1)
+
+    monkeypatch.setattr(fastpath, "_grouped_torch", mean)
+    blk, cache = make_block(), make_cache()
+    x = torch.randn(2, 30, DIM, generator=torch.Generator().manual_seed(7))
+    alone = [block_alone(blk, x[s]) for s in range(2)]
+    at = 0
+
+    def decode(both=False):
+        nonlocal at
+        cache.reserve(0)
+        if both:
+            cache.reserve(1)
+        got = step(blk, cache, torch.stack([x[0, at], x[1, int(cache.lens[1]) if both else 0]])[:, None])
+        assert torch.allclose(got[0, 0], alone[0][at], atol=1e-4)
+        at += 1
+        return got[1, 0]
+
+    decode()
+    cache.reserve(1, 20, prompt=True)
+    decode()
+    got = pagedkv.prefill_block(blk, x[1:, :13], FREQS, cache, 0, 1)
+    assert torch.allclose(got[0], alone[1][:13], atol=1e-4)
+    decode()
+    cache.prefilled(1, 13)
+    decode()
+    got = pagedkv.prefill_block(blk, x[1:, 13:20], FREQS, cache, 0, 1, rows=13, position=13)
+    assert torch.allclose(got[0], alone[1][13:20], atol=1e-4)
+    decode()
+    cache.prefilled(1, 7)
+    assert cache.lens.tolist() == [5, 20] and cache.next_pos.tolist() == [5, 20]
+    decode()  # nothing is reserved for its next token yet
+    for t in range(20, 25):
+        assert torch.allclose(decode(both=True), alone[1][t], atol=1e-4)
+    assert cache.lens.tolist() == [11, 25]
+
+
+def test_while_a_prompt_is_filled_in_nothing_takes_its_rows():
+    cache = make_cache()
+    cache.reserve(0, 20)
+    cache.reserve(1, 20, prompt=True)
+    for call in (lambda: cache.evict(8), lambda: cache.evict_and_trim(8), lambda: cache.trim(1, 8)):
+        with pytest.raises(RuntimeError, match="prompt"):
+            call()
+    for rows in (21, -1):
+        with pytest.raises(ValueError, match="20 are reserved"):
+            cache.prefilled(1, rows)
+    with pytest.raises(ValueError, match="0 are reserved"):
+        cache.prefilled(0, 1)
+    assert cache.active.tolist() == [1, 0] and cache.lens.tolist() == [0, 0]
+    cache.release(1)
+    cache.trim(0, 8)
+    cache.reserve(1)
+    assert cache.active.tolist() == [1, 1] and cache.free_pages() == 6
+
+
+def test_rows_taken_back_by_a_trim_are_not_stepped_into():
+    cache = make_cache(track=False)
+    cache.reserve(0, 40)  # ahead
+    cache.lens[0] = 30
+    cache.lens[0] = 20  # an eviction
+    cache.trim(0, 20)
+    cache.begin_step()
+    assert cache.rows.tolist() == [-1, -1] and cache.part.tolist() == [0, 0]
+    cache.reserve(0)
+    cache.begin_step()
+    assert cache.rows.tolist() == [20, -1] and cache.live.tolist() == [21, 0]

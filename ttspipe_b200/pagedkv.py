@@ -161,8 +161,12 @@ class PagedKVCache:
 
     A decode step: ``reserve(stream)`` for every stream that takes part (its next row needs a
     page), ``begin_step()``, the blocks (``decode_block``), ``end_step()``; between steps
-    ``evict`` where streams grow past a budget. A stream without ``active`` is passed over.
-    Everything but ``reserve``, ``trim`` and ``release`` runs on the device and can be captured."""
+    ``evict`` where streams grow past a budget. Rows can be reserved for several steps ahead. A
+    stream whose reserved rows are used up, or without ``active``, is passed over: its rows, weights,
+    length and next position stay as they are.
+    A prompt: ``reserve(stream, rows, prompt=True)``, ``prefill_block`` through the layers,
+    ``prefilled(stream, rows)``; steps in between pass the stream over.
+    Everything but ``reserve``, ``prefilled``, ``trim`` and ``release`` runs on the device and can be captured."""
 
     def __init__(self, n_layers: int, n_seqs: int, max_len: int, n_pages: int, n_kv: int, *, page_size: int = 64,
                  device, dtype=torch.bfloat16, track: bool = True):
@@ -178,22 +182,30 @@ class PagedKVCache:
         self.position = per_layer(pool[:3], torch.int32) if track else [None] * n_layers
         self.block_table = torch.full((n_seqs, self.max_pages), -1, dtype=torch.int32, device=device)
         i32 = dict(dtype=torch.int32, device=device)
-        self.lens = torch.zeros(n_seqs, **i32)       # rows of each stream
-        self.next_pos = torch.zeros(n_seqs, **i32)   # position of its next token
-        self.active = torch.zeros(n_seqs, **i32)     # 1: takes part in the steps
+        # a stream takes part in a step where its two numbers in _at, its length and 0, are below those in _below,
+        # the rows promised to it and `active`
+        self._at, self._below, self._is_below = (torch.zeros(2, n_seqs, **i32) for _ in range(3))
+        self.lens = self._at[0]                       # rows of each stream
+        self.next_pos = torch.zeros(n_seqs, **i32)    # position of its next token
+        self.active = self._below[1]                  # 1: takes part in the steps that it has rows for
+        self._promised = self._below[0].unbind()
+        self.part = torch.zeros(n_seqs, **i32)        # of a step: 1 for each stream that takes part
         self.rows = torch.full((n_seqs,), -1, **i32)  # of a step: the new row of each stream, -1 for none
         self.live = torch.zeros(n_seqs, **i32)        # of a step: the rows its token attends to, 0 for none
         self._left = torch.zeros(n_seqs, **i32)
         self._free = list(range(n_pages - 1, -1, -1))
         self._pages: list = [[] for _ in range(n_seqs)]
         self._rows = [0] * n_seqs  # rows promised to each stream
+        self._prompt = [0] * n_seqs  # those of them that a prompt has not filled yet
 
     def free_pages(self) -> int:
         return len(self._free)
 
-    def reserve(self, seq: int, rows: int = 1) -> None:
+    def reserve(self, seq: int, rows: int = 1, *, prompt: bool = False) -> None:
         """Pages for `rows` more rows of a stream, which becomes active. Refuses (ValueError) what is past the
-        stream's capacity and (RuntimeError) what the free pages do not hold, changing nothing."""
+        stream's capacity and (RuntimeError) what the free pages do not hold, changing nothing.
+        `prompt`: the rows are filled by ``prefill_block``, and the stream is passed over until ``prefilled`` has
+        counted them (otherwise each step takes the next of them for its token)."""
         want = self._rows[seq] + rows
         need = -(-want // self.page_size)
         if rows < 0 or need > self.max_pages:
@@ -205,13 +217,33 @@ class PagedKVCache:
             new = [self._free.pop() for _ in range(need - len(held))]
             self.block_table[seq, len(held):need] = torch.tensor(new, dtype=torch.int32).to(self.block_table.device)
             held += new
-        if self._rows[seq] == 0 and rows:
+        if prompt and rows:
+            self._prompt[seq] += rows
+            self.active[seq] = 0
+        elif self._rows[seq] == 0 and rows:
             self.active[seq] = 1
         self._rows[seq] = want
+        self._promised[seq].fill_(want)
+
+    def prefilled(self, seq: int, rows: int) -> None:
+        """`rows` tokens of a prompt have passed through every layer's ``prefill_block``: they count as rows of the
+        stream and as positions, and with the last of those reserved the stream takes part in steps."""
+        if not 0 <= rows <= self._prompt[seq]:
+            raise ValueError(f"{rows} rows of stream {seq}, {self._prompt[seq]} are reserved for its prompt")
+        self._prompt[seq] -= rows
+        self.lens[seq] += rows
+        self.next_pos[seq] += rows
+        if rows and not self._prompt[seq]:
+            self.active[seq] = 1
 
     def trim(self, seq: int, rows: int) -> None:
-        """A stream has `rows` rows left (after an eviction): later pages become free."""
-        self._rows[seq] = min(self._rows[seq], rows)
+        """A stream has `rows` rows left (after an eviction): later pages become free. Refused (RuntimeError) while
+        its prompt is still being filled in."""
+        if self._prompt[seq]:
+            raise RuntimeError(f"{self._prompt[seq]} rows of stream {seq} are reserved for its prompt")
+        if rows < self._rows[seq]:
+            self._rows[seq] = rows
+            self._promised[seq].fill_(rows)
         keep = -(-self._rows[seq] // self.page_size)
         held = self._pages[seq]
         if keep < len(held):
@@ -221,20 +253,23 @@ class PagedKVCache:
 
     def release(self, seq: int) -> None:
         """A stream has ended: its pages become free and its place can be used again."""
+        self._prompt[seq] = 0
         self.trim(seq, 0)
         self.lens[seq] = 0
         self.next_pos[seq] = 0
         self.active[seq] = 0
 
     def begin_step(self) -> None:
-        """Rows and lengths of one new token of each active stream; the others have no row and length 0, so
+        """Rows and lengths of one new token of each stream that takes part; the others have no row and length 0, so
         that nothing is written for them, attended to or weighed."""
-        torch.add(self.lens, 1, out=self.live).mul_(self.active)
+        torch.lt(self._at, self._below, out=self._is_below)
+        torch.amin(self._is_below, 0, out=self.part)
+        torch.addcmul(self.part, self.part, self.lens, out=self.live)
         torch.sub(self.live, 1, out=self.rows)
 
     def end_step(self) -> None:
-        self.lens.add_(self.active)
-        self.next_pos.add_(self.active)
+        self.lens.add_(self.part)
+        self.next_pos.add_(self.part)
 
     def write(self, layer: int, qkv, rows, positions, freqs, *, n_head: int, **kw):
         """``write`` into one layer's pools."""
@@ -246,7 +281,10 @@ class PagedKVCache:
         return attention(q, self.k[layer], self.v[layer], self.block_table, self.live, weight=self.weight[layer], **kw)
 
     def evict(self, budget: int, *, recent: int = 0, sink: int = 0) -> None:
-        """``evict`` in every layer (each head by its own weights); afterwards ``trim`` frees the pages."""
+        """``evict`` in every layer (each head by its own weights); afterwards ``trim`` frees the pages. Refused
+        (RuntimeError) while a prompt is still being filled in: its rows lie past the lengths."""
+        if any(self._prompt):
+            raise RuntimeError(f"the prompt of stream {next(s for s, n in enumerate(self._prompt) if n)} is not filled in")
         for i in range(self.n_layers):
             evict(self.k[i], self.v[i], self.weight[i], self.position[i], self.block_table, self.lens, budget=budget,
                   recent=recent, sink=sink, lens_out=self._left)
@@ -322,7 +360,7 @@ def decode_block(block, x, freqs, cache: PagedKVCache, layer: int):
     """One token of every stream through a transformer block: ``fusedlayer.decode_block``
     for a batch, over a paged cache. `x` is [n_seqs, 1, dim], `freqs` the whole rotary
     table (rows, 64, 2); between ``cache.begin_step()`` and ``cache.end_step()``. The
-    rows of streams that are not active are computed and mean nothing."""
+    rows of streams that take no part (``cache.part``) are computed and mean nothing."""
     from ttspipe_b200 import nf4gemv
 
     a = block.attention
@@ -338,7 +376,7 @@ def decode_block(block, x, freqs, cache: PagedKVCache, layer: int):
 def prefill_block(block, x, freqs, cache: PagedKVCache, layer: int, seq: int, rows: int = 0, position: int = 0):
     """The tokens `x` [1, T, dim] of one stream through a transformer block, entering the
     cache after its `rows` rows, from token position `position` on (both on the host;
-    ``reserve`` T rows first and, after the last layer, add T to ``lens`` and ``next_pos``).
+    ``reserve`` T rows with ``prompt`` first, and ``prefilled`` after the last layer).
     Each attends to the rows before it and to itself, by the grouped torch formulation
     of ``fastpath``; weights are not accumulated here."""
     from ttspipe_b200 import fastpath, nf4gemv
