@@ -271,3 +271,14 @@ def test_rows_taken_back_by_a_trim_are_not_stepped_into():
     cache.reserve(0)
     cache.begin_step()
     assert cache.rows.tolist() == [20, -1] and cache.live.tolist() == [21, 0]
+
+
+@pytest.mark.parametrize("rows,position", [(0, 0), (10, 10), (-1, 0)])
+def test_prefill_refuses_rows_that_are_not_reserved(rows, position):
+    blk, cache = make_block(), make_cache()
+    cache.reserve(0, 20, prompt=True)
+    cache.reserve(1, 20, prompt=True)
+    before = cache.k[0].clone()
+    with pytest.raises(ValueError, match="reserved"):
+        pagedkv.prefill_block(blk, torch.randn(1, 21, DIM), FREQS, cache, 0, 1, rows=rows, position=position)
+    assert torch.equal(cache.k[0], before)

@@ -201,6 +201,10 @@ class PagedKVCache:
     def free_pages(self) -> int:
         return len(self._free)
 
+    def reserved(self, seq: int) -> int:
+        """The rows promised to a stream, those that it has among them."""
+        return self._rows[seq]
+
     def reserve(self, seq: int, rows: int = 1, *, prompt: bool = False) -> None:
         """Pages for `rows` more rows of a stream, which becomes active. Refuses (ValueError) what is past the
         stream's capacity and (RuntimeError) what the free pages do not hold, changing nothing.
@@ -382,6 +386,8 @@ def prefill_block(block, x, freqs, cache: PagedKVCache, layer: int, seq: int, ro
     from ttspipe_b200 import fastpath, nf4gemv
 
     a, n = block.attention, x.shape[1]
+    if rows < 0 or rows + n > cache.reserved(seq):
+        raise ValueError(f"rows {rows} to {rows + n} of stream {seq}: {cache.reserved(seq)} are reserved")
     dev = x.device
     qkv = _normed_linear(block.attention_norm, a.wqkv, x)
     at = torch.arange(n, dtype=torch.int32, device=dev)
