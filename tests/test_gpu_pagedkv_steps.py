@@ -157,3 +157,30 @@ def test_replayed_steps_pass_over_streams_that_are_not_reserved():
                     assert all(torch.equal(a[: len(b)], b) for a, b in zip(held_by(cache, s)[:4], before[s][:4]))
         assert cache.lens.tolist() == at == [40, 33, 35]
         del graph
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_positions_past_the_rotary_table_are_passed_over(captured):
+    """A bounded stream runs on until its positions reach the table's end and stops there, unchanged."""
+    blk, table = model.random_block(CFG, device="cuda", seed=60), freqs(40)
+    caches = [pagedkv.PagedKVCache(1, 2, 64, 8, 2, page_size=16, device="cuda") for _ in range(2)]
+    x = randn_bf16((2, 1, CFG.dim), seed=61, device="cuda")
+    side, cache = torch.cuda.Stream(), caches[1]
+    with torch.inference_mode(), torch.cuda.stream(side):
+        step(blk, caches[0], x, table)
+        graph = torch.cuda.CUDAGraph()
+        if captured:
+            with torch.cuda.graph(graph, stream=side):
+                step(blk, cache, x, table)
+        for t in range(50):
+            cache.reserve(0)
+            before = held_by(cache, 0)
+            graph.replay() if captured else step(blk, cache, x, table)
+            assert t < 40 or unchanged(cache, 0, before)
+            if cache.lens[0] >= 30 and t < 40:
+                cache.evict_and_trim(16, recent=4, sink=1)
+            if t >= 40:
+                cache.trim(0, int(cache.lens[0]))
+        assert cache.next_pos.tolist() == [40, 0] and cache.part.tolist() == [0, 0]
+        del graph
+    torch.cuda.synchronize()

@@ -282,3 +282,35 @@ def test_prefill_refuses_rows_that_are_not_reserved(rows, position):
     with pytest.raises(ValueError, match="reserved"):
         pagedkv.prefill_block(blk, torch.randn(1, 21, DIM), FREQS, cache, 0, 1, rows=rows, position=position)
     assert torch.equal(cache.k[0], before)
+
+
+def test_positions_past_the_rotary_table_are_passed_over():
+    """An evicted stream's positions run ahead of its rows: at the table's end it stops, with nothing changed."""
+    blk, cache = make_block(), make_cache()
+    x = torch.randn(2, 9, DIM, generator=torch.Generator().manual_seed(8))
+    cache.reserve(0)
+    step(blk, cache, x[:, :1])  # the longer table is seen first
+    cache.next_pos[0] = 3
+    cache.reserve(0, 4)
+    cache.reserve(1, 9)
+    for t in range(8):
+        if t >= 3:
+            before = held_by(cache, 0)
+        cache.begin_step()
+        pagedkv.decode_block(blk, x[:, t:t + 1], FREQS[:6], cache, 0)
+        cache.end_step()
+        assert t < 3 or unchanged(cache, 0, before)
+    assert cache.lens.tolist() == [4, 6] and cache.next_pos.tolist() == [6, 6]
+    assert cache.part.tolist() == [0, 0] and cache.live.tolist() == [0, 0]
+    cache.release(0)
+    cache.reserve(0)
+    cache.begin_step()
+    assert cache.part.tolist() == [1, 0]
+
+
+@pytest.mark.parametrize("rows,position", [(0, 2), (0, -1)])
+def test_prefill_refuses_positions_outside_the_rotary_table(rows, position):
+    blk, cache = make_block(), make_cache()
+    cache.reserve(0, 5, prompt=True)
+    with pytest.raises(ValueError, match="rotary"):
+        pagedkv.prefill_block(blk, torch.randn(1, 5, DIM), FREQS[:6], cache, 0, 0, rows=rows, position=position)

@@ -162,8 +162,8 @@ class PagedKVCache:
     A decode step: ``reserve(stream)`` for every stream that takes part (its next row needs a
     page), ``begin_step()``, the blocks (``decode_block``), ``end_step()``; between steps
     ``evict`` where streams grow past a budget. Rows can be reserved for several steps ahead. A
-    stream whose reserved rows are used up, or without ``active``, is passed over: its rows, weights,
-    length and next position stay as they are.
+    stream whose reserved rows are used up, whose next position is past the rotary table, or without
+    ``active``, is passed over: its rows, weights, length and next position stay as they are.
     A prompt: ``reserve(stream, rows, prompt=True)``, ``prefill_block`` through the layers,
     ``prefilled(stream, rows)``; steps in between pass the stream over.
     Everything but ``reserve``, ``prefilled``, ``trim`` and ``release`` runs on the device and can be captured."""
@@ -182,12 +182,14 @@ class PagedKVCache:
         self.position = per_layer(pool[:3], torch.int32) if track else [None] * n_layers
         self.block_table = torch.full((n_seqs, self.max_pages), -1, dtype=torch.int32, device=device)
         i32 = dict(dtype=torch.int32, device=device)
-        # a stream takes part in a step where its two numbers in _at, its length and 0, are below those in _below,
-        # the rows promised to it and `active`
-        self._at, self._below, self._is_below = (torch.zeros(2, n_seqs, **i32) for _ in range(3))
+        # a stream takes part in a step where its three numbers in _at, its length, its next token's position and 0,
+        # are below those in _below: the rows promised to it, the rotary table's and `active`
+        self._at, self._below, self._is_below = (torch.zeros(3, n_seqs, **i32) for _ in range(3))
         self.lens = self._at[0]                       # rows of each stream
-        self.next_pos = torch.zeros(n_seqs, **i32)    # position of its next token
-        self.active = self._below[1]                  # 1: takes part in the steps that it has rows for
+        self.next_pos = self._at[1]                   # position of its next token
+        self.active = self._below[2]                  # 1: takes part in the steps that it has rows for
+        self._positions = self._step_positions = 2**31 - 1  # rows of the shortest rotary table seen, in this step
+        self._below[1] = self._positions
         self._promised = self._below[0].unbind()
         self.part = torch.zeros(n_seqs, **i32)        # of a step: 1 for each stream that takes part
         self.rows = torch.full((n_seqs,), -1, **i32)  # of a step: the new row of each stream, -1 for none
@@ -266,17 +268,24 @@ class PagedKVCache:
     def begin_step(self) -> None:
         """Rows and lengths of one new token of each stream that takes part; the others have no row and length 0, so
         that nothing is written for them, attended to or weighed."""
+        self._step_positions = 2**31 - 1
         torch.lt(self._at, self._below, out=self._is_below)
         torch.amin(self._is_below, 0, out=self.part)
         torch.addcmul(self.part, self.part, self.lens, out=self.live)
         torch.sub(self.live, 1, out=self.rows)
 
     def end_step(self) -> None:
-        self.lens.add_(self.part)
-        self.next_pos.add_(self.part)
+        self._at[:2].add_(self.part)
 
     def write(self, layer: int, qkv, rows, positions, freqs, *, n_head: int, **kw):
-        """``write`` into one layer's pools."""
+        """``write`` into one layer's pools. The first call with a rotary table (or a shorter one) bounds the positions
+        of later steps by it."""
+        n = freqs.shape[0]
+        if n < self._positions and n < self._step_positions:
+            self._below[1].fill_(n)
+            self._step_positions = n
+            if not (self.lens.is_cuda and torch.cuda.is_current_stream_capturing()):  # else only the replays set it
+                self._positions = n
         return write(qkv, self.k[layer], self.v[layer], self.block_table, rows, positions, freqs, n_head=n_head,
                      weight=self.weight[layer], position=self.position[layer], **kw)
 
@@ -388,6 +397,8 @@ def prefill_block(block, x, freqs, cache: PagedKVCache, layer: int, seq: int, ro
     a, n = block.attention, x.shape[1]
     if rows < 0 or rows + n > cache.reserved(seq):
         raise ValueError(f"rows {rows} to {rows + n} of stream {seq}: {cache.reserved(seq)} are reserved")
+    if position < 0 or position + n > freqs.shape[0]:
+        raise ValueError(f"positions {position} to {position + n}: the rotary table has {freqs.shape[0]} rows")
     dev = x.device
     qkv = _normed_linear(block.attention_norm, a.wqkv, x)
     at = torch.arange(n, dtype=torch.int32, device=dev)
