@@ -583,8 +583,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 && kWarps == 4 ? 3 : 1)
 // attention kernel left (a row's weight needs the sum over all rows, which only the
 // joins know). Four rows to a thread; a reduction instruction instead of a read and a
 // write, so that sequences which share a page add up. Rows that take no part have the
-// score -inf and receive 0. Memory bounds it: 4 groups + 8 bytes a row and KV head, 20 us
-// for 64 x 8192 rows (100 MB), about 4 us for small calls.
+// score -inf and receive 0, also where the sum of a head is NaN. Memory bounds it: 4 groups + 8 bytes a row and KV head,
+// 20 us for 64 x 8192 rows (100 MB), about 4 us for small calls.
 constexpr int kWThreads = 256;
 constexpr int kWTiles = kWThreads / 4;  // tiles of one pass of a CTA
 
@@ -617,6 +617,16 @@ __global__ void __launch_bounds__(kWThreads) paged_weight_kernel(const __grid_co
       w.w += exp2_fast(x.w - L);
     }
     if (pg < 0 || pg >= p.n_pages) continue;
+    if (!(w.x == w.x && w.y == w.y && w.z == w.z && w.w == w.w)) {
+      // a head whose sum is NaN (a visible score is NaN or +inf): the rows that take no part keep what they have
+      const int n = seq_rows(p, b) - (tile * kTile + i);
+      const uint8_t* mask =
+          p.mask == nullptr ? nullptr : p.mask + (size_t)b * p.max_pages * p.page_size + tile * kTile + i;
+      if (n <= 0 || (mask != nullptr && mask[0] == 0)) w.x = 0.f;
+      if (n <= 1 || (mask != nullptr && mask[1] == 0)) w.y = 0.f;
+      if (n <= 2 || (mask != nullptr && mask[2] == 0)) w.z = 0.f;
+      if (n <= 3 || (mask != nullptr && mask[3] == 0)) w.w = 0.f;
+    }
     float* out = p.weight + ((size_t)pg * p.n_kv + h) * p.page_size + (size_t)(tile % tpp) * kTile + i;
     asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(out), "f"(w.x), "f"(w.y), "f"(w.z), "f"(w.w)
                  : "memory");
