@@ -542,7 +542,8 @@ size_t nf4b_paged_attention_workspace_size(int n_seqs, int n_head, int n_kv, int
  * stay; nothing else moves (attention does not depend on the order of rows), so
  * rows [0, lens_out[s]) hold the sequence and later pages are free. weight_out, position_out and
  * lens_out receive those rows' weights and positions and the new lengths; each may be
- * its input. Needs weight and position, budget >= 1, sink + recent <= budget,
+ * its input. Rows of unassigned pages are not there: those below the new length are no
+ * places, so as many fewer rows stay, and the others cannot stay. Needs weight and position, budget >= 1, sink + recent <= budget,
  * and pages that no other sequence shares. The workspace needs no initial value.
  */
 int nf4b_paged_evict(const nf4b_paged_kv* cache, const int32_t* lens, int budget, int recent, int sink,

@@ -9,7 +9,7 @@ import torch
 
 from oracle import paged_oracle as po
 from tests.test_gpu_pagedkv import DT, Pool, attend, f64
-from ttspipe_b200 import nf4gemv
+from ttspipe_b200 import nf4gemv, pagedkv
 
 pytestmark = pytest.mark.gpu
 
@@ -44,3 +44,54 @@ def test_a_score_that_is_not_finite_reaches_the_weights_of_visible_rows_only(val
     assert nan.any() and np.array_equal(np.isnan(w), nan)
     assert np.all(np.abs(w - added)[~nan] <= 2.0 ** -13 * added[~nan])
     assert np.array_equal(np.isnan(f64(got)), np.isnan(want))
+
+
+@pytest.mark.parametrize("n,page,gone,budget,recent,sink", [
+    (96, 16, [1], 48, 16, 0),          # a gap below the budget
+    (96, 16, [0, 4], 48, 16, 3),       # the first page, and one that would move
+    (96, 16, [5], 48, 16, 0),          # the newest rows are not there
+    (70, 16, [1, 2], 40, 40, 0),       # the budget ends in a page that is assigned, all places protected
+    (70, 16, [2], 40, 4, 2),           # the budget ends inside the gap
+    (70, 16, [0, 1, 2, 3, 4], 30, 3, 1),  # nothing is there
+    (3000, 48, [3, 7, 20, 61], 1111, 200, 5),
+    (9001, 64, list(range(10, 40)), 4000, 64, 4),
+    (40000, 128, [1, 2, 100, 200, 311], 20001, 2000, 16),
+])
+@pytest.mark.parametrize("inplace", [False, True])
+def test_evict_of_a_table_with_unassigned_pages(n, page, gone, budget, recent, sink, inplace):
+    """The places below the budget that have a page go to the best of the rows that have one."""
+    p = Pool([n, 50], n_kv=2, page=page, dtype=torch.bfloat16, seed=n)
+    tab = p.table.cpu().numpy()
+    tab[0, gone] = [-1 if i % 2 else p.n_pages + i for i in range(len(gone))]
+    p.table.copy_(torch.from_numpy(tab))
+    rng = np.random.default_rng(n)
+    k0, v0, left = p.k.clone(), p.v.clone(), min(n, budget)
+    pg, at = po.slots(tab[0], np.arange(n), p.n_pages, page)
+    there = np.nonzero(pg >= 0)[0]
+    w, pos = rng.random((2, n)).astype(np.float32).round(2), np.stack([rng.permutation(n) for _ in range(2)])
+    for h in range(2):
+        p.weight[pg[there], h, at[there]] = torch.as_tensor(w[h, there], device="cuda")
+        p.position[pg[there], h, at[there]] = torch.as_tensor(pos[h, there], dtype=torch.int32, device="cuda")
+    outs = (p.weight, p.position, p.lens) if inplace else \
+        (torch.full_like(p.weight, -7.0), torch.full_like(p.position, -7), torch.full_like(p.lens, -7))
+    pagedkv.evict(p.k, p.v, p.weight, p.position, p.table, p.lens, budget=budget, recent=recent, sink=sink,
+                  weight_out=outs[0], position_out=outs[1], lens_out=outs[2])
+    assert outs[2].tolist() == [left, min(50, budget)]
+    inside = there[there < left]
+    k1, v1 = k0.clone(), v0.clone()
+    for h in range(2):
+        keep = np.zeros(n, bool)
+        if len(inside):
+            keep[there] = po.kept(w[h, there], pos[h, there], len(inside), recent, sink)
+        to, src = inside[~keep[inside]], there[(there >= left) & keep[there]]
+        assert len(to) == len(src)
+        k1[pg[to], h, at[to]], v1[pg[to], h, at[to]] = k0[pg[src], h, at[src]], v0[pg[src], h, at[src]]
+        new = np.arange(n)
+        new[to] = src
+        assert np.array_equal(outs[0][pg[inside], h, at[inside]].cpu().numpy(), w[h, new[inside]])
+        assert np.array_equal(outs[1][pg[inside], h, at[inside]].cpu().numpy(), pos[h, new[inside]])
+    mine = np.zeros(p.n_pages, bool)
+    mine[pg[there]] = True
+    for now, want in ((p.k, k1), (p.v, v1)):
+        now, want = now[torch.from_numpy(mine).cuda()], want[torch.from_numpy(mine).cuda()]
+        assert torch.equal(now.view(torch.int16), want.view(torch.int16))

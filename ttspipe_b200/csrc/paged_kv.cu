@@ -214,6 +214,10 @@ __global__ void __launch_bounds__(kWriteWarps * 32, kPairs == 4 ? 7 : 1)
 // past `left` that stay move, in order, into the rows below it that do not: there are
 // equally many, the two sets are disjoint, and attention does not depend on the order
 // of rows (the rotary is in the keys), so nothing else has to move.
+// Rows without a page hold nothing. Below `left` they are no places: they count as kept where
+// they are, before all others (there are at most `left` of them, and equal keys go by rising
+// row), so as many rows stay as there are places with a page. From `left` on they come last,
+// and rows with a page suffice: the places' own are as many.
 //
 // paged_select_kernel, one CTA or one cluster of CTAs a list, finds the smallest kept key
 // digit by digit from the top (11, 11 and 10 bits, a histogram each) and lists the moves;
@@ -224,7 +228,8 @@ __global__ void __launch_bounds__(kWriteWarps * 32, kPairs == 4 ? 7 : 1)
 constexpr int kBins = 2048;
 
 // Weights in rising order as unsigned integers; 0xFFFFFFFF (no weight maps there,
-// NaN being taken as -inf) is for the protected rows, 0 for rows without a page.
+// NaN being taken as -inf) is for the protected rows and those below `left` without a page, 0
+// for the others without one.
 __device__ __forceinline__ uint32_t weight_key(float w) {
   if (!(w == w)) w = -INFINITY;
   const uint32_t u = __float_as_uint(w + 0.0f);  // -0 as 0
@@ -384,14 +389,19 @@ __global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : 1024 / kThrea
     for (int r = 1; r < size; ++r) newest = max(newest, *cluster_peer(&s_newest, (rank + r) % size));
   // positions above this are among the newest (no position is above INT_MAX)
   const int guard = p.recent == 0 ? INT_MAX : newest < INT_MIN + p.recent ? INT_MIN : newest - p.recent;
-  auto to_keys = [&]() {
+  auto to_keys = [&](int first) {
     auto key = [&](float wt, int pos) -> uint32_t {
       return pos < p.sink || pos > guard ? 0xFFFFFFFFu : weight_key(wt);
     };
 #pragma unroll
-    for (int u = 0; u < kDeep; ++u)
-      k[u] = at[u] < 0 ? make_uint4(0, 0, 0, 0)
-                       : make_uint4(key(w[u].x, x[u].x), key(w[u].y, x[u].y), key(w[u].z, x[u].z), key(w[u].w, x[u].w));
+    for (int u = 0; u < kDeep; ++u) {
+      if (at[u] >= 0) {
+        k[u] = make_uint4(key(w[u].x, x[u].x), key(w[u].y, x[u].y), key(w[u].z, x[u].z), key(w[u].w, x[u].w));
+      } else {
+        const int i = left - (first + u * 128);
+        k[u] = make_uint4(i > 0 ? ~0u : 0u, i > 1 ? ~0u : 0u, i > 2 ? ~0u : 0u, i > 3 ? ~0u : 0u);
+      }
+    }
   };
   // f(u, i) for every group of the run, its first row i, with k[u] and at[u]
   auto each_batch = [&](auto f) {
@@ -399,12 +409,12 @@ __global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : 1024 / kThrea
     for (int i0 = r0; i0 < r1; i0 += kDeep * 128) {
       if (!kOnce) {
         load(q, true);
-        to_keys();
+        to_keys(i0 + lane * 4);
       }
       f(i0 + lane * 4);
     }
   };
-  if (kOnce) to_keys();
+  if (kOnce) to_keys(r0 + lane * 4);
 
   // the first digit's histogram
   const uint32_t kZero = weight_key(0.f);
@@ -621,8 +631,8 @@ __global__ void __launch_bounds__(kThreads, kThreads == 1024 ? 1 : 1024 / kThrea
       int hole_to = hole_at + (mine & 0xFFFF), out_to = out_at + (mine >> 16);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (hole[u] >> j & 1) to[hole_to++] = at[u] < 0 ? -1 : at[u] + j;
-        if (out[u] >> j & 1) src[out_to++] = at[u] < 0 ? -1 : at[u] + j;
+        if (hole[u] >> j & 1) to[hole_to++] = at[u] + j;
+        if (out[u] >> j & 1) src[out_to++] = at[u] + j;
       }
       hole_at += sum & 0xFFFF;
       out_at += sum >> 16;
@@ -654,7 +664,6 @@ __global__ void __launch_bounds__(kMoveWarps * 32, 4)
     if (lane < kMoveRows && row + mine < p.max_moves && row + mine < p.count[list]) {
       from = p.src[(size_t)list * p.max_moves + row + mine];
       at = p.to[(size_t)list * p.max_moves + row + mine];
-      if (from < 0 || at < 0) from = at = -1;
     }
     list += step_list;
     row += step_row;

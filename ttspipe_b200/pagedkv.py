@@ -134,7 +134,8 @@ def evict(k, v, weight, position, block_table, lens, *, budget: int, recent: int
     [0, new length) hold the sequence - in another order, which attention does not
     see - and the pages after them are free. `weight_out`, `position_out` and
     `lens_out` receive the rows' weights and positions and the new lengths; None: in place.
-    The sequences must not share pages."""
+    The sequences must not share pages. Rows of unassigned pages are not there: those below the
+    new length are no places, so as many fewer of the others stay."""
     call, dev = (_native or _bound()).evict, k.get_device()
     stream = _stream(dev) if dev >= 0 else 0
     args = (k, v, weight, position, block_table, lens, budget, recent, sink,
