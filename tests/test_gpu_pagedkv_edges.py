@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from oracle import paged_oracle as po
-from tests.test_gpu_pagedkv import DT, Pool, attend, f64
+from tests.test_gpu_pagedkv import DT, Pool, attend, f64, one_rounding
 from ttspipe_b200 import nf4gemv, pagedkv
 
 pytestmark = pytest.mark.gpu
@@ -95,3 +95,41 @@ def test_evict_of_a_table_with_unassigned_pages(n, page, gone, budget, recent, s
     for now, want in ((p.k, k1), (p.v, v1)):
         now, want = now[torch.from_numpy(mine).cuda()], want[torch.from_numpy(mine).cuda()]
         assert torch.equal(now.view(torch.int16), want.view(torch.int16))
+
+
+@pytest.mark.parametrize("name", ["bf16", "fp16"])
+@pytest.mark.parametrize("heads", [(8, 2), (16, 1)])
+@pytest.mark.parametrize("n", [300, 9000])
+def test_attention_of_infinite_values(n, heads, name):
+    """An infinity in a visible value is one of the output's, opposite ones are NaN; no other dimension notices."""
+    p = Pool([n, 40], n_kv=heads[1], page=16, dtype=DT[name], seed=5)
+    q = torch.randn(2, heads[0], 128, generator=torch.Generator().manual_seed(4)).to(DT[name]).cuda()
+    for s, r, d, val in ((0, 3, 7, np.inf), (0, n - 100, 9, -np.inf), (0, 5, 11, np.inf), (0, n - 10, 11, -np.inf),
+                         (0, n - 1, 127, np.nan), (1, 39, 0, np.inf), (1, 0, 0, np.inf)):
+        p.v[int(p.table[s, r // 16]), :, r % 16, d] = float(val)
+    with np.errstate(invalid="ignore"):
+        want, _, size = po.attention(f64(q), f64(p.k), f64(p.v), p.table.cpu().numpy(), p.lens_host, scale=128 ** -0.5)
+    got = attend(p, q, weight=p.weight)
+    odd = ~np.isfinite(want)
+    assert odd[0].sum(0).any() and np.array_equal(f64(got)[odd], want[odd], equal_nan=True)
+    want[odd], size[odd] = 0.0, 0.0
+    assert one_rounding(got.masked_fill(torch.from_numpy(odd).cuda(), 0), want, 2.0 ** -14 * size)
+
+
+@pytest.mark.parametrize("name", ["bf16", "fp16"])
+def test_attention_of_an_infinite_value_of_the_largest_and_of_a_small_weight(name):
+    """Weight 1 exactly, and 2^-20 exactly, leave nothing when they are cut to 16 bits; a score of -inf has no weight."""
+    p = Pool([3, 3], n_kv=1, page=16, dtype=DT[name], seed=6)
+    q = torch.zeros(2, 1, 128, dtype=DT[name], device="cuda")
+    q[..., 0] = 1.0
+    for s in range(2):
+        pg = int(p.table[s, 0])
+        p.k[pg, 0, :3] = 0.0
+        p.k[pg, 0, :3, 0] = torch.tensor([0.0, -20.0, -20.0], dtype=DT[name])
+        p.v[pg, 0, :3] = 1.0
+        p.v[pg, 0, 0, 0] = p.v[pg, 0, 1, 1] = float("inf")
+    got = attend(p, q, scale=float(np.log(2.0)))
+    assert torch.isinf(got[:, 0, :2]).all() and (got[:, 0, 2:] == 1).all()
+    p.k[int(p.table[0, 0]), 0, 0, 0] = float("-inf")  # its value is infinite: 0 * inf, as the formula
+    got = attend(p, q, scale=float(np.log(2.0)))
+    assert torch.isnan(got[0, 0, 0]) and torch.isinf(got[0, 0, 1]) and (got[0, 0, 2:] == 1).all()

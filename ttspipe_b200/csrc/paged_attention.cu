@@ -145,11 +145,26 @@ struct Parts {
 //
 // The weights exp(s - m) enter the second product in 16 bits. Rounded once, each
 // would be off by as much as the output's own rounding; so they enter twice, as the
-// rounded value and as what rounding left (the MMA units idle otherwise: memory bounds
-// this kernel), which leaves 2^-17. fp16 has no exponents for the small weights of
+// value cut to 16 bits and as what cutting left (the MMA units idle otherwise: memory bounds
+// this kernel), which leaves 2^-16. fp16 has no exponents for the small weights of
 // many rows next to one large one, so there they are lifted by 2^14 (exact).
+// An infinite value has to stay one: cut towards zero, both parts have the weight's sign, and
+// where nothing is left the second is kLeast (2^-38 or 2^-126 of the largest weight) instead of 0.
 template <bool F16>
 constexpr float kLift = F16 ? 14.f : 0.f;
+template <bool F16>
+constexpr float kLeast = F16 ? 0x1p-24f : 0x1p-126f;
+
+// Two fp32 numbers cut towards zero, `lo` in the low half.
+template <bool F16>
+__device__ __forceinline__ uint32_t cut_act2(float lo, float hi) {
+  uint32_t r;
+  if (F16)
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
 
 template <int NT>
 struct WarpState {
@@ -413,7 +428,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 && kWarps == 4 ? 3 : 1)
         }
       }
       if (next < t1) load_k(row);
-      uint32_t ph[NT][2], pl[NT][2];  // P^T as the B operand: the rounded weights and what rounding left
+      uint32_t ph[NT][2], pl[NT][2];  // P^T as the B operand: the cut weights and what cutting left
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float x[4];
@@ -450,8 +465,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 && kWarps == 4 ? 3 : 1)
         }
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-          ph[nt][n] = pack_act2<F16>(e[2 * n], e[2 * n + 1]);
-          pl[nt][n] = pack_act2<F16>(e[2 * n] - act_lo<F16>(ph[nt][n]), e[2 * n + 1] - act_hi<F16>(ph[nt][n]));
+          ph[nt][n] = cut_act2<F16>(e[2 * n], e[2 * n + 1]);
+          auto left = [](float w, float cut) { return w > 0.f ? fmaxf(w - cut, kLeast<F16>) : 0.f; };
+          pl[nt][n] = pack_act2<F16>(left(e[2 * n], act_lo<F16>(ph[nt][n])), left(e[2 * n + 1], act_hi<F16>(ph[nt][n])));
         }
       }
       if (!full) {  // 0 * NaN of an unwritten row is NaN
