@@ -55,6 +55,15 @@ def up_to_date() -> bool:
     return all(p.stat().st_mtime <= t for p in _deps())
 
 
+def _cxx_runtime() -> list[str]:
+    """The C++ runtime that this process's PyTorch runs on, to link the binding against. A compiler that has only
+    the static one would put a second copy into the binding; two of them in a process crash where one formats numbers
+    with the other's locale, as every refusal that names a shape does."""
+    with open("/proc/self/maps") as maps:
+        found = {line.split()[-1] for line in maps if "/libstdc++.so" in line}
+    return sorted(found)
+
+
 def build_binding(force: bool = False, verbose: bool = False) -> Path:
     """Compile the Python binding of the paged KV cache. Returns its path."""
     deps = [BIND_SRC, *INCLUDE.glob("*.h")]
@@ -74,7 +83,7 @@ def build_binding(force: bool = False, verbose: bool = False) -> Path:
     tmp = BIND.with_suffix(".so.tmp")
     cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{i}" for i in inc), str(BIND_SRC),
-           f"-L{home / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-o", str(tmp)]
+           f"-L{home / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10", *_cxx_runtime(), "-o", str(tmp)]
     if verbose:
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True, env=dict(os.environ, TMPDIR=str(BUILD)))
