@@ -5,6 +5,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -65,6 +66,12 @@ void* take_or_null(const char* name, PyObject* o, at::ScalarType type, at::IntAr
   return o == Py_None ? nullptr : take(name, o, type, shape, device);
 }
 
+// The kernels are launched on the current device's GPU, which cannot read another one's memory.
+void check_device(at::Device device, at::DeviceIndex current) {
+  TORCH_CHECK_VALUE(device.index() == current, "pools on ", device.str(), ", the current device is cuda:",
+                    static_cast<int>(current));
+}
+
 // A cache's description, after its checks.
 struct Cache {
   nf4b_paged_kv c;
@@ -78,6 +85,7 @@ struct Cache {
     device = k.device();
     TORCH_CHECK_VALUE((type == at::kBFloat16 || type == at::kHalf) && device.is_cuda(), "pools of ", type_text(type),
                       " on ", device.str(), " are not served");
+    check_device(device, c10::impl::VirtualGuardImpl(at::kCUDA).getDevice().index());
     TORCH_CHECK_VALUE(k.dim() == 4 && k.size(3) == kD && table.dim() == 2 && k.numel() > 0 && table.numel() > 0,
                       "pools [n_pages, n_kv, page_size, 128] and a table [n_seqs, max_pages] needed, got ",
                       shape_text(k.sizes()), " and ", shape_text(table.sizes()));
@@ -233,8 +241,20 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
+// (device index of the pools, current device index): the check that every call makes
+PyObject* check_device_of(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  HANDLE_TH_ERRORS
+  count(n_args, 2);
+  check_device(at::Device(at::kCUDA, static_cast<at::DeviceIndex>(int32("device", a[0]))),
+               static_cast<at::DeviceIndex>(int32("current", a[1])));
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind)), METH_FASTCALL, nullptr},
+    {"check_device", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(check_device_of)), METH_FASTCALL,
+     nullptr},
     {"write", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(write)), METH_FASTCALL, nullptr},
     {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(attention)), METH_FASTCALL, nullptr},
     {"evict", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(evict)), METH_FASTCALL, nullptr},

@@ -20,7 +20,7 @@ of them stay on the device and are read there, so a CUDA graph of a step serves
 every state of the cache. ``PagedKVCache`` holds the pools of all layers and hands
 out pages; ``decode_block`` is a transformer block's decode step for a batch of streams.
 
-A tensor of a wrong type, shape, layout or device is refused with ValueError,
+A tensor of a wrong type, shape, layout or device (all on the current one) is refused with ValueError,
 what the library refuses (head groups over 16, page sizes that are not a multiple of 16,
 ...) with ``Nf4bError``, in both cases before anything is launched.
 """
