@@ -145,26 +145,11 @@ struct Parts {
 //
 // The weights exp(s - m) enter the second product in 16 bits. Rounded once, each
 // would be off by as much as the output's own rounding; so they enter twice, as the
-// value cut to 16 bits and as what cutting left (the MMA units idle otherwise: memory bounds
-// this kernel), which leaves 2^-16. fp16 has no exponents for the small weights of
+// rounded value and as what rounding left (the MMA units idle otherwise: memory bounds
+// this kernel), which leaves 2^-17. fp16 has no exponents for the small weights of
 // many rows next to one large one, so there they are lifted by 2^14 (exact).
-// An infinite value has to stay one: cut towards zero, both parts have the weight's sign, and
-// where nothing is left the second is kLeast (2^-38 or 2^-126 of the largest weight) instead of 0.
 template <bool F16>
 constexpr float kLift = F16 ? 14.f : 0.f;
-template <bool F16>
-constexpr float kLeast = F16 ? 0x1p-24f : 0x1p-126f;
-
-// Two fp32 numbers cut towards zero, `lo` in the low half.
-template <bool F16>
-__device__ __forceinline__ uint32_t cut_act2(float lo, float hi) {
-  uint32_t r;
-  if (F16)
-    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  else
-    asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
 
 template <int NT>
 struct WarpState {
@@ -188,6 +173,11 @@ struct AttnShared {
   Join joins[2];  // what this CTA joins
   int n_joins, wide;
 };
+
+// Whether none of the four is infinite or NaN.
+__device__ __forceinline__ bool finite4(const float (&x)[4]) {
+  return (x[0] - x[0]) + (x[1] - x[1]) + ((x[2] - x[2]) + (x[3] - x[3])) == 0.f;
+}
 
 // The finished row of one query head, four dimensions to a lane.
 template <bool F16>
@@ -284,6 +274,49 @@ __device__ __forceinline__ void join_parts(const PagedAttnParams& p, const Join*
     }
     x = next;
   } while (x.n);
+}
+
+// An infinite value times the rest that rounding a weight left, which may be 0 or negative, is
+// NaN, so the sums of dimensions with such values are wrong. Where a part ends with sums that are
+// not finite under weights that are, a warp adds up the infinite and NaN values by themselves: of
+// query head `head` and tiles t0 to t1, four dimensions to a lane, those of rows of weight 0
+// (a score of -inf) as NaN, as 0 times them is. A dimension that has any gets that sum. Called, so that
+// its code is not in the way of calls without such values (1 x 2048 rows: 7.3 us, 7.5 inline).
+template <bool F16>
+__device__ __noinline__ void sum_infinities(const PagedAttnParams& p, int b, int h, int head, int t0, int t1,
+                                            float (&o)[4]) {
+  const int lane = threadIdx.x & 31, tpp = p.page_size / kTile, rows = seq_rows(p, b);
+  const int* table = p.table + (size_t)b * p.max_pages;
+  const uint8_t* mask = p.mask == nullptr ? nullptr : p.mask + (size_t)b * p.max_pages * p.page_size;
+  const uint2 q = reinterpret_cast<const uint2*>(p.q + ((size_t)b * p.n_head + (size_t)h * p.groups + head) * kD)[lane];
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+  for (int tile = t0; tile < t1; ++tile) {
+    const int pg = table[tile / tpp];
+    if (pg < 0 || pg >= p.n_pages) continue;
+    const size_t row = (((size_t)pg * p.n_kv + h) * p.page_size + (size_t)(tile % tpp) * kTile) * kD;
+    uint2 v[kTile];
+#pragma unroll
+    for (int r = 0; r < kTile; ++r) v[r] = reinterpret_cast<const uint2*>(p.v + row + r * kD)[lane];
+#pragma unroll
+    for (int r = 0; r < kTile; ++r) {
+      const float x[4] = {act_lo<F16>(v[r].x), act_hi<F16>(v[r].x), act_lo<F16>(v[r].y), act_hi<F16>(v[r].y)};
+      const int j = tile * kTile + r;
+      if (!__any_sync(0xffffffffu, !finite4(x)) || j >= rows || (mask != nullptr && mask[j] == 0)) continue;
+      const uint2 k = reinterpret_cast<const uint2*>(p.k + row + r * kD)[lane];
+      float s = act_lo<F16>(q.x) * act_lo<F16>(k.x) + act_hi<F16>(q.x) * act_hi<F16>(k.x) +
+                act_lo<F16>(q.y) * act_lo<F16>(k.y) + act_hi<F16>(q.y) * act_hi<F16>(k.y);
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+      const bool none = s * p.scale_log2 == -INFINITY;
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+        if (!(x[d] - x[d] == 0.f)) sum[d] += none ? NAN : x[d];
+    }
+  }
+#pragma unroll
+  for (int d = 0; d < 4; ++d)
+    if (sum[d] != 0.f) o[d] = sum[d];
 }
 
 template <int NT, int kWarps, bool F16>
@@ -428,7 +461,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 && kWarps == 4 ? 3 : 1)
         }
       }
       if (next < t1) load_k(row);
-      uint32_t ph[NT][2], pl[NT][2];  // P^T as the B operand: the cut weights and what cutting left
+      uint32_t ph[NT][2], pl[NT][2];  // P^T as the B operand: the rounded weights and what rounding left
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float x[4];
@@ -465,9 +498,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 && kWarps == 4 ? 3 : 1)
         }
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-          ph[nt][n] = cut_act2<F16>(e[2 * n], e[2 * n + 1]);
-          auto left = [](float w, float cut) { return w > 0.f ? fmaxf(w - cut, kLeast<F16>) : 0.f; };
-          pl[nt][n] = pack_act2<F16>(left(e[2 * n], act_lo<F16>(ph[nt][n])), left(e[2 * n + 1], act_hi<F16>(ph[nt][n])));
+          ph[nt][n] = pack_act2<F16>(e[2 * n], e[2 * n + 1]);
+          pl[nt][n] = pack_act2<F16>(e[2 * n] - act_lo<F16>(ph[nt][n]), e[2 * n + 1] - act_hi<F16>(ph[nt][n]));
         }
       }
       if (!full) {  // 0 * NaN of an unwritten row is NaN
@@ -536,6 +568,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 && kWarps == 4 ? 3 : 1)
         o[2] = fmaf(f, x.z, o[2]);
         o[3] = fmaf(f, x.w, o[3]);
       }
+      if (__any_sync(0xffffffffu, l == l && !finite4(o))) sum_infinities<F16>(p, b, h, head, t0, t1, o);
       if (whole) {
         store_out<F16>(p, head0 + head, lane, mu, l, o);
       } else {
