@@ -524,9 +524,14 @@ int nf4b_paged_write(const nf4b_paged_kv* cache, const void* qkv, const int32_t*
  * of its KV head) is added to it, in fp32; a page that several sequences share
  * receives all of theirs, in no fixed order. Otherwise results do not depend on
  * timing. out must not overlap an input. `workspace` (nf4b_paged_attention_workspace_size, tracked = whether
- * weight is given) is zeroed once before its first use and serves calls of any
- * sizes that fit it; calls that overlap on the GPU must not share one.
+ * weight is given) is zeroed once before its first use (its first
+ * NF4B_PAGED_COUNTER_BYTES are enough) and serves calls of any
+ * sizes that fit it; calls that overlap on the GPU must not share one. A captured
+ * graph uses the workspace of its capture at every replay: a graph that may
+ * run beside other calls needs one of its own.
  */
+#define NF4B_PAGED_COUNTER_BYTES 278528u
+
 int nf4b_paged_attention(const nf4b_paged_kv* cache, const void* q, const int32_t* lens, const uint8_t* mask,
                          float scale, void* out, int n_head, void* workspace, size_t workspace_bytes, void* stream);
 
@@ -551,6 +556,13 @@ int nf4b_paged_evict(const nf4b_paged_kv* cache, const int32_t* lens, int budget
                      size_t workspace_bytes, void* stream);
 
 size_t nf4b_paged_evict_workspace_size(int n_seqs, int n_kv, int max_pages, int page_size, int budget);
+
+/*
+ * The id of the capture that `stream` is part of, the same for all streams of
+ * one capture and for no other; 0 where it is not capturing. A host that
+ * keeps workspaces by stream gives each capture one of its own by it.
+ */
+unsigned long long nf4b_capture_id(void* stream);
 
 #ifdef __cplusplus
 }

@@ -5,6 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from tests.helpers import randn_bf16
 from tests.test_gpu_pagedkv import Pool
 from ttspipe_b200 import _lib, model, nf4gemv, pagedkv
 
@@ -72,3 +73,95 @@ def test_what_the_library_refuses_names_the_numbers():
     for call in a:  # as they are, they are served
         getattr(pagedkv, call)(**a[call])
     torch.cuda.synchronize()
+
+
+class Work:
+    """Attention of long sequences (joined from many parts), with weights, and an eviction of copies."""
+
+    def __init__(self, seed):
+        self.p = Pool([4000, 1, 2500, 3999], n_kv=8, page=64, dtype=torch.bfloat16, seed=seed)
+        self.p.position[self.p.table.clamp(min=0).long()] = 1
+        self.q = randn_bf16((4, 32, 128), seed=seed, device="cuda")
+        self.out, self.weight = torch.empty_like(self.q), torch.zeros_like(self.p.weight)
+        self.evicted = [torch.zeros_like(t) for t in (self.p.weight, self.p.position, self.p.lens)]
+        self.k, self.v = self.p.k.clone(), self.p.v.clone()
+
+    def run(self):
+        p = self.p
+        self.weight.zero_()
+        for _ in range(3):
+            pagedkv.attention(self.q, p.k, p.v, p.table, p.lens, weight=self.weight, out=self.out)
+        self.k.copy_(p.k), self.v.copy_(p.v)
+        pagedkv.evict(self.k, self.v, self.weight, p.position, p.table, p.lens, budget=1111, recent=0, sink=0,
+                      weight_out=self.evicted[0], position_out=self.evicted[1], lens_out=self.evicted[2])
+
+    def result(self):
+        torch.cuda.synchronize()
+        return [t.clone().view(torch.uint8) for t in (self.out, self.weight, self.k, self.v, *self.evicted)]
+
+
+def same(a, b):
+    return all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_a_capture_needs_no_warm_up():
+    """The usual form: on torch's own capture stream, where nothing of this kind has run."""
+    work = Work(1)
+    work.run()
+    want = work.result()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        work.run()
+    for t in (work.out, work.weight, *work.evicted):
+        t.zero_()
+    for _ in range(3):
+        graph.replay()
+        assert same(work.result(), want)
+    del graph
+
+
+def test_graphs_of_one_capture_stream_replay_side_by_side():
+    """Two graphs captured on one stream, replayed on two others, with calls on that stream in between."""
+    works = [Work(2), Work(3), Work(4)]
+    side, lanes = torch.cuda.Stream(), [torch.cuda.Stream() for _ in range(2)]
+    graphs, want = [torch.cuda.CUDAGraph() for _ in lanes], []
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for work in works:
+            work.run()
+            want.append(work.result())
+        for graph, work in zip(graphs, works):
+            with torch.cuda.graph(graph, stream=side):
+                work.run()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for _ in range(5):
+            for lane, graph in zip(lanes, graphs):
+                with torch.cuda.stream(lane):
+                    graph.replay()
+            with torch.cuda.stream(side):
+                works[2].run()
+        for work, w in zip(works, want):
+            assert same(work.result(), w)
+    del graphs
+
+
+def test_streams_of_one_capture_do_not_share_a_workspace():
+    works = [Work(5), Work(6)]
+    want = []
+    for work in works:
+        work.run()
+        want.append(work.result())
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        works[0].run()
+        with torch.cuda.stream(side):
+            works[1].run()
+        main.wait_stream(side)
+    for _ in range(20):
+        graph.replay()
+        for work, w in zip(works, want):
+            assert same(work.result(), w)
+    del graph

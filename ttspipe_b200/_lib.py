@@ -21,6 +21,8 @@ NF4B_ERR_ARG, NF4B_ERR_SHAPE, NF4B_ERR_ALIGN, NF4B_ERR_DTYPE = -1, -2, -3, -4
 NF4B_ERR_WORKSPACE, NF4B_ERR_LAUNCH, NF4B_ERR_DEVICE = -5, -6, -7
 NF4B_EPI_NONE, NF4B_EPI_RESIDUAL, NF4B_EPI_SILU_GATE = 0, 1, 2
 NF4B_F32, NF4B_F16, NF4B_BF16 = 0, 1, 2
+#: Of a paged attention's workspace, what has to be zero before its first use.
+PAGED_COUNTER_BYTES = 278528
 
 
 def act_type(dtype):
@@ -70,6 +72,7 @@ EXPORTS = (
     "nf4b_paged_attention_workspace_size",
     "nf4b_paged_evict",
     "nf4b_paged_evict_workspace_size",
+    "nf4b_capture_id",
 )
 
 
@@ -186,6 +189,7 @@ def _declare(lib) -> None:
         "nf4b_paged_attention_workspace_size": (sz, [i32, i32, i32, i32, i32, i32]),
         "nf4b_paged_evict": (i32, [pp, vp, i32, i32, i32, vp, vp, vp, vp, sz, vp]),
         "nf4b_paged_evict_workspace_size": (sz, [i32, i32, i32, i32, i32]),
+        "nf4b_capture_id": (ctypes.c_ulonglong, [vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

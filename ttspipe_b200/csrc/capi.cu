@@ -1017,6 +1017,7 @@ int check_paged_heads(int n_head, int n_kv) {
 }
 
 int check_workspace(const void* workspace, size_t given, size_t need) {
+  static_assert(PAGED_COUNTER_BYTES == NF4B_PAGED_COUNTER_BYTES, "the header's figure");
   if (workspace == nullptr || given < need)
     return fail(NF4B_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace ? given : (size_t)0);
   if (!aligned(workspace, 256)) return fail(NF4B_ERR_ALIGN, "workspace is not 256-byte aligned");
@@ -1133,6 +1134,16 @@ int nf4b_paged_attention(const nf4b_paged_kv* cache, const void* q, const int32_
   p.weight = cache->weight;
   return launch_status(launch_paged_attention(p, plan.grid, sms, f16, reinterpret_cast<cudaStream_t>(stream)),
                        "paged attention launch");
+}
+
+unsigned long long nf4b_capture_id(void* stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(reinterpret_cast<cudaStream_t>(stream), &status, &id) != cudaSuccess) {
+    cudaGetLastError();  // the default stream while another one captures: not part of it
+    return 0;
+  }
+  return status == cudaStreamCaptureStatusNone ? 0 : id;
 }
 
 size_t nf4b_paged_evict_workspace_size(int n_seqs, int n_kv, int max_pages, int page_size, int budget) {

@@ -20,6 +20,7 @@ namespace {
 decltype(&nf4b_paged_write) g_write = nullptr;
 decltype(&nf4b_paged_attention) g_attention = nullptr;
 decltype(&nf4b_paged_evict) g_evict = nullptr;
+decltype(&nf4b_capture_id) g_capture_id = nullptr;
 
 constexpr int64_t kD = 128;
 
@@ -137,6 +138,13 @@ at::Tensor fresh(at::IntArrayRef shape, at::ScalarType type, at::Device device) 
   return at::Tensor(at::detail::empty_cuda(shape, type, device, std::nullopt));
 }
 
+// Whether a workspace made in the capture `id` (0: in none) is this call's: calls that are captured keep to their
+// capture's own, or graphs that are replayed side by side would share one. The default stream is never captured.
+bool own_workspace(PyObject* workspace, PyObject* id, void* stream) {
+  return workspace == Py_None || stream == nullptr ||
+         g_capture_id(stream) == static_cast<unsigned long long>(integer(id));
+}
+
 // The output tensor where the call succeeded, else the library's status.
 PyObject* answer(int status, const at::Tensor& out, PyObject* given) {
   if (status != NF4B_OK) return PyLong_FromLong(status);
@@ -182,10 +190,10 @@ PyObject* write(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   END_HANDLE_TH_ERRORS
 }
 
-// (q, k, v, block_table, lens, mask, scale, weight, out, workspace, workspace_bytes, stream)
+// (q, k, v, block_table, lens, mask, scale, weight, out, workspace, workspace_bytes, its capture, stream)
 PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
-  count(n_args, 12);
+  count(n_args, 13);
   Cache cache(a[1], a[2], a[3], a[7], Py_None);
   const at::Tensor& q = tensor("q", a[0]);
   const int64_t n = cache.c.n_seqs;
@@ -202,18 +210,19 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   }
   const at::Tensor out = a[8] == Py_None ? fresh(q.sizes(), cache.type, d) : tensor("out", a[8]);
   void* o = take("out", out, cache.type, q.sizes(), d);
+  if (!own_workspace(a[9], a[11], address(a[12]))) return PyLong_FromLong(NF4B_ERR_WORKSPACE);
   const int status = g_attention(&cache.c, x, static_cast<int32_t*>(lens), static_cast<uint8_t*>(mask),
                                  (float)number(a[6]), o, (int)q.size(1), address(a[9]), (size_t)integer(a[10]),
-                                 address(a[11]));
+                                 address(a[12]));
   return answer(status, out, a[8]);
   END_HANDLE_TH_ERRORS
 }
 
 // (k, v, weight, position, block_table, lens, budget, recent, sink, weight_out, position_out, lens_out, workspace,
-//  workspace_bytes, stream)
+//  workspace_bytes, its capture, stream)
 PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
-  count(n_args, 15);
+  count(n_args, 16);
   Cache cache(a[0], a[1], a[4], a[2], a[3]);
   const auto& d = cache.device;
   const int64_t n = cache.c.n_seqs;
@@ -222,20 +231,22 @@ PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   void* position = take("position_out", a[10], at::kInt, cache.slots, d);
   const at::Tensor& out = tensor("lens_out", a[11]);
   void* o = take("lens_out", out, at::kInt, {n}, d);
+  if (!own_workspace(a[12], a[14], address(a[15]))) return PyLong_FromLong(NF4B_ERR_WORKSPACE);
   const int status = g_evict(&cache.c, static_cast<int32_t*>(lens), int32("budget", a[6]), int32("recent", a[7]),
                              int32("sink", a[8]), static_cast<float*>(weight), static_cast<int32_t*>(position),
-                             static_cast<int32_t*>(o), address(a[12]), (size_t)integer(a[13]), address(a[14]));
+                             static_cast<int32_t*>(o), address(a[12]), (size_t)integer(a[13]), address(a[15]));
   return answer(status, out, a[11]);
   END_HANDLE_TH_ERRORS
 }
 
-// (addresses of nf4b_paged_write, nf4b_paged_attention, nf4b_paged_evict)
+// (addresses of nf4b_paged_write, nf4b_paged_attention, nf4b_paged_evict, nf4b_capture_id)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   HANDLE_TH_ERRORS
-  count(n_args, 3);
+  count(n_args, 4);
   g_write = reinterpret_cast<decltype(g_write)>(address(a[0]));
   g_attention = reinterpret_cast<decltype(g_attention)>(address(a[1]));
   g_evict = reinterpret_cast<decltype(g_evict)>(address(a[2]));
+  g_capture_id = reinterpret_cast<decltype(g_capture_id)>(address(a[3]));
   if (PyErr_Occurred()) throw python_error();
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS

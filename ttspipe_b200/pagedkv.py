@@ -35,8 +35,11 @@ from ttspipe_b200 import _lib
 
 HEAD_DIM = 128
 _stats = {"write": 0, "attention": 0, "evict": 0, "block": 0}
-_workspaces: dict = {}  # (kind, device, stream): (tensor, address, bytes); calls on other streams may overlap
-_retired: list = []  # replaced workspaces: a captured graph may still name them
+# (kind, device, stream): (tensor, address, bytes, capture); calls on other streams may overlap, and so may a captured
+# graph's replays: those of a capture (its id, 0 for none) are the capture's own, from its graph's memory
+_NONE = (None, None, 0, 0)
+_workspaces: dict = {}
+_captured: dict = {}  # of the latest capture on each stream, to be dropped once it is over
 _native = None
 
 #: The current stream's handle, without the Stream object (2 us a call) torch.cuda.current_stream makes.
@@ -53,8 +56,8 @@ def _bound():
             from ttspipe_b200 import _pagedkv
         except ImportError as exc:
             raise RuntimeError("_pagedkv.so is not built; run `python -m ttspipe_b200.build`") from exc
-        _pagedkv.bind(*(ctypes.cast(getattr(lib, f"nf4b_paged_{name}"), ctypes.c_void_p).value
-                        for name in ("write", "attention", "evict")))
+        _pagedkv.bind(*(ctypes.cast(getattr(lib, f"nf4b_{name}"), ctypes.c_void_p).value
+                        for name in ("paged_write", "paged_attention", "paged_evict", "capture_id")))
         _native = _pagedkv
     return _native
 
@@ -63,15 +66,26 @@ def stats() -> dict:
     return dict(_stats)
 
 
-def _grow(kind: str, device, stream: int, need: int):
-    """A larger zeroed workspace for a device and stream, outside graph capture only."""
-    if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError(f"paged {kind} workspace must be sized before graph capture")
-    old = _workspaces.get((kind, device, stream))
-    if old is not None:
-        _retired.append(old[0])
-    ws = torch.zeros(max(need, 2 * old[2] if old else 1 << 20), dtype=torch.uint8, device=torch.device("cuda", device))
-    got = _workspaces[(kind, device, stream)] = (ws, ws.data_ptr(), ws.numel())
+def _capture_id(stream: int) -> int:
+    return _lib.lib().nf4b_capture_id(stream)
+
+
+def _empty(size: int, device: int):
+    return torch.empty(size, dtype=torch.uint8, device=torch.device("cuda", device))
+
+
+def _workspace(kind: str, device: int, stream: int, need: int):
+    """The workspace of a call that the stream's usual one does not serve: a larger one for the stream, or, in a
+    graph capture, the capture's own. What has to be zero in a new one is zeroed (in a capture, by every replay)."""
+    key, capture = (kind, device, stream), _capture_id(stream)
+    kept = _captured if capture else _workspaces
+    got = kept.get(key, _NONE)
+    if got[3] != capture or got[2] < need:
+        size = need if capture else max(need, 2 * got[2], 1 << 20)
+        ws = _empty(size, device)
+        if kind == "attention":
+            ws[:_lib.PAGED_COUNTER_BYTES].zero_()
+        got = kept[key] = (ws, ws.data_ptr(), size, capture)
     return got
 
 
@@ -109,16 +123,18 @@ def attention(q, k, v, block_table, lens, *, mask=None, scale: float | None = No
     call, dev = (_native or _bound()).attention, k.get_device()
     stream = _stream(dev) if dev >= 0 else 0
     scale = HEAD_DIM ** -0.5 if scale is None else scale
-    _, ws, size = _workspaces.get(("attention", dev, stream)) or (None, None, 0)
-    got = call(q, k, v, block_table, lens, mask, scale, weight, out, ws, size, stream)
+    _, ws, size, capture = _workspaces.get(("attention", dev, stream), _NONE)
+    got = call(q, k, v, block_table, lens, mask, scale, weight, out, ws, size, capture, stream)
     if type(got) is int:
         if got != _lib.NF4B_ERR_WORKSPACE:
             _raise(got)
-        _, ws, size = _grow("attention", dev, stream, _lib.lib().nf4b_paged_attention_workspace_size(
+        _, ws, size, capture = _workspace("attention", dev, stream, _lib.lib().nf4b_paged_attention_workspace_size(
             q.shape[0], q.shape[1], k.shape[1], block_table.shape[1], k.shape[2], weight is not None))
-        got = call(q, k, v, block_table, lens, mask, scale, weight, out, ws, size, stream)
+        got = call(q, k, v, block_table, lens, mask, scale, weight, out, ws, size, capture, stream)
         if type(got) is int:
             _raise(got)
+    elif _captured:
+        _captured.clear()
     _stats["attention"] += 1
     return got
 
@@ -141,16 +157,18 @@ def evict(k, v, weight, position, block_table, lens, *, budget: int, recent: int
     args = (k, v, weight, position, block_table, lens, budget, recent, sink,
             weight if weight_out is None else weight_out, position if position_out is None else position_out,
             lens if lens_out is None else lens_out)
-    _, ws, size = _workspaces.get(("evict", dev, stream)) or (None, None, 0)
-    got = call(*args, ws, size, stream)
+    _, ws, size, capture = _workspaces.get(("evict", dev, stream), _NONE)
+    got = call(*args, ws, size, capture, stream)
     if type(got) is int:
         if got != _lib.NF4B_ERR_WORKSPACE:
             _raise(got)
-        _, ws, size = _grow("evict", dev, stream, _lib.lib().nf4b_paged_evict_workspace_size(
+        _, ws, size, capture = _workspace("evict", dev, stream, _lib.lib().nf4b_paged_evict_workspace_size(
             block_table.shape[0], k.shape[1], block_table.shape[1], k.shape[2], budget))
-        got = call(*args, ws, size, stream)
+        got = call(*args, ws, size, capture, stream)
         if type(got) is int:
             _raise(got)
+    elif _captured:
+        _captured.clear()
     _stats["evict"] += 1
     return got
 
