@@ -5,13 +5,16 @@ Each ``csrc/*.cu`` is compiled separately (in parallel) with
 next to this file, so it travels with the source tree. The CUDA runtime is
 linked statically: the library carries its own runtime and shares only the
 driver (and therefore the current context and streams) with the PyTorch that
-calls it. ``csrc/pagedkv_bind.cpp`` becomes ``_pagedkv.so`` beside it, a Python
-module against this PyTorch's headers. ``python -m ttspipe_b200.build`` rebuilds
-when a source is newer than what was built from it.
+calls it. ``csrc/pagedkv_bind.cpp`` then becomes ``_pagedkv.so`` beside it, a Python
+module against this PyTorch's headers; the library needs neither it nor PyTorch.
+``python -m ttspipe_b200.build`` rebuilds when a source is newer than what was built
+from it, and the binding also for another PyTorch, Python or compiler.
 """
 
 from __future__ import annotations
 
+import importlib.metadata
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -66,16 +69,18 @@ def _cxx_runtime() -> list[str]:
 
 def build_binding(force: bool = False, verbose: bool = False) -> Path:
     """Compile the Python binding of the paged KV cache. Returns its path."""
-    deps = [BIND_SRC, *INCLUDE.glob("*.h")]
-    if not force and BIND.exists() and all(p.stat().st_mtime <= BIND.stat().st_mtime for p in deps):
+    cxx = os.environ.get("CXX") or shutil.which("g++")
+    deps, stamp = [BIND_SRC, *INCLUDE.glob("*.h")], BUILD / "pagedkv_bind.txt"
+    made_for = f"{importlib.metadata.version('torch')} {sys.version} {cxx}"
+    if (not force and BIND.exists() and all(p.stat().st_mtime <= BIND.stat().st_mtime for p in deps)
+            and stamp.exists() and (not cxx or stamp.read_text() == made_for)):
         return BIND
+    if not cxx:
+        raise FileNotFoundError("no C++ compiler (set CXX or install g++)")
     import sysconfig
 
     import torch
 
-    cxx = os.environ.get("CXX") or shutil.which("g++")
-    if not cxx:
-        raise FileNotFoundError("no C++ compiler (set CXX or install g++)")
     BUILD.mkdir(exist_ok=True)
     home = Path(torch.__file__).resolve().parent
     inc = [INCLUDE, home / "include", home / "include" / "torch" / "csrc" / "api" / "include",
@@ -90,12 +95,23 @@ def build_binding(force: bool = False, verbose: bool = False) -> Path:
     if r.returncode != 0:
         raise RuntimeError(f"{cxx} failed on {BIND_SRC.name}:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, BIND)
+    stamp.write_text(made_for)
     return BIND
 
 
 def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> Path:
-    """Compile the binding and every kernel source and link the shared library. Returns its path."""
-    build_binding(force=force, verbose=verbose)
+    """Compile every kernel source and link the shared library, then the binding (not where there is no PyTorch).
+    Returns the library's path."""
+    build_library(force=force, verbose=verbose, ptxas_info=ptxas_info)
+    if importlib.util.find_spec("torch") is None:
+        print("no PyTorch: the paged cache's Python binding is left out", file=sys.stderr)
+    else:
+        build_binding(force=force, verbose=verbose)
+    return LIB
+
+
+def build_library(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> Path:
+    """Compile every kernel source and link the shared library. Returns its path."""
     if not force and up_to_date() and not ptxas_info:
         return LIB
     BUILD.mkdir(exist_ok=True)

@@ -55,7 +55,10 @@ def _bound():
         try:
             from ttspipe_b200 import _pagedkv
         except ImportError as exc:
-            raise RuntimeError("_pagedkv.so is not built; run `python -m ttspipe_b200.build`") from exc
+            from ttspipe_b200 import build
+
+            why = f"does not load ({exc})" if build.BIND.exists() else "is not built"
+            raise RuntimeError(f"_pagedkv.so {why}; run `python -m ttspipe_b200.build`") from exc
         _pagedkv.bind(*(ctypes.cast(getattr(lib, f"nf4b_{name}"), ctypes.c_void_p).value
                         for name in ("paged_write", "paged_attention", "paged_evict", "capture_id")))
         _native = _pagedkv
