@@ -184,3 +184,20 @@ def test_positions_past_the_rotary_table_are_passed_over(captured):
         assert cache.next_pos.tolist() == [40, 0] and cache.part.tolist() == [0, 0]
         del graph
     torch.cuda.synchronize()
+
+
+def test_steps_of_streams_reserved_together():
+    """The host runs ahead: each step goes by the reservations made before it, none by a later one."""
+    cache = pagedkv.PagedKVCache(1, 4, 256, 64, 2, page_size=16, device="cuda", track=False)
+    g = torch.Generator().manual_seed(3)
+    parts, seen = [], []
+    torch.cuda._sleep(int(2e8))
+    for _ in range(100):
+        seqs = [s for s in range(4) if torch.rand((), generator=g) < 0.5]
+        cache.reserve(seqs)
+        cache.begin_step()
+        cache.end_step()
+        parts.append([int(s in seqs) for s in range(4)])
+        seen.append(cache.part.clone())
+    assert torch.stack(seen).tolist() == parts
+    assert cache.lens.tolist() == [sum(p[s] for p in parts) for s in range(4)]

@@ -314,3 +314,40 @@ def test_prefill_refuses_positions_outside_the_rotary_table(rows, position):
     cache.reserve(0, 5, prompt=True)
     with pytest.raises(ValueError, match="rotary"):
         pagedkv.prefill_block(blk, torch.randn(1, 5, DIM), FREQS[:6], cache, 0, 0, rows=rows, position=position)
+
+
+def test_streams_reserved_together_are_reserved_as_one_after_the_other():
+    caches = [make_cache(4, track=False) for _ in range(2)]
+    rng = torch.Generator().manual_seed(9)
+    for t in range(30):
+        seqs = [s for s in range(4) if torch.rand((), generator=rng) < 0.6]
+        rows = 1 + t % 2
+        try:
+            caches[0].reserve(seqs, rows)
+        except RuntimeError:
+            break
+        for s in seqs:
+            caches[1].reserve(s, rows)
+        for c in caches:
+            c.begin_step()
+            c.end_step()
+        for name in ("lens", "next_pos", "active", "block_table", "part", "rows", "_below", "_at"):
+            assert torch.equal(getattr(caches[0], name), getattr(caches[1], name)), name
+        assert caches[0]._pages == caches[1]._pages and caches[0]._rows == caches[1]._rows
+    assert t > 10 and caches[0].free_pages() < 3
+
+
+def test_a_joint_reservation_that_does_not_fit_changes_nothing():
+    c = make_cache(4, track=False)
+    c.reserve([0, 2], 30)
+    state = [c.block_table.clone(), c._below.clone(), list(c._rows), list(c._free)]
+    for seqs, rows, error, match in (([1, 3, 0], 33, RuntimeError, "stream 3 needs 3 pages, 1 are free"),
+                                     ([1, 0], 35, ValueError, "stream 0: at most 64"), ([1, 1], 1, ValueError, "twice"),
+                                     ([1, 2], -1, ValueError, "at most")):
+        with pytest.raises(error, match=match):
+            c.reserve(seqs, rows)
+        assert torch.equal(c.block_table, state[0]) and torch.equal(c._below, state[1])
+        assert c._rows == state[2] and c._free == state[3]
+    c.reserve([], 5)
+    c.reserve(range(4))
+    assert c._rows == [31, 1, 31, 1]
