@@ -999,7 +999,7 @@ int check_paged(const nf4b_paged_kv* c, bool* f16) {
     return fail(NF4B_ERR_SHAPE, "page size %d is not a multiple of %d", c->page_size, PAGED_TILE);
   if (c->n_pages <= 0 || c->max_pages <= 0 || (long long)c->max_pages * c->page_size >= (1LL << 30) ||
       (long long)c->n_seqs * c->n_kv * ((long long)c->max_pages * (c->page_size / PAGED_TILE) + PAGED_SEQ_TILES) >=
-          (1LL << 31))
+          (1LL << 31) - PAGED_MAX_STEP)
     return fail(NF4B_ERR_SHAPE, "%d pages, %d of %d rows for each sequence", c->n_pages, c->max_pages, c->page_size);
   if (!aligned(c->k, 16) || !aligned(c->v, 16)) return fail(NF4B_ERR_ALIGN, "pools not 16-byte aligned");
   if ((long long)c->n_pages * c->n_kv * c->page_size >= (1LL << 31))

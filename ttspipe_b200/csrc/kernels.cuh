@@ -395,6 +395,8 @@ constexpr int PAGED_MIN_TILES = 8;
 // Units that a (sequence, head) costs besides its tiles (32 ragged sequences of up to 4096
 // rows: 56 us with 0, 47 with 4, 42 with 8, 44 with 24).
 constexpr int PAGED_SEQ_TILES = 8;
+// Units that a kernel may step past the last one before it compares: all units, and these, fit 31 bits.
+constexpr int PAGED_MAX_STEP = 64;
 constexpr int PAGED_MAX_SEQS = 4096;  // sequences of one call (their tile counts lie in shared memory)
 constexpr int PAGED_MAX_GROUPS = 16;
 constexpr int PAGED_MAX_LISTS = 65535;  // (sequence, KV head) pairs of one call
