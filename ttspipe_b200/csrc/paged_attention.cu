@@ -284,8 +284,8 @@ __device__ __forceinline__ void join_parts(const PagedAttnParams& p, const Join*
 // its code is not in the way of calls without such values (1 x 2048 rows: 7.3 us, 7.5 inline). With
 // one such value a page 64 x 8192 rows take 1.3 ms instead of 0.32, with one in every row 3.5.
 template <bool F16>
-__device__ __noinline__ void sum_infinities(const PagedAttnParams& p, int b, int h, int head, int t0, int t1,
-                                            float (&o)[4]) {
+__device__ __noinline__ float4 sum_infinities(const PagedAttnParams& p, int b, int h, int head, int t0, int t1,
+                                              float4 o) {
   constexpr int kRows = 4;  // of a tile at a time, where it has any; few registers, which are the caller's too
   const int lane = threadIdx.x & 31, tpp = p.page_size / kTile, rows = seq_rows(p, b);
   const int* table = p.table + (size_t)b * p.max_pages;
@@ -340,9 +340,8 @@ __device__ __noinline__ void sum_infinities(const PagedAttnParams& p, int b, int
       }
     }
   }
-#pragma unroll
-  for (int d = 0; d < 4; ++d)
-    if (sum[d] != 0.f) o[d] = sum[d];
+  return make_float4(sum[0] != 0.f ? sum[0] : o.x, sum[1] != 0.f ? sum[1] : o.y, sum[2] != 0.f ? sum[2] : o.z,
+                     sum[3] != 0.f ? sum[3] : o.w);
 }
 
 template <int NT, int kWarps, bool F16>
@@ -594,7 +593,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 && kWarps == 4 ? 3 : 1)
         o[2] = fmaf(f, x.z, o[2]);
         o[3] = fmaf(f, x.w, o[3]);
       }
-      if (__any_sync(0xffffffffu, l == l && !finite4(o))) sum_infinities<F16>(p, b, h, head, t0, t1, o);
+      if (__any_sync(0xffffffffu, l == l && !finite4(o))) {
+        const float4 x = sum_infinities<F16>(p, b, h, head, t0, t1, make_float4(o[0], o[1], o[2], o[3]));
+        o[0] = x.x, o[1] = x.y, o[2] = x.z, o[3] = x.w;
+      }
       if (whole) {
         store_out<F16>(p, head0 + head, lane, mu, l, o);
       } else {
