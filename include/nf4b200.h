@@ -475,8 +475,8 @@ int nf4b_qkv_attention_ex(const void* qkv, const void* q_norm_w, const void* k_n
  *                all tokens since the row was written; NULL where it is not kept
  *   position     int32 [n_pages, n_kv, page_size]: each row's token position; or NULL
  * page_size is a multiple of 16, n_seqs at most 4096, n_seqs * n_kv at most 65535;
- * the pools are below 2^31 rows and a sequence's capacity max_pages * page_size
- * below 2^30. weight and position are 16-byte aligned, other int32 arrays 4-byte.
+ * the pools are below 2^31 rows, a sequence's capacity max_pages * page_size
+ * below 2^30 and n_seqs * n_kv * (max_pages * page_size / 16 + 8) below 2^31 - 64. weight and position are 16-byte aligned, other int32 arrays 4-byte.
  * Lengths, rows and tables are read on the device, so a captured graph serves every
  * state of the cache.
  */
@@ -496,7 +496,8 @@ typedef struct nf4b_paged_kv {
 
 /*
  * n_tokens tokens enter their pages: nf4b_qk_rope_kv (optional q/k norm, rotary,
- * the same rounding points, so rows have the same bits as in a dense cache) for
+ * the same rounding points, so rows have the same bits as in a dense cache; the
+ * norm's fp64 sum is taken in another order, which the rounding to fp32 hides) for
  * every token of qkv [n_tokens, n_head + 2 n_kv, 128], with the rotary row
  * freqs[positions[t]] of a table of freqs_rows rows and the cache row rows[t] of
  * sequence seqs[t] (seqs NULL: sequence t). Writes q_out [n_tokens, n_head, 128],
@@ -517,7 +518,8 @@ int nf4b_paged_write(const nf4b_paged_kv* cache, const void* qkv, const int32_t*
  * 128] over rows [0, lens[s]) of sequence s (lens is brought into [0, capacity]),
  * out [n_seqs, n_head, 128] = softmax(scale q k^T) v, one rounding at the end.
  * Rows whose `mask` byte (uint8 [n_seqs, max_pages * page_size], NULL = all
- * visible) is 0 take no part, whatever their pages hold. A sequence without a
+ * visible) is 0 take no part, whatever their pages hold; infinities and NaN in the
+ * others count as the formula has them. A sequence without a
  * visible row, or whose scores are all -inf, gets zeros. Query head h reads KV head
  * h / (n_head / n_kv); up to 16 query heads to a KV head.
  * With cache->weight every visible row's weight (the sum over the query heads

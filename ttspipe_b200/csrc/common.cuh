@@ -181,7 +181,7 @@ __device__ __forceinline__ float rsqrt_exact(double ss, int width, float eps) {
 
 // RMS-normalise the M rows of K bf16 values staged at xr (shared memory) in
 // place with weight w, with the arithmetic of nf4b_rms_norm: fp64 sum of
-// squares (exact for bf16 inputs, so its order does not matter),
+// squares (each exact; the order of their sum shows past its 53rd bit at most),
 // r = 1 / sqrt(fp32(ss / K) + eps), y = bf16(bf16(x * r) * w). Called by every
 // thread of the CTA after a barrier that made x visible; ends with a barrier.
 // `red` holds one double per warp. Row m starts at element m * row_stride

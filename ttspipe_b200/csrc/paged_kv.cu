@@ -17,9 +17,10 @@ constexpr int kD = 128;
 // takes kGroups times 2 kPairs heads of one token, so that the rotary row and the page are
 // had once for all of them and the norm's reciprocal square root (fp64, one lane a head) once
 // for each 2 kPairs. The arithmetic is
-// qk_rope_kv_kernel's, rounding point for rounding point (the norm's sum of squares in
-// fp64 is exact in any order), so a row in a page has the bits it would have in a
-// dense cache. 8188 tokens of 48 heads (202 MB) take 41 us with norm, 35 without: 4.9 and
+// qk_rope_kv_kernel's, rounding point for rounding point, so a row in a page has the bits it
+// would have in a dense cache. (The norm's squares are exact in fp64. Their sum is taken in
+// another order, which makes a difference past its 53rd bit at most, where values of a head are
+// far apart, and is then rounded to 24: it shows for about one such head in 2^26.) 8188 tokens of 48 heads (202 MB) take 41 us with norm, 35 without: 4.9 and
 // 5.8 TB/s, the norm bound by instruction issue (61% of all slots); one token 1.9 us, the launch.
 constexpr int kWriteWarps = 4;
 
@@ -221,9 +222,9 @@ __global__ void __launch_bounds__(kWriteWarps * 32, kPairs == 4 ? 7 : 1)
 //
 // paged_select_kernel, one CTA or one cluster of CTAs a list, finds the smallest kept key
 // digit by digit from the top (11, 11 and 10 bits, a histogram each) and lists the moves;
-// paged_move_kernel makes them. 8 x 32768 rows halved (64 lists, 562 MB) take 134 us:
-// about 30 to select, a chain of dependent steps (read, newest, three histograms, two
-// counts), and 104 to move some 524,000 rows, 256 bytes of key and of value each between
+// paged_move_kernel makes them. 8 x 32768 rows halved (64 lists, 562 MB) take 130 us:
+// about 27 to select, a chain of dependent steps (read, newest, three histograms, two
+// counts), and 103 to move some 524,000 rows, 256 bytes of key and of value each between
 // scattered places, at 5.2 TB/s of DRAM. 1 x 2048 rows are the chain alone, 9 us.
 constexpr int kBins = 2048;
 
@@ -755,8 +756,8 @@ cudaError_t launch_paged_evict(const PagedEvictParams& p, int sms, cudaStream_t 
   const int lists = p.n_seqs * p.n_kv, cap = p.max_pages * p.page_size;
   // Lists of up to 4096 rows: 8 rows to each of 256 or 512 threads (1 x 4096: 10.3 us, 12.7 with 16
   // rows). Longer ones: 1024 threads with 8 rows, in clusters of up to 8 CTAs, while every list's cluster
-  // has SMs of its own (1 x 32768: 29 us, 34 with 16 rows); else 16 rows (8 x 32768: 134 us, 145
-  // with 8), up to 8192 of them to 512 threads (32 x 8192: 127 us, 139 with 1024). Past 131072
+  // has SMs of its own (1 x 32768: 29 us, 34 with 16 rows); else 16 rows (8 x 32768: 130 us, 11
+  // more with 8), up to 8192 of them to 512 threads (32 x 8192: 127 us, 139 with 1024). Past 131072
   // rows a cluster of 8 reads its list several times.
   auto cluster_for = [&](int rows) {
     int c = 1;

@@ -23,6 +23,11 @@ out pages; ``decode_block`` is a transformer block's decode step for a batch of 
 A tensor of a wrong type, shape, layout or device (all on the current one) is refused with ValueError,
 what the library refuses (head groups over 16, page sizes that are not a multiple of 16,
 ...) with ``Nf4bError``, in both cases before anything is launched.
+
+Workspaces: one for each stream, grown as calls need it, by capacity (max_pages * page_size) and not
+by length: a tracked attention takes 4 * n_head bytes a row. A captured graph has its own, from its own memory,
+so captures need no warm-up here and graphs may be replayed side by side; the linears of
+``decode_block`` share one workspace a device (``nf4gemv``), so steps of blocks may not.
 """
 
 from __future__ import annotations
@@ -120,7 +125,7 @@ def attention(q, k, v, block_table, lens, *, mask=None, scale: float | None = No
     128], over its rows [0, lens[s]); returns [n_seqs, n_head, 128] of q's type.
 
     `mask` (bool or uint8 [n_seqs, max_pages * page_size], True = visible) hides rows,
-    whatever they hold; a sequence that sees none gets zeros. `scale` defaults to
+    whatever they hold; a sequence that sees none gets zeros. `out` must not overlap an input. `scale` defaults to
     128 ** -0.5. `weight` receives every visible row's weight, summed over the query
     heads of its KV head. Up to 16 query heads to a KV head."""
     call, dev = (_native or _bound()).attention, k.get_device()
@@ -427,7 +432,11 @@ def prefill_block(block, x, freqs, cache: PagedKVCache, layer: int, seq: int, ro
     cache after its `rows` rows, from token position `position` on (both on the host;
     ``reserve`` T rows with ``prompt`` first, and ``prefilled`` after the last layer).
     Each attends to the rows before it and to itself, by the grouped torch formulation
-    of ``fastpath``; weights are not accumulated here."""
+    of ``fastpath``: over copies of the stream's rows, with its roundings of scores and
+    probabilities to the activation type, which ``attention`` does not make, and
+    n_head x T x rows of scores. Weights are not accumulated here: a prompt's rows start with
+    weight 0 and gather it from the tokens decoded after it, so an eviction that comes soon
+    keeps mostly the lowest of them, besides `sink` and `recent`."""
     from ttspipe_b200 import fastpath, nf4gemv
 
     a, n = block.attention, x.shape[1]
