@@ -351,3 +351,46 @@ def test_a_joint_reservation_that_does_not_fit_changes_nothing():
     c.reserve([], 5)
     c.reserve(range(4))
     assert c._rows == [31, 1, 31, 1]
+
+
+def test_only_a_steps_own_table_bounds_its_positions():
+    """Rows written with positions of one's own, from part of the table, say nothing about the steps."""
+    blk, cache = make_block(), make_cache()
+    at = torch.arange(5, dtype=torch.int32)
+    cache.reserve(0, 5, prompt=True)
+    cache.write(0, torch.randn(5, (HEADS + 2 * KV) * 128), at, at, FREQS[:5], n_head=HEADS, seqs=torch.zeros_like(at))
+    cache.prefilled(0, 5)
+    cache.reserve([0, 1])
+    step(blk, cache, torch.randn(2, 1, DIM))
+    assert cache.part.tolist() == [1, 1] and cache.lens.tolist() == [6, 1]
+
+
+def test_a_longer_rotary_table_lets_streams_go_on():
+    blk, cache = make_block(), make_cache()
+    cache.reserve([0, 1], 20)
+
+    def steps(n, table):
+        for _ in range(n):
+            cache.begin_step()
+            pagedkv.decode_block(blk, torch.randn(2, 1, DIM), table, cache, 0)
+            cache.end_step()
+
+    steps(8, FREQS[:6])
+    assert cache.lens.tolist() == [6, 6]
+    steps(4, FREQS)
+    assert cache.lens.tolist() == [10, 10] and cache.next_pos.tolist() == [10, 10]
+    steps(2, FREQS[:7])
+    assert cache.lens.tolist() == [10, 10]
+
+
+def test_a_prompt_that_fills_the_rotary_table_is_not_stepped_past():
+    """The cache learns of the table with the step's first layer, and the step goes by it all the same."""
+    blk, cache = make_block(), make_cache()
+    cache.reserve(0, 6, prompt=True)
+    cache.prefilled(0, 6)
+    cache.reserve([0, 1])
+    before = held_by(cache, 0)
+    cache.begin_step()
+    pagedkv.decode_block(blk, torch.randn(2, 1, DIM), FREQS[:6], cache, 0)
+    cache.end_step()
+    assert unchanged(cache, 0, before) and cache.part.tolist() == [0, 1] and cache.lens.tolist() == [6, 1]

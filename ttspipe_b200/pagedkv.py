@@ -215,8 +215,9 @@ class PagedKVCache:
         self.lens = self._at[0]                       # rows of each stream
         self.next_pos = self._at[1]                   # position of its next token
         self.active = self._below[2]                  # 1: takes part in the steps that it has rows for
-        self._positions = self._step_positions = 2**31 - 1  # rows of the shortest rotary table seen, in this step
-        self._below[1] = self._positions
+        self._below[1] = 2**31 - 1
+        self._positions = None       # what _below[1] is set to, where the host knows
+        self._step_positions = None  # rows of the shortest rotary table of this step so far
         self._promised = self._below[0].unbind()
         self.part = torch.zeros(n_seqs, **i32)        # of a step: 1 for each stream that takes part
         self.rows = torch.full((n_seqs,), -1, **i32)  # of a step: the new row of each stream, -1 for none
@@ -309,7 +310,10 @@ class PagedKVCache:
     def begin_step(self) -> None:
         """Rows and lengths of one new token of each stream that takes part; the others have no row and length 0, so
         that nothing is written for them, attended to or weighed."""
-        self._step_positions = 2**31 - 1
+        self._step_positions = None
+        self._take_part()
+
+    def _take_part(self) -> None:
         torch.lt(self._at, self._below, out=self._is_below)
         torch.amin(self._is_below, 0, out=self.part)
         torch.addcmul(self.part, self.part, self.lens, out=self.live)
@@ -318,15 +322,25 @@ class PagedKVCache:
     def end_step(self) -> None:
         self._at[:2].add_(self.part)
 
+    def _bound_positions(self, n: int) -> None:
+        """A step's rotary table has `n` rows: streams whose next position is past it take no part, in this step
+        if its first layer says so, else (another layer's table is shorter) from the next one on."""
+        first = self._step_positions is None
+        if not first and n >= self._step_positions:
+            return
+        self._step_positions = n
+        known, captured = self._positions == n, self.lens.is_cuda and torch.cuda.is_current_stream_capturing()
+        if known and not captured:
+            return
+        self._below[1].fill_(n)  # by every replay too: steps with another table may run in between
+        self._positions = None if captured else n
+        if first and not known:
+            self._take_part()
+
     def write(self, layer: int, qkv, rows, positions, freqs, *, n_head: int, **kw):
-        """``write`` into one layer's pools. The first call with a rotary table (or a shorter one) bounds the positions
-        of later steps by it."""
-        n = freqs.shape[0]
-        if n < self._positions and n < self._step_positions:
-            self._below[1].fill_(n)
-            self._step_positions = n
-            if not (self.lens.is_cuda and torch.cuda.is_current_stream_capturing()):  # else only the replays set it
-                self._positions = n
+        """``write`` into one layer's pools; of a step's tokens where `positions` is ``next_pos``."""
+        if positions is self.next_pos:
+            self._bound_positions(freqs.shape[0])
         return write(qkv, self.k[layer], self.v[layer], self.block_table, rows, positions, freqs, n_head=n_head,
                      weight=self.weight[layer], position=self.position[layer], **kw)
 
